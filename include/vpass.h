@@ -346,6 +346,84 @@ int vp_step_graph(vp_ctx* ctx, vp_drafter* d, int32_t B, int32_t branch, vp_grap
 int vp_graph_launch(vp_graph* g, void* stream);
 void vp_graph_destroy(vp_graph* g);
 
+/* ---- paged key-value cache: many requests over one pool of pages ----
+ * No counterpart in the reference, which serves one request over one contiguous cache
+ * (Engine.swift:113, :922). A cache layer is two pools, K and V, of pages of page_size slots, and a
+ * table that names the pages of each request in order: slot j of request s, head h, element d is at
+ *   table[s * table_stride + j / page_size] * page_stride + h * head_stride + (j % page_size) * slot_stride + d
+ * (elements; the same strides for both pools). The caller owns all of it. Work runs on the current
+ * device and `stream`, allocates nothing and synchronises nothing, and may be captured in a graph.
+ *   limits  type VP_T_F16 or VP_T_BF16; head_dim 64 or 128; page_size 16, 32, 64, 128 or 256; pools
+ *           16-byte aligned, their strides positive multiples of 8 elements below 2^39.
+ * Entries of the table are read only where a request's slots use them. What the device finds wrong
+ * is told in *status (device int32, may be NULL; bits are OR'ed in and never cleared), not by a
+ * fault: VP_DEV_ERR_PAGE a page outside [0, n_pages), read as zeros and not written;
+ * VP_DEV_ERR_SLOT a request, slot, position or length outside the table (or the rotations), dropped
+ * or clipped. Slots at or past a request's length, and slots that no row of a call sees, may hold
+ * anything, NaN included. */
+enum vp_type { VP_T_F16 = 0, VP_T_BF16 = 1, VP_T_F32 = 2 };
+#define VP_DEV_ERR_PAGE 16
+#define VP_DEV_ERR_SLOT 32
+typedef struct {
+  void* k;
+  void* v;
+  const int32_t* table;  /* [n_seqs][max_pages], rows table_stride apart */
+  int32_t* status;
+  int64_t page_stride, head_stride, slot_stride, table_stride;
+  int32_t type, n_kv, head_dim, page_size, n_pages, n_seqs, max_pages;
+} vp_paged;
+
+/* New rows join the cache: row t's keys, rotated to pos[t], and values go to slot[t] of request
+ * seq[t] (seq[t] < 0: a padding row, not stored), its queries, rotated, to q_out. The rotation is
+ * read from rope, fp32 [rope_rows][rot_dim / 2] (cos, sin) pairs: elements (i, i + rot_dim / 2) of a
+ * head turn by rope[pos][i], or (2i, 2i + 1) when interleaved; elements from rot_dim on are copied.
+ * Arithmetic is fp32, rounded once to the cache's type. Two rows of one call must not share a slot.
+ *   q, k, v  [rows][heads][head_dim] of `type` (the cache's type, or VP_T_F32), rows and heads
+ *            *_row and *_head elements apart (multiples of 8; 4 for VP_T_F32), 16-byte aligned: parts
+ *            of one fused projection will do. q_out has the cache's type; it may be q itself.
+ *   limits   rot_dim 0 or a multiple of 16, at most head_dim. */
+typedef struct {
+  const void *q, *k, *v;
+  void* q_out;
+  const int32_t *seq, *slot, *pos;
+  const float* rope;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+  int32_t type, rows, n_q, rope_rows, rot_dim, interleaved;
+} vp_paged_rows;
+int vp_paged_append(const vp_paged* c, const vp_paged_rows* r, void* stream);
+
+/* Attention over the cache: out = softmax(scale q K^T) V over the slots that a row sees, per query
+ * head (head h reads cache head h / (n_q / n_kv)); lse, if not NULL, its log sum exp (natural). A row
+ * that sees nothing gives zeros and -inf. Scores, softmax statistics and sums are fp32.
+ * vp_paged_decode: the newest rows of n requests, `rows` (1..16) each, which are the last slots of
+ *   lens[i]: q and out [n][rows][n_q][head_dim], lse [n][rows][n_q]. Row r sees every slot before the
+ *   new ones, and new slot j if bit j of mask[i * rows + r] is set (NULL: j <= r), so a draft tree is
+ *   verified with its ancestor bitmasks (the row's own bit included). Its position is the number of
+ *   old slots plus its set bits minus one.
+ * vp_paged_prefill: prompt rows of n requests, ragged: rows q_start[i] .. q_start[i + 1] - 1 of q and
+ *   out [rows][n_q][head_dim] (lse [rows][n_q]) are the last slots of lens[i], each seeing the slots up
+ *   to its own (all of them new, or a chunk over a cached prefix).
+ * window > 0: a row at position p sees a slot at position j only if p - j < window or j < sinks.
+ * seqs (NULL: i) names request i's row of the table. Rows before a request's first slot (more rows
+ * than its length) see nothing. Strides as above; lse is dense. work: vp_paged_work_bytes(...) bytes,
+ * 256-byte aligned, zeroed once before its first use (each call leaves it ready for the next); calls
+ * that share it must not overlap on the GPU. Results depend on the inputs alone, not on timing.
+ *   limits   n_q a multiple of n_kv, n_q / n_kv <= 64; sinks >= 0, window >= 0. */
+typedef struct {
+  const void* q;
+  void* out;
+  float* lse;
+  const int32_t *lens, *seqs, *mask, *q_start;
+  void* work;
+  uint64_t work_bytes;
+  int64_t q_seq, q_row, q_head, out_seq, out_row, out_head;
+  float scale;
+  int32_t n, rows, n_q, window, sinks;
+} vp_paged_attn;
+size_t vp_paged_work_bytes(int32_t head_dim, int32_t n_q, int32_t n_kv, int32_t rows);
+int vp_paged_decode(const vp_paged* c, const vp_paged_attn* a, void* stream);
+int vp_paged_prefill(const vp_paged* c, const vp_paged_attn* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -24,6 +24,7 @@ EXPORTS = (
     "vp_sketch_bytes", "vp_pack_sketch", "vp_sketch_work_bytes", "vp_sketch_bounds_offset",
     "vp_head_argmax_sketch", "vp_drafter_create", "vp_drafter_destroy", "vp_drafter_begin", "vp_draft",
     "vp_pass_graph", "vp_step_graph", "vp_graph_launch", "vp_graph_destroy",
+    "vp_paged_append", "vp_paged_work_bytes", "vp_paged_decode", "vp_paged_prefill",
 )
 
 
@@ -49,6 +50,26 @@ _ARR = _P * MAX_LAYERS
 class VpWeights(ctypes.Structure):
     _fields_ = [("embed", _P), ("final_norm", _P), ("wqkv", _ARR), ("bqkv", _ARR), ("wo", _ARR),
                 ("wgu", _ARR), ("wd", _ARR), ("ln1", _ARR), ("ln2", _ARR)]
+
+
+class VpPaged(ctypes.Structure):
+    _fields_ = ([(n, _P) for n in ("k", "v", "table", "status")]
+                + [(n, ctypes.c_int64) for n in ("page_stride", "head_stride", "slot_stride", "table_stride")]
+                + [(n, ctypes.c_int32) for n in ("type", "n_kv", "head_dim", "page_size", "n_pages", "n_seqs", "max_pages")])
+
+
+class VpPagedRows(ctypes.Structure):
+    _fields_ = ([(n, _P) for n in ("q", "k", "v", "q_out", "seq", "slot", "pos", "rope")]
+                + [(n, ctypes.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "out_row", "out_head")]
+                + [(n, ctypes.c_int32) for n in ("type", "rows", "n_q", "rope_rows", "rot_dim", "interleaved")])
+
+
+class VpPagedAttn(ctypes.Structure):
+    _fields_ = ([(n, _P) for n in ("q", "out", "lse", "lens", "seqs", "mask", "q_start", "work")]
+                + [("work_bytes", ctypes.c_uint64)]
+                + [(n, ctypes.c_int64) for n in ("q_seq", "q_row", "q_head", "out_seq", "out_row", "out_head")]
+                + [("scale", ctypes.c_float)]
+                + [(n, ctypes.c_int32) for n in ("n", "rows", "n_q", "window", "sinks")])
 
 
 class VpError(RuntimeError):
@@ -110,6 +131,10 @@ def load(path: os.PathLike | None = None) -> ctypes.CDLL:
         "vp_step_graph": (ctypes.c_int, [vp, vp, i32, i32, ctypes.POINTER(vp)]),
         "vp_graph_launch": (ctypes.c_int, [vp, vp]),
         "vp_graph_destroy": (None, [vp]),
+        "vp_paged_append": (ctypes.c_int, [vp, vp, vp]),
+        "vp_paged_work_bytes": (sz, [i32, i32, i32, i32]),
+        "vp_paged_decode": (ctypes.c_int, [vp, vp, vp]),
+        "vp_paged_prefill": (ctypes.c_int, [vp, vp, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

@@ -7,7 +7,7 @@ from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
-SOURCES = [PKG / "csrc" / "vpass.cu", PKG / "csrc" / "vpdraft.cu"]
+SOURCES = [PKG / "csrc" / "vpass.cu", PKG / "csrc" / "vpdraft.cu", PKG / "csrc" / "vppaged.cu"]
 HEADERS = sorted((PKG / "csrc").glob("*.cuh")) + [ROOT / "include" / "vpass.h"]
 OUT = PKG / "libvpass.so"
 # the trace build (performance work only): the same kernels with %globaltimer stamps at every stage

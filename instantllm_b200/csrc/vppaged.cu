@@ -1,0 +1,340 @@
+// Paged key-value cache operators (include/vpass.h, vp_paged_*): appending rotated rows, attention of
+// the newest rows of many requests, attention of prompts.
+#include <cuda_runtime.h>
+
+#include <exception>
+#include <string>
+
+#include "vp_paged.cuh"
+
+using namespace vp;
+
+void vp_set_last_error(const std::string& msg);
+
+namespace vp {
+
+// ---- append ----
+// One CTA per row, HD / 16 threads per head: each turns two runs of 8 elements (or copies 16), so a
+// thread keeps its 8 (cos, sin) pairs in registers over the heads it serves. 16-byte accesses.
+// Bytes bound it: each row is read and written once.
+constexpr int APPEND_THREADS = 128;
+
+template <typename TI>
+__device__ __forceinline__ void load8(const TI* p, float (&x)[8]) {
+  const uint4 w = *reinterpret_cast<const uint4*>(p);
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = PgType<TI>::up(u[i]);
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  uint4 w;
+  w.x = PgType<T>::down(x[0], x[1]);
+  w.y = PgType<T>::down(x[2], x[3]);
+  w.z = PgType<T>::down(x[4], x[5]);
+  w.w = PgType<T>::down(x[6], x[7]);
+  *reinterpret_cast<uint4*>(p) = w;
+}
+
+template <typename TI, typename T, int HD>
+__global__ void __launch_bounds__(APPEND_THREADS) k_paged_append(const vp_paged c, const vp_paged_rows r) {
+  constexpr int J = HD / 16;
+  const long long t = blockIdx.x;
+  const int j = threadIdx.x % J;
+  const int seq = r.seq[t], slot = r.slot[t];
+  const int pos = r.rot_dim ? r.pos[t] : 0;
+  const bool turns = 16 * j < r.rot_dim;
+  const bool pos_ok = !r.rot_dim || (pos >= 0 && pos < r.rope_rows);
+  // runs a and b of the head: the two halves of 8 rotation pairs, or 16 elements in a row
+  const bool half = turns && !r.interleaved;
+  const int da = half ? 8 * j : 16 * j, db = half ? r.rot_dim / 2 + 8 * j : 16 * j + 8;
+  float cs[8], sn[8];
+  if (turns && pos_ok) {
+    const float4* p = reinterpret_cast<const float4*>(r.rope + ((long long)pos * (r.rot_dim / 2) + 8 * j) * 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 f = __ldg(p + i);
+      cs[2 * i] = f.x, sn[2 * i] = f.y, cs[2 * i + 1] = f.z, sn[2 * i + 1] = f.w;
+    }
+  }
+  bool keep = seq >= 0 && pos_ok;
+  long long at = 0;
+  if (seq >= 0) {
+    bool ok = seq < c.n_seqs && slot >= 0 && slot / c.page_size < c.max_pages;
+    int page = -1;
+    if (ok) page = c.table[seq * c.table_stride + slot / c.page_size];
+    const bool page_ok = page >= 0 && page < c.n_pages;
+    if (threadIdx.x == 0 && !(ok && page_ok && pos_ok))
+      pg_status(c.status, !ok || !pos_ok ? VP_DEV_ERR_SLOT : VP_DEV_ERR_PAGE);
+    keep = keep && ok && page_ok;
+    at = (long long)page * c.page_stride + (long long)(slot % c.page_size) * c.slot_stride;
+  } else if (threadIdx.x == 0 && !pos_ok) {
+    pg_status(c.status, VP_DEV_ERR_SLOT);
+  }
+  const int heads = r.n_q + 2 * c.n_kv, step = blockDim.x / J;
+#pragma unroll 4
+  for (int h = threadIdx.x / J; h < heads; h += step) {
+    const bool is_q = h < r.n_q, is_v = h >= r.n_q + c.n_kv;
+    const int hh = is_q ? h : is_v ? h - r.n_q - c.n_kv : h - r.n_q;
+    if (!is_q && !keep) continue;
+    const TI* src = is_q ? static_cast<const TI*>(r.q) + t * r.q_row + hh * r.q_head
+                  : is_v ? static_cast<const TI*>(r.v) + t * r.v_row + hh * r.v_head
+                         : static_cast<const TI*>(r.k) + t * r.k_row + hh * r.k_head;
+    T* dst = is_q ? static_cast<T*>(r.q_out) + t * r.out_row + hh * r.out_head
+                  : static_cast<T*>(is_v ? c.v : c.k) + at + hh * c.head_stride;
+    float a[8], b[8];
+    if (is_v) {
+      load8<TI>(src + 16 * j, a);
+      load8<TI>(src + 16 * j + 8, b);
+      store8<T>(dst + 16 * j, a);
+      store8<T>(dst + 16 * j + 8, b);
+      continue;
+    }
+    load8<TI>(src + da, a);
+    load8<TI>(src + db, b);
+    if (!pos_ok) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+    } else if (half) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = a[i], y = b[i];
+        a[i] = x * cs[i] - y * sn[i];
+        b[i] = y * cs[i] + x * sn[i];
+      }
+    } else if (turns) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], w = b[2 * i + 1];
+        a[2 * i] = x * cs[i] - y * sn[i];
+        a[2 * i + 1] = y * cs[i] + x * sn[i];
+        b[2 * i] = z * cs[4 + i] - w * sn[4 + i];
+        b[2 * i + 1] = w * cs[4 + i] + z * sn[4 + i];
+      }
+    }
+    store8<T>(dst + da, a);
+    store8<T>(dst + db, b);
+  }
+}
+
+// ---- attention, one warp per row and query head ----
+// The running maximum and sum of the softmax over 32 slots at a time: lane i scores slot i, then
+// every lane adds the 32 weighted values of its own HD / 32 elements.
+template <typename T, int HD, bool PROMPT>
+__global__ void k_paged_attn(const vp_paged c, const vp_paged_attn a) {
+  constexpr int E = HD / 32;
+  const int lane = threadIdx.x & 31;
+  const long long w = blockIdx.x * (long long)(blockDim.x / 32) + threadIdx.x / 32;
+  const int h = (int)(w % a.n_q);
+  const long long row = w / a.n_q;
+  int i, r, n_new;
+  if (PROMPT) {
+    if (row >= a.rows) return;
+    i = 0;
+    while (i < a.n && a.q_start[i + 1] <= row) ++i;
+    if (i == a.n || a.q_start[i] > row) return;
+    r = (int)row - a.q_start[i];
+    n_new = a.q_start[i + 1] - a.q_start[i];
+  } else {
+    if (row >= (long long)a.n * a.rows) return;
+    i = (int)(row / a.rows);
+    r = (int)(row % a.rows);
+    n_new = a.rows;
+  }
+  const PgSeq s = pg_seq(c, a.seqs, a.lens, i);
+  const int base = s.len - n_new;
+  uint32_t anc[PROMPT ? 1 : PG_MAX_ROWS] = {};
+  uint32_t bits = 0;
+  if (!PROMPT) {
+    for (int t = 0; t < n_new; ++t) {
+      anc[t] = a.mask ? (uint32_t)a.mask[(long long)i * n_new + t] & ((1u << n_new) - 1) : (2u << t) - 1;
+      if (t == r) bits = anc[t];
+    }
+  }
+  const int end = base + r < 0 ? 0 : PROMPT ? base + r + 1 : s.len;
+  const int at = PROMPT ? base + r : 0;
+  const T* q = static_cast<const T*>(a.q) + (PROMPT ? row * a.q_row : i * a.q_seq + r * a.q_row) + h * a.q_head;
+  const int hk = h / (a.n_q / c.n_kv);
+  float m = -INFINITY, l = 0.f, o[E] = {};
+  for (int j0 = 0; j0 < end; j0 += 32) {
+    const int j = j0 + lane;
+    bool see = j < end;
+    if (see) see = PROMPT ? !a.window || at - j < a.window || j < a.sinks
+                          : pg_sees(j, s.len, base, bits, anc, a.window, a.sinks);
+    float sc = -INFINITY;
+    int page = -1;
+    if (see) {
+      page = s.pages[j / c.page_size];
+      if (page < 0 || page >= c.n_pages) pg_status(c.status, VP_DEV_ERR_PAGE), page = -1;
+      sc = 0.f;
+      if (page >= 0) {
+        const T* k = static_cast<const T*>(c.k) + page * c.page_stride + hk * c.head_stride + (j % c.page_size) * c.slot_stride;
+        for (int d = 0; d < HD; ++d) sc += (float)q[d] * (float)k[d];
+      }
+      sc *= a.scale;
+    }
+    const float mn = fmaxf(m, warp_max(sc));
+    if (mn == -INFINITY) continue;
+    const float f = expf(m - mn), p = expf(sc - mn);
+    l = l * f + warp_sum(p);
+    m = mn;
+    for (int e = 0; e < E; ++e) o[e] *= f;
+    for (int t = 0; t < 32; ++t) {
+      const float pt = __shfl_sync(0xffffffffu, p, t);
+      const int pg = __shfl_sync(0xffffffffu, see ? page : -1, t);
+      if (pg < 0) continue;
+      const T* v = static_cast<const T*>(c.v) + pg * c.page_stride + hk * c.head_stride + ((j0 + t) % c.page_size) * c.slot_stride;
+      for (int e = 0; e < E; ++e) o[e] += pt * (float)v[lane + 32 * e];
+    }
+  }
+  T* out = static_cast<T*>(a.out) + (PROMPT ? row * a.out_row : i * a.out_seq + r * a.out_row) + h * a.out_head;
+  for (int e = 0; e < E; ++e) out[lane + 32 * e] = (T)(l > 0.f ? o[e] / l : 0.f);
+  if (a.lse && lane == 0) a.lse[row * a.n_q + h] = l > 0.f ? m + logf(l) : -INFINITY;
+}
+
+}  // namespace vp
+
+namespace {
+
+int pfail(int code, const char* msg) {
+  vp_set_last_error(msg);
+  return code;
+}
+int launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return VP_OK;
+  vp_set_last_error(std::string(what) + ": " + cudaGetErrorString(e));
+  return VP_ERR_CUDA;
+}
+
+bool off16(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
+
+int check_cache(const vp_paged* c) {
+  if (!c) return pfail(VP_ERR_ARG, "null cache");
+  if (c->type != VP_T_F16 && c->type != VP_T_BF16) return pfail(VP_ERR_ARG, "the cache's type must be f16 or bf16");
+  if (c->head_dim != 64 && c->head_dim != 128) return pfail(VP_ERR_ARG, "head_dim must be 64 or 128");
+  if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
+    return pfail(VP_ERR_ARG, "page_size must be 16, 32, 64, 128 or 256");
+  if (c->n_kv < 1 || c->n_kv > 4096) return pfail(VP_ERR_ARG, "n_kv out of range");
+  if (c->n_pages < 1 || c->n_seqs < 0 || c->max_pages < 1 || (long long)c->max_pages * c->page_size > (1 << 30))
+    return pfail(VP_ERR_ARG, "n_pages, n_seqs or max_pages out of range");
+  if (!c->k || !c->v || !c->table) return pfail(VP_ERR_ARG, "null pool or table");
+  if (off16(c->k) || off16(c->v)) return pfail(VP_ERR_ARG, "pools must be 16-byte aligned");
+  const int64_t s[3] = {c->page_stride, c->head_stride, c->slot_stride};
+  for (int64_t x : s)
+    if (x <= 0 || x % 8 || x >= (1ll << 39)) return pfail(VP_ERR_ARG, "pool strides must be positive multiples of 8 elements below 2^39");
+  if (c->table_stride < c->max_pages) return pfail(VP_ERR_ARG, "table_stride below max_pages");
+  return VP_OK;
+}
+
+bool bad_strides(int64_t a, int64_t b, int unit) { return a % unit || b % unit; }
+
+template <typename TI, typename T>
+void append_launch(const vp_paged& c, const vp_paged_rows& r, cudaStream_t st) {
+  const int want = (r.n_q + 2 * c.n_kv) * (c.head_dim / 16);
+  const int threads = want < APPEND_THREADS ? (want + 31) / 32 * 32 : APPEND_THREADS;
+  if (c.head_dim == 64) k_paged_append<TI, T, 64><<<r.rows, threads, 0, st>>>(c, r);
+  else k_paged_append<TI, T, 128><<<r.rows, threads, 0, st>>>(c, r);
+}
+
+int check_attn(const vp_paged* c, const vp_paged_attn* a) {
+  if (const int e = check_cache(c)) return e;
+  if (!a) return pfail(VP_ERR_ARG, "null arguments");
+  if (a->n < 0 || a->rows < 0 || a->n > (1 << 24)) return pfail(VP_ERR_ARG, "n or rows out of range");
+  if (a->n_q < 1 || a->n_q % c->n_kv) return pfail(VP_ERR_ARG, "n_q must be a multiple of n_kv");
+  if (a->n_q / c->n_kv > PG_MAX_GROUP) return pfail(VP_ERR_ARG, "more than 64 query heads per cache head");
+  if (a->window < 0 || a->sinks < 0) return pfail(VP_ERR_ARG, "window and sinks must not be negative");
+  if (!(a->scale > 0.f && a->scale < 3e38f)) return pfail(VP_ERR_ARG, "scale must be positive and finite");
+  if (a->n == 0 || a->rows == 0) return VP_OK;
+  if (!a->q || !a->out || !a->lens) return pfail(VP_ERR_ARG, "null q, out or lens");
+  if (off16(a->q) || off16(a->out)) return pfail(VP_ERR_ARG, "q and out must be 16-byte aligned");
+  if (bad_strides(a->q_row, a->q_head, 8) || bad_strides(a->out_row, a->out_head, 8) ||
+      bad_strides(a->q_seq, a->out_seq, 8))
+    return pfail(VP_ERR_ARG, "strides of q and out must be multiples of 8 elements");
+  if (!a->work || (reinterpret_cast<uintptr_t>(a->work) & 255)) return pfail(VP_ERR_ARG, "work must be 256-byte aligned");
+  if (a->work_bytes < vp_paged_work_bytes(c->head_dim, a->n_q, c->n_kv, a->rows < PG_MAX_ROWS ? a->rows : PG_MAX_ROWS))
+    return pfail(VP_ERR_ARG, "work is smaller than vp_paged_work_bytes");
+  return VP_OK;
+}
+
+template <typename T, bool PROMPT>
+void attn_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
+  const long long warps = (long long)(PROMPT ? 1 : a.n) * a.rows * a.n_q;
+  const unsigned grid = (unsigned)((warps + 3) / 4);
+  if (c.head_dim == 64) k_paged_attn<T, 64, PROMPT><<<grid, 128, 0, st>>>(c, a);
+  else k_paged_attn<T, 128, PROMPT><<<grid, 128, 0, st>>>(c, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int vp_paged_append(const vp_paged* c, const vp_paged_rows* r, void* stream) try {
+  if (const int e = check_cache(c)) return e;
+  if (!r) return pfail(VP_ERR_ARG, "null rows");
+  if (r->type != c->type && r->type != VP_T_F32) return pfail(VP_ERR_ARG, "rows must have the cache's type or f32");
+  if (r->rows < 0 || r->n_q < 1 || r->n_q > 4096) return pfail(VP_ERR_ARG, "rows or n_q out of range");
+  if (r->rot_dim < 0 || r->rot_dim % 16 || r->rot_dim > c->head_dim)
+    return pfail(VP_ERR_ARG, "rot_dim must be a multiple of 16, at most head_dim");
+  if (r->rot_dim && r->rope_rows < 1) return pfail(VP_ERR_ARG, "empty rotation table");
+  if (r->rows == 0) return VP_OK;
+  if (!r->q || !r->k || !r->v || !r->q_out || !r->seq || !r->slot) return pfail(VP_ERR_ARG, "null buffer");
+  if (r->rot_dim && (!r->pos || !r->rope || off16(r->rope))) return pfail(VP_ERR_ARG, "null or unaligned pos or rope");
+  if (off16(r->q) || off16(r->k) || off16(r->v) || off16(r->q_out)) return pfail(VP_ERR_ARG, "rows must be 16-byte aligned");
+  const int unit = r->type == VP_T_F32 ? 4 : 8;
+  if (bad_strides(r->q_row, r->q_head, unit) || bad_strides(r->k_row, r->k_head, unit) ||
+      bad_strides(r->v_row, r->v_head, unit) || bad_strides(r->out_row, r->out_head, 8))
+    return pfail(VP_ERR_ARG, "strides of rows must be multiples of 16 bytes");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (c->type == VP_T_F16) {
+    if (r->type == VP_T_F32) append_launch<float, __half>(*c, *r, st);
+    else append_launch<__half, __half>(*c, *r, st);
+  } else {
+    if (r->type == VP_T_F32) append_launch<float, __nv_bfloat16>(*c, *r, st);
+    else append_launch<__nv_bfloat16, __nv_bfloat16>(*c, *r, st);
+  }
+  return launched("vp_paged_append");
+} catch (const std::exception&) {
+  return VP_ERR_NOMEM;
+}
+
+size_t vp_paged_work_bytes(int32_t head_dim, int32_t n_q, int32_t n_kv, int32_t rows) {
+  if ((head_dim != 64 && head_dim != 128) || n_kv < 1 || n_q < 1 || n_q % n_kv || n_q / n_kv > PG_MAX_GROUP || rows < 1)
+    return 0;
+  return 256;
+}
+
+int vp_paged_decode(const vp_paged* c, const vp_paged_attn* a, void* stream) try {
+  if (const int e = check_attn(c, a)) return e;
+  if (a->rows > PG_MAX_ROWS) return pfail(VP_ERR_ARG, "a decode call takes 1 to 16 rows per request");
+  if (a->n == 0 || a->rows == 0) return VP_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (c->type == VP_T_F16) attn_launch<__half, false>(*c, *a, st);
+  else attn_launch<__nv_bfloat16, false>(*c, *a, st);
+  return launched("vp_paged_decode");
+} catch (const std::exception&) {
+  return VP_ERR_NOMEM;
+}
+
+int vp_paged_prefill(const vp_paged* c, const vp_paged_attn* a, void* stream) try {
+  if (const int e = check_attn(c, a)) return e;
+  if (a->n == 0 || a->rows == 0) return VP_OK;
+  if (!a->q_start) return pfail(VP_ERR_ARG, "null q_start");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (c->type == VP_T_F16) attn_launch<__half, true>(*c, *a, st);
+  else attn_launch<__nv_bfloat16, true>(*c, *a, st);
+  return launched("vp_paged_prefill");
+} catch (const std::exception&) {
+  return VP_ERR_NOMEM;
+}
+
+}  // extern "C"

@@ -1,0 +1,595 @@
+"""The paged key-value cache (include/vpass.h, vp_paged_*; instantllm_b200/paged.py) against the 64-bit oracle: rows
+joining the cache with their rotation, attention of the newest rows, attention of prompts; sizes, masks and layouts at which
+they can go wrong; refusals.
+
+Tolerances. u is half a unit in the last place of the cache's type (2^-11 fp16, 2^-8 bf16: 11 and 8 significant bits). A rotated element is rounded
+once from fp32: u |y| plus 4 ulp of the fp32 products. An attention output rounds its weights (u p each, or half of fp16's
+smallest step 2^-24 below its normal range) and itself (u |o|); a score summed over head_dim products in fp32 is off by at most
+head_dim 2^-23 sum |q k| scale, which moves a weight by that share, as the exponential's own error (2^-20) does."""
+import ctypes
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from instantllm_b200 import _lib, build, paged
+from oracle import paged as O
+
+U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+# ------------------------------------------------------------------------------------------------
+# host side (no GPU)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build.build()
+    return _lib.load()
+
+
+def good_cache(**kw):
+    c = dict(k=4096, v=8192, table=256, status=None, page_stride=2 * 64 * 64, head_stride=64 * 64, slot_stride=64,
+             table_stride=4, type=0, n_kv=2, head_dim=64, page_size=64, n_pages=8, n_seqs=2, max_pages=4)
+    c.update(kw)
+    return _lib.VpPaged(**c)
+
+
+def good_attn(**kw):
+    a = dict(q=4096, out=8192, lse=None, lens=256, seqs=None, mask=None, q_start=512, work=1 << 20, work_bytes=1 << 30,
+             q_seq=896, q_row=896, q_head=64, out_seq=896, out_row=896, out_head=64, scale=0.125, n=1, rows=1, n_q=14,
+             window=0, sinks=0)
+    a.update(kw)
+    return _lib.VpPagedAttn(**a)
+
+
+def good_rows(**kw):
+    r = dict(q=4096, k=8192, v=12288, q_out=16384, seq=256, slot=512, pos=768, rope=1024, q_row=896, q_head=64, k_row=128,
+             k_head=64, v_row=128, v_head=64, out_row=896, out_head=64, type=0, rows=1, n_q=14, rope_rows=16, rot_dim=64,
+             interleaved=0)
+    r.update(kw)
+    return _lib.VpPagedRows(**r)
+
+
+BAD_CACHE = [dict(type=2), dict(type=7), dict(head_dim=96), dict(head_dim=32), dict(page_size=48), dict(page_size=8),
+             dict(page_size=512), dict(n_kv=0), dict(n_pages=0), dict(max_pages=0), dict(k=None), dict(v=4104), dict(table=None),
+             dict(page_stride=0), dict(head_stride=-64), dict(slot_stride=66), dict(page_stride=1 << 40), dict(table_stride=3),
+             dict(max_pages=1 << 28, table_stride=1 << 28)]
+BAD_ATTN = [dict(n=-1), dict(rows=-1), dict(n_q=13), dict(n_q=0), dict(n_q=2 * 65), dict(window=-1), dict(sinks=-1),
+            dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(out=None), dict(lens=None),
+            dict(q=4098), dict(out=8200), dict(q_row=900), dict(out_head=4), dict(work=None), dict(work=1 << 20 | 16)]
+BAD_ROWS = [dict(type=1), dict(type=3), dict(rows=-1), dict(n_q=0), dict(rot_dim=8), dict(rot_dim=80), dict(rot_dim=-16),
+            dict(rope_rows=0), dict(q=None), dict(k=None), dict(v=None), dict(q_out=None), dict(seq=None), dict(slot=None),
+            dict(pos=None), dict(rope=None), dict(rope=1028), dict(q=4100), dict(k_row=132), dict(out_row=900)]
+
+
+def test_refusals_without_device(lib):
+    """Bad arguments are refused before any CUDA call; the addresses are never touched."""
+    a, r = good_attn(), good_rows()
+    for bad in BAD_CACHE:
+        c = good_cache(**bad)
+        for call, arg in ((lib.vp_paged_decode, a), (lib.vp_paged_prefill, a), (lib.vp_paged_append, r)):
+            assert call(ctypes.addressof(c), ctypes.addressof(arg), None) == -1, bad
+    c = good_cache()
+    for bad in BAD_ATTN:
+        a = good_attn(**bad)
+        assert lib.vp_paged_decode(ctypes.addressof(c), ctypes.addressof(a), None) == -1, bad
+        assert lib.vp_paged_prefill(ctypes.addressof(c), ctypes.addressof(a), None) == -1, bad
+    for bad in BAD_ROWS:
+        r = good_rows(**bad)
+        assert lib.vp_paged_append(ctypes.addressof(c), ctypes.addressof(r), None) == -1, bad
+    a = good_attn(rows=17)
+    assert lib.vp_paged_decode(ctypes.addressof(c), ctypes.addressof(a), None) == -1
+    assert b"16 rows" in lib.vp_last_error()
+    a = good_attn(q_start=None)
+    assert lib.vp_paged_prefill(ctypes.addressof(c), ctypes.addressof(a), None) == -1
+    a = good_attn(work_bytes=0)
+    assert lib.vp_paged_decode(ctypes.addressof(c), ctypes.addressof(a), None) == -1
+    assert lib.vp_paged_prefill(ctypes.addressof(c), ctypes.addressof(a), None) == -1
+    for call in (lib.vp_paged_decode, lib.vp_paged_prefill, lib.vp_paged_append):
+        assert call(None, ctypes.addressof(a), None) == -1
+        assert call(ctypes.addressof(c), None, None) == -1
+
+
+def test_nothing_to_do_without_device(lib):
+    c = good_cache()
+    for kw in (dict(n=0), dict(rows=0)):
+        a = good_attn(q=None, out=None, **kw)
+        assert lib.vp_paged_decode(ctypes.addressof(c), ctypes.addressof(a), None) == 0
+        assert lib.vp_paged_prefill(ctypes.addressof(c), ctypes.addressof(a), None) == 0
+    r = good_rows(rows=0)
+    assert lib.vp_paged_append(ctypes.addressof(c), ctypes.addressof(r), None) == 0
+
+
+def test_work_bytes(lib):
+    assert lib.vp_paged_work_bytes(64, 14, 2, 1) > 0
+    assert lib.vp_paged_work_bytes(128, 32, 8, 16) >= lib.vp_paged_work_bytes(128, 32, 8, 1)
+    for bad in ((96, 14, 2, 1), (64, 13, 2, 1), (64, 14, 0, 1), (64, 0, 2, 1), (64, 130, 2, 1), (64, 14, 2, 0)):
+        assert lib.vp_paged_work_bytes(*bad) == 0
+
+
+def test_layer_wants_cuda_pools():
+    k = torch.zeros(2, 2, 16, 64, dtype=torch.float16)
+    with pytest.raises(ValueError):
+        paged.PagedLayer(k, k, torch.zeros(1, 2, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        paged.PagedLayer(k, k[:, :1], torch.zeros(1, 2, dtype=torch.int32))
+
+
+def test_page_pool():
+    p = paged.PagePool(6, 16, 3, 4)
+    assert p.reserve(0, 17) == (0, [0, 1])
+    assert p.reserve(0, 32) == (2, [])
+    assert p.reserve(1, 1) == (0, [2])
+    assert p.reserve(0, 33) == (2, [3])
+    with pytest.raises(_lib.VpError):
+        p.reserve(2, 65)  # over the table row
+    with pytest.raises(_lib.VpError):
+        p.reserve(2, 48)  # two pages are left
+    assert p.held[2] == [] and len(p.free) == 2
+    assert p.release(0) == [0, 1, 3] and p.release(0) == []
+    assert p.reserve(2, 64) == (0, [0, 1, 3, 4])
+
+
+def test_ancestor_masks():
+    t = {"n": 5, "depth": [0, 1, 1, 2, 3], "parent": [-1, 0, 0, 2, 3], "tok": [0] * 5}
+    m = paged.ancestor_masks([t, {"n": 1, "depth": [0], "parent": [-1], "tok": [0]}])
+    assert m.shape == (2, 16) and m.dtype == torch.int32
+    assert m[0, :6].tolist() == [0b1, 0b11, 0b101, 0b1101, 0b11101, 0] and m[1, :2].tolist() == [1, 0]
+
+
+def test_oracle_visibility():
+    """The two forms of visibility agree where a tree is a chain, and a chain is the causal triangle."""
+    chain = [(2 << r) - 1 for r in range(5)]
+    for n in (3, 5, 9, 30):
+        for w, s in ((0, 0), (1, 0), (4, 2), (7, 0)):
+            t = O.sees_tree(n, chain, w, s)
+            if n >= 5:
+                assert (t == O.sees_prompt(n, 5, w, s)).all()
+    assert O.sees_tree(3, chain, 0, 0).sum(1).tolist() == [0, 0, 1, 2, 3]
+
+
+# ------------------------------------------------------------------------------------------------
+# GPU
+
+
+def make_cache(rng, lens, nkv, hd, ps, dtype, layout="hnd", spare=2, fill=None, extra_rows=0):
+    """Pools with random pages for requests of these lengths (slots past a length hold `fill`), as (layer, k, v on the host in
+    float64 [pages][heads][page_size][head_dim], table rows)."""
+    need = [-(-n // ps) for n in lens]
+    pages = sum(need) + spare
+    shape = (pages, nkv, ps, hd) if layout == "hnd" else (pages, ps, nkv, hd)
+    order = list(rng.permutation(pages))
+    width = max(need + [1]) + 1
+    table = np.full((len(lens) + extra_rows, width), -1, dtype=np.int32)
+    for i, n in enumerate(need):
+        table[i, :n] = [order.pop() for _ in range(n)]
+    pools = []
+    for _ in range(2):
+        p = torch.from_numpy(rng.standard_normal(shape).astype(np.float32)).to(dtype)
+        if fill is not None:
+            keep = torch.zeros((pages, ps), dtype=torch.bool)
+            for i, n in enumerate(lens):
+                for j in range(n):
+                    keep[table[i, j // ps], j % ps] = True
+            view = p.transpose(1, 2) if layout == "hnd" else p
+            view[~keep] = fill
+        pools.append(p.cuda() if layout == "hnd" else p.cuda().transpose(1, 2))
+    host = [p.cpu().double().numpy() for p in pools]
+    t = torch.from_numpy(table).cuda()
+    return paged.PagedLayer(pools[0], pools[1], t), host[0], host[1], table
+
+
+def tolerance(o, spread, smax, n, hd, dtype):
+    u = U[dtype]
+    step = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    delta = hd * 2.0 ** -23 * smax + 2.0 ** -20
+    return u * np.abs(o) + (u + 2 * delta) * spread + step * (n * spread.max(initial=0.0) + 1)
+
+
+def compare(out, lse, want, dtype, hd):
+    """out [..][hd], lse [..] against a list of (index, (o, lse, spread, smax), slots seen)."""
+    out = out.double().cpu().numpy()
+    lse = lse.double().cpu().numpy()
+    assert np.isfinite(out).all()
+    for at, (o, le, spread, smax), n in want:
+        off = np.abs(out[at] - o)
+        tol = tolerance(o, spread, smax, n, hd, dtype)
+        assert (off <= tol).all(), (at, float(off.max()), float(tol.min()))
+        if np.isinf(le):
+            assert lse[at] == -np.inf and (out[at] == 0).all(), at
+        else:
+            assert abs(lse[at] - le) <= hd * 2.0 ** -23 * smax + 2.0 ** -20 + 2.0 ** -22 * abs(le), at
+
+
+def tree_masks(rng, n, rows):
+    m = np.zeros((n, rows), dtype=np.int64)
+    for i in range(n):
+        for r in range(rows):
+            m[i, r] = (m[i, rng.integers(0, r)] if r else 0) | 1 << r
+    return m
+
+
+def want_decode(q, k, v, table, lens, masks, window, sinks, scale, ps, seqs=None, clip=None):
+    n, rows, nq, hd = q.shape
+    group = nq // k.shape[1]
+    want = []
+    for i, length in enumerate(lens):
+        row = table[i if seqs is None else seqs[i]]
+        ks, vs = (O.slots(p, row, length) for p in (k, v))
+        seen = O.sees_tree(length, [int(x) for x in masks[i]], window, sinks)
+        for r in range(rows):
+            for h in range(nq):
+                want.append(((i, r, h), O.attend(q[i, r, h], ks[h // group], vs[h // group], seen[r], scale), int(seen[r].sum())))
+    return want
+
+
+SHAPES = [(14, 2, 64, torch.float16, 64, "hnd"), (14, 2, 64, torch.bfloat16, 16, "nhd"), (8, 2, 128, torch.bfloat16, 32, "hnd"),
+          (4, 4, 128, torch.float16, 256, "nhd"), (9, 1, 64, torch.float16, 128, "hnd"), (64, 1, 64, torch.float16, 16, "hnd")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nkv,hd,dtype,ps,layout", SHAPES)
+@pytest.mark.parametrize("rows", [1, 2, 5, 16])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (5, 3), (64, 0), (100, 70)])
+def test_decode(nq, nkv, hd, dtype, ps, layout, rows, window, sinks):
+    """Lengths of zero, one, around a tile and a page and past several, NaN in every unused slot, requests shorter than their
+    rows, random trees."""
+    rng = np.random.default_rng(rows * 1000 + window + nq + ps)
+    lens = [300, 0, 1, 15, 16, 17, 63, 64, 65, 128, 257, 2 * rows + 1, rows]
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, ps, dtype, layout, fill=float("nan"))
+    q = torch.from_numpy(rng.standard_normal((len(lens), rows, nq, hd)).astype(np.float32)).to(dtype)
+    masks = tree_masks(rng, len(lens), rows)
+    chain = rows == 5
+    if chain:
+        masks[:] = [(2 << r) - 1 for r in range(rows)]
+    out, lse = kv.decode(q.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(),
+                         mask=None if chain else torch.from_numpy(masks.astype(np.int32)).cuda(), window=window, sinks=sinks,
+                         return_lse=True)
+    kv.check()
+    compare(out, lse, want_decode(q.double().numpy(), k, v, table, lens, masks, window, sinks, hd ** -0.5, ps), dtype, hd)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,nq,nkv,ps,dtype", [(64, 14, 2, 64, torch.float16), (128, 8, 2, 16, torch.bfloat16)])
+def test_decode_long_and_uneven(hd, nq, nkv, ps, dtype):
+    """One long request beside short ones (its length is split and joined), single rows given as [n][heads][head_dim] slices of
+    one projection, a scale of the caller's, and the same bits when called again."""
+    rng = np.random.default_rng(hd)
+    lens = [9001, 3, 700, 1, 4097, 0]
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, ps, dtype)
+    fused = torch.from_numpy(rng.standard_normal((len(lens), (nq + 2 * nkv) * hd)).astype(np.float32)).to(dtype).cuda()
+    q = fused[:, :nq * hd].unflatten(1, (nq, hd))
+    ln = torch.tensor(lens, dtype=torch.int32).cuda()
+    out, lse = kv.decode(q, ln, scale=0.2, return_lse=True)
+    again = kv.decode(q, ln, scale=0.2)
+    assert out.shape == (len(lens), nq, hd) and torch.equal(out, again)
+    masks = np.ones((len(lens), 1), dtype=np.int64)
+    want = want_decode(q.double().cpu().numpy()[:, None], k, v, table, lens, masks, 0, 0, 0.2, ps)
+    compare(out[:, None], lse[:, None], want, dtype, hd)
+
+
+@pytest.mark.gpu
+def test_decode_large_scores_and_empty_masks():
+    """Scores far past exp's range, rising and falling along the cache; rows whose mask has no bit see the old slots only, and
+    nothing when there are none."""
+    rng = np.random.default_rng(5)
+    lens, hd, nq, nkv = [500, 2, 66], 64, 14, 2
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, 64, torch.float16)
+    kv.k.mul_(30)
+    k = kv.k.double().cpu().numpy()
+    q = torch.from_numpy(20 * rng.standard_normal((3, 2, nq, hd)).astype(np.float32)).half()
+    masks = np.array([[1, 0], [0, 0], [0, 3]])
+    out, lse = kv.decode(q.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), mask=torch.from_numpy(masks.astype(np.int32)).cuda(),
+                         return_lse=True)
+    assert (out[1] == 0).all()
+    compare(out, lse, want_decode(q.double().numpy(), k, v, table, lens, masks, 0, 0, hd ** -0.5, 64), torch.float16, hd)
+
+
+@pytest.mark.gpu
+def test_decode_requests_by_index_and_out_of_range():
+    """seqs picks rows of the table; a request, a length or a page outside the cache is told by check(), the other requests
+    are served."""
+    rng = np.random.default_rng(6)
+    lens, hd, nq, nkv, ps = [100, 40, 17], 64, 4, 2, 16
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, ps, torch.float16)
+    q = torch.from_numpy(rng.standard_normal((2, 1, nq, hd)).astype(np.float32)).half()
+    seqs = [2, 0]
+    ln = [lens[s] for s in seqs]
+
+    def run(seqs, ln):
+        return kv.decode(q.cuda(), torch.tensor(ln, dtype=torch.int32).cuda(), seqs=torch.tensor(seqs, dtype=torch.int32).cuda(),
+                         return_lse=True)
+
+    ones = np.ones((2, 1), dtype=np.int64)
+    want = want_decode(q.double().numpy(), k, v, table, ln, ones, 0, 0, hd ** -0.5, ps, seqs)
+    out, lse = run(seqs, ln)
+    compare(out, lse, want, torch.float16, hd)
+    kv.check()
+    for bad_seq, bad_len in ((99, ln[1]), (-1, ln[1]), (0, -5)):
+        o2, l2 = run([seqs[0], bad_seq], [ln[0], bad_len])
+        assert torch.equal(o2[0], out[0]) and (o2[1] == 0).all() and (l2[1] == -np.inf).all()
+        with pytest.raises(_lib.VpError, match="slot"):
+            kv.check()
+        kv.check()
+    kv.table[0, 1] = 1 << 20  # a page that does not exist reads as zeros
+    k[table[0, 1]], v[table[0, 1]] = 0, 0
+    out, lse = run(seqs, ln)
+    with pytest.raises(_lib.VpError, match="page"):
+        kv.check()
+    compare(out, lse, want_decode(q.double().numpy(), k, v, table, ln, ones, 0, 0, hd ** -0.5, ps, seqs), torch.float16, hd)
+
+
+@pytest.mark.gpu
+def test_window_reads_no_page_before_it():
+    """Pages that a window has left behind may be anybody's: their table entries are not read."""
+    rng = np.random.default_rng(7)
+    lens, hd, nq, nkv, ps = [1000, 333], 64, 14, 2, 16
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, ps, torch.float16)
+    q = torch.from_numpy(rng.standard_normal((2, 1, nq, hd)).astype(np.float32)).half().cuda()
+    ln = torch.tensor(lens, dtype=torch.int32).cuda()
+    starts = torch.tensor([0, 1, 2], dtype=torch.int32).cuda()
+    out = kv.decode(q, ln, window=64, sinks=4)
+    pre = kv.prefill(q[:, 0].contiguous(), starts, ln, window=64, sinks=4)
+    for i, n in enumerate(lens):
+        kv.table[i, 1:(n - 64) // ps] = -7
+        first = int(table[i, 0])  # beside the sinks, the first page holds whatever its next owner wrote
+        kv.k[first, :, 4:] = float("nan")
+        kv.v[first, :, 4:] = float("inf")
+        edge = int(table[i, (n - 64) // ps])
+        kv.v[edge, :, :(n - 64) % ps] = float("nan")
+    assert torch.equal(kv.decode(q, ln, window=64, sinks=4), out)
+    assert torch.equal(kv.prefill(q[:, 0].contiguous(), starts, ln, window=64, sinks=4), pre)
+    kv.check()
+
+
+def want_prefill(q, k, v, table, starts, lens, window, sinks, scale):
+    group = q.shape[1] // k.shape[1]
+    want = []
+    for i, length in enumerate(lens):
+        a, b = starts[i], starts[i + 1]
+        ks, vs = (O.slots(p, table[i], length) for p in (k, v))
+        new = b - a
+        seen = np.zeros((new, length), dtype=bool)
+        have = min(new, length)
+        if have:
+            seen[new - have:] = O.sees_prompt(length, have, window, sinks)
+        for r in range(new):
+            for h in range(q.shape[1]):
+                want.append(((a + r, h), O.attend(q[a + r, h], ks[h // group], vs[h // group], seen[r], scale), int(seen[r].sum())))
+    return want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nkv,hd,dtype,ps,layout", SHAPES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (7, 3), (130, 0), (64, 140)])
+def test_prefill(nq, nkv, hd, dtype, ps, layout, window, sinks):
+    """Whole prompts, chunks over a cached prefix, requests without rows, without slots, with more rows than slots."""
+    rng = np.random.default_rng(window + nq + ps + hd)
+    lens = [37, 0, 1, 129, 300, 64, 5, 400]
+    new = [37, 0, 1, 129, 40, 3, 9, 1]
+    starts = np.concatenate([[0], np.cumsum(new)])
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, ps, dtype, layout, fill=float("nan"))
+    q = torch.from_numpy(rng.standard_normal((int(starts[-1]), nq, hd)).astype(np.float32)).to(dtype)
+    out, lse = kv.prefill(q.cuda(), torch.from_numpy(starts.astype(np.int32)).cuda(), torch.tensor(lens, dtype=torch.int32).cuda(),
+                          window=window, sinks=sinks, return_lse=True)
+    kv.check()
+    compare(out, lse, want_prefill(q.double().numpy(), k, v, table, starts, lens, window, sinks, hd ** -0.5), dtype, hd)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nkv,hd,dtype", [(14, 2, 64, torch.float16), (4, 1, 128, torch.bfloat16)])
+def test_prefill_long(nq, nkv, hd, dtype):
+    """A prompt of many tiles, scores that rise along it (the running maximum moves far), and a chunk over a long prefix; the
+    same bits when called again. Rows are sampled."""
+    rng = np.random.default_rng(nq)
+    lens, new = [1500, 3001], [1500, 77]
+    starts = np.concatenate([[0], np.cumsum(new)])
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, 64, dtype)
+    ramp = torch.zeros(kv.k.shape[0], 64, device="cuda")
+    for i, n in enumerate(lens):
+        for j in range(-(-n // 64)):
+            ramp[int(table[i, j])] = 0.2 + 0.15 * j
+    kv.k.mul_(ramp[:, None, :, None].to(dtype))
+    k = kv.k.double().cpu().numpy()
+    q = torch.from_numpy(3 * rng.standard_normal((int(starts[-1]), nq, hd)).astype(np.float32)).to(dtype)
+    args = (q.cuda(), torch.from_numpy(starts.astype(np.int32)).cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    out, lse = kv.prefill(*args, return_lse=True)
+    assert torch.equal(out, kv.prefill(*args))
+    pick = sorted(rng.choice(int(starts[-1]), 40, replace=False))
+    want = []
+    for t in pick:
+        i = int(np.searchsorted(starts, t, side="right") - 1)
+        p = lens[i] - new[i] + t - starts[i]
+        ks, vs = (O.slots(x, table[i], p + 1) for x in (k, v))
+        for h in range(nq):
+            g = h // (nq // nkv)
+            want.append(((t, h), O.attend(q[t, h].double().numpy(), ks[g], vs[g], np.ones(p + 1, dtype=bool), hd ** -0.5), p + 1))
+    compare(out, lse, want, dtype, hd)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("src,dtype", [(torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16),
+                                       (torch.float32, torch.float16), (torch.float32, torch.bfloat16)])
+@pytest.mark.parametrize("nq,nkv,hd,rot,interleaved,layout", [(14, 2, 64, 64, False, "hnd"), (8, 2, 128, 128, True, "nhd"),
+                                                             (3, 1, 64, 32, False, "nhd"), (5, 5, 128, 48, True, "hnd"),
+                                                             (14, 2, 64, 0, False, "hnd")])
+def test_append(src, dtype, nq, nkv, hd, rot, interleaved, layout):
+    """Slices of one projection, padding rows, rows out of range; slots that no row names keep their bits."""
+    rng = np.random.default_rng(hd + rot + nq)
+    lens, ps = [40, 1, 130], 16
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, ps, dtype, layout)
+    rows = 23
+    fused = torch.from_numpy(rng.standard_normal((rows, nq + 2 * nkv, hd)).astype(np.float32)).to(src)
+    d = fused.cuda()
+    places = [(s, j) for s, n in enumerate(lens) for j in range(n)]
+    rng.shuffle(places)
+    seq = np.array([p[0] for p in places[:rows]], dtype=np.int32)
+    slot = np.array([p[1] for p in places[:rows]], dtype=np.int32)
+    pos = rng.integers(0, 200, rows).astype(np.int32)
+    seq[4], seq[9] = -1, 77
+    slot[11] = 10 ** 6
+    pos[13] = 200
+    rope = paged.rope_table(200, rot, 1e4) if rot else None
+    q = kv.append(d[:, :nq], d[:, nq:nq + nkv], d[:, nq + nkv:], *(torch.from_numpy(x).cuda() for x in (seq, slot, pos)), rope,
+                  interleaved=interleaved)
+    with pytest.raises(_lib.VpError):
+        kv.check()
+    f = fused.double().numpy()
+    cs = rope.cpu().numpy() if rot else np.zeros((200, 0, 2))
+    want_q = np.zeros((rows, nq, hd))
+    touched = np.zeros(k.shape[:1] + k.shape[2:3], dtype=bool)
+    for t in range(rows):
+        if rot and pos[t] >= 200:
+            continue
+        y = O.rotate(f[t], cs[min(pos[t], 199)], interleaved)
+        want_q[t] = y[:nq]
+        if 0 <= seq[t] < len(lens) and slot[t] < 1000:
+            at = table[seq[t], slot[t] // ps], slot[t] % ps
+            touched[at] = True
+            k[at[0], :, at[1]], v[at[0], :, at[1]] = y[nq:nq + nkv], f[t, nq + nkv:]
+    assert touched.sum() == rows - 4 + (0 if rot else 1)
+    u = U[dtype]
+
+    def near(got, want, size):
+        got = got.double().cpu().numpy()
+        assert (np.abs(got - want) <= u * np.abs(want) + 2.0 ** -22 * size + 2.0 ** -25).all()
+
+    near(q, want_q, 8.0)
+    gk, gv = kv.k.cpu(), kv.v.cpu()
+    near(gk, k, 8.0)
+    near(gv, v, 0.0)
+    untouched = torch.from_numpy(~touched)
+    for g, w in ((gk, k), (gv, v)):  # bit for bit
+        assert np.array_equal(g.double().numpy().swapaxes(1, 2)[untouched.numpy()], w.swapaxes(1, 2)[untouched.numpy()])
+
+
+@pytest.mark.gpu
+def test_append_in_place_and_one_row():
+    rng = np.random.default_rng(1)
+    kv, k, v, table = make_cache(rng, [70], 2, 64, 64, torch.float16)
+    x = torch.from_numpy(rng.standard_normal((1, 18, 64)).astype(np.float32)).half().cuda()
+    idx = [torch.tensor([i], dtype=torch.int32).cuda() for i in (0, 69, 69)]
+    rope = paged.rope_table(70)
+    q = kv.append(x[:, :14], x[:, 14:16], x[:, 16:], *idx, rope)
+    same = x[:, :14]
+    assert kv.append(same, x[:, 14:16], x[:, 16:], *idx, rope, out=same) is same
+    assert torch.equal(same, q)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """A pool of more than 2^32 elements: its last page is written and read like its first."""
+    hd, ps, nkv, nq = 64, 64, 2, 14
+    pages = (1 << 32) // (hd * ps * nkv) + 40
+    pool = torch.zeros((pages, nkv, ps, hd), dtype=torch.float16, device="cuda")
+    rng = np.random.default_rng(2)
+    n = 130
+    ids = [pages - 1, 3, pages - 30]
+    table = torch.tensor([ids], dtype=torch.int32).cuda()
+    kv = paged.PagedLayer(pool, pool, table)  # keys and values in one pool: both read what is written last, the values
+    x = torch.from_numpy(rng.standard_normal((n, nq + 2 * nkv, hd)).astype(np.float32)).half()
+    d = x.cuda()
+    zero = torch.zeros(n, dtype=torch.int32).cuda()
+    slot = torch.arange(n, dtype=torch.int32).cuda()
+    vals = d[:, nq:nq + nkv]
+    q = kv.append(d[:, :nq], vals, vals, zero, slot, None, None)
+    kv.check()
+    k = np.zeros((3, nkv, ps, hd))
+    for j in range(n):
+        k[j // ps, :, j % ps] = x[j, nq:nq + nkv].double().numpy()
+    assert torch.equal(pool[ids[2], :, 1].cpu(), x[n - 1, nq:nq + nkv])
+    lens = torch.tensor([n], dtype=torch.int32).cuda()
+    out, lse = kv.decode(q[-1:], lens, return_lse=True)
+    qh = q.double().cpu().numpy()
+    want = want_decode(qh[None, -1:], k, k, np.array([[0, 1, 2]]), [n], np.ones((1, 1), dtype=np.int64), 0, 0, hd ** -0.5, ps)
+    compare(out[None], lse[None], want, torch.float16, hd)
+    starts = torch.tensor([0, n], dtype=torch.int32).cuda()
+    out, lse = kv.prefill(q, starts, lens, return_lse=True)
+    compare(out, lse, want_prefill(qh, k, k, np.array([[0, 1, 2]]), [0, n], [n], 0, 0, hd ** -0.5), torch.float16, hd)
+
+
+@pytest.mark.gpu
+def test_refusals():
+    rng = np.random.default_rng(3)
+    kv, *_ = make_cache(rng, [20, 20], 2, 64, 16, torch.float16)
+    q = torch.zeros(2, 1, 14, 64, dtype=torch.float16, device="cuda")
+    ln = torch.tensor([20, 20], dtype=torch.int32).cuda()
+    for bad in (dict(q=q.float()), dict(q=q.cpu()), dict(q=q[..., :32]), dict(lens=ln.long()), dict(lens=ln[:1]), dict(lens=ln.cpu()),
+                dict(mask=torch.zeros(2, 2, dtype=torch.int32).cuda()), dict(out=q[:1]), dict(q=q[0, 0]),
+                dict(q=torch.zeros(3, 1, 14, 64).half().cuda(), lens=torch.tensor([1, 1, 1], dtype=torch.int32).cuda())):
+        with pytest.raises(ValueError):
+            kv.decode(**{**dict(q=q, lens=ln), **bad})
+    for bad in (dict(q=q[:, :, :13]), dict(window=-1), dict(sinks=-1), dict(scale=0.0),
+                dict(q=torch.zeros(2, 17, 14, 64).half().cuda()),
+                dict(q=torch.zeros(2 * 14 * 64 + 4).half().cuda()[4:].view(2, 1, 14, 64))):
+        with pytest.raises(_lib.VpError):
+            kv.decode(**{**dict(q=q, lens=ln), **bad})
+    with pytest.raises(ValueError):
+        kv.prefill(q[:, 0], torch.tensor([0, 1], dtype=torch.int32).cuda(), ln)
+    with pytest.raises(ValueError):
+        kv.prefill(q, torch.tensor([0, 1, 2], dtype=torch.int32).cuda(), ln)
+    x = torch.zeros(2, 18, 64, dtype=torch.float16, device="cuda")
+    i = torch.zeros(2, dtype=torch.int32, device="cuda")
+    good = dict(q=x[:, :14], k=x[:, 14:16], v=x[:, 16:], seq=i, slot=i, pos=i, rope=paged.rope_table(8))
+    for bad in (dict(k=x[:, 14:15]), dict(v=x[:, 14:15]), dict(q=x[:, :14].bfloat16()), dict(pos=None), dict(seq=i[:1]),
+                dict(rope=paged.rope_table(8).half()), dict(q=x[:, :14, :32])):
+        with pytest.raises(ValueError):
+            kv.append(**{**good, **bad})
+    with pytest.raises(_lib.VpError):
+        kv.append(**{**good, "rope": paged.rope_table(8, 8)})
+    with pytest.raises(ValueError):
+        paged.PagedLayer(kv.k, kv.v, kv.table.long())
+    with pytest.raises(ValueError):
+        paged.PagedLayer(kv.k, kv.v.bfloat16(), kv.table)
+
+
+@pytest.mark.gpu
+def test_pool_of_a_model():
+    """PagedKV: pages given, grown and returned; the table follows, and other requests' pages stay."""
+    kv = paged.PagedKV(n_layers=2, n_pages=8, page_size=16, max_seqs=3, max_len=64)
+    kv.reserve(0, 20)
+    kv.reserve(1, 16)
+    kv.reserve(0, 33)
+    assert kv.table[0, :4].tolist() == [0, 1, 3, -1] and kv.table[1, 0].item() == 2 and kv.free_pages == 4
+    kv.release(0)
+    assert kv.table[0].tolist() == [-1] * 4 and kv.free_pages == 7 and kv.table[1, 0].item() == 2
+    with pytest.raises(_lib.VpError):
+        kv.reserve(2, 65)
+    assert len(kv) == 2 and kv[1].k.data_ptr() == kv.k[1].data_ptr()
+    kv.check()
+
+
+@pytest.mark.gpu
+def test_other_stream_and_graph():
+    """Calls follow torch's current stream, and a captured append + decode step replays on new inputs."""
+    rng = np.random.default_rng(4)
+    lens, nq, nkv, hd = [200, 31], 14, 2, 64
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, 64, torch.float16)
+    x = torch.from_numpy(rng.standard_normal((2, nq + 2 * nkv, hd)).astype(np.float32)).half().cuda()
+    seq = torch.tensor([0, 1], dtype=torch.int32).cuda()
+    ln = torch.tensor(lens, dtype=torch.int32).cuda()
+    last = ln - 1
+    rope = paged.rope_table(256)
+
+    def step():
+        q = kv.append(x[:, :nq], x[:, nq:nq + nkv], x[:, nq + nkv:], seq, last, last, rope)
+        return kv.decode(q, ln)
+
+    first = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = step()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            third = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(first, second)
+    x.copy_(x.flip(0))
+    torch.cuda.synchronize()
+    g.replay()
+    torch.cuda.synchronize()
+    replayed = third.clone()
+    assert torch.equal(replayed, step()) and not torch.equal(replayed, first)
