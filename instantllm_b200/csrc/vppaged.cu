@@ -6,10 +6,10 @@
 #include <string>
 
 #include "vp_paged.cuh"
+#include "vp_paged_decode.cuh"
+#include "vp_paged_host.h"
 
 using namespace vp;
-
-void vp_set_last_error(const std::string& msg);
 
 namespace vp {
 
@@ -126,50 +126,29 @@ __global__ void __launch_bounds__(APPEND_THREADS) k_paged_append(const vp_paged 
   }
 }
 
-// ---- attention, one warp per row and query head ----
+// ---- attention of prompts, one warp per row and query head ----
 // The running maximum and sum of the softmax over 32 slots at a time: lane i scores slot i, then
 // every lane adds the 32 weighted values of its own HD / 32 elements.
-template <typename T, int HD, bool PROMPT>
-__global__ void k_paged_attn(const vp_paged c, const vp_paged_attn a) {
+template <typename T, int HD>
+__global__ void k_paged_prompt(const vp_paged c, const vp_paged_attn a) {
   constexpr int E = HD / 32;
   const int lane = threadIdx.x & 31;
   const long long w = blockIdx.x * (long long)(blockDim.x / 32) + threadIdx.x / 32;
   const int h = (int)(w % a.n_q);
   const long long row = w / a.n_q;
-  int i, r, n_new;
-  if (PROMPT) {
-    if (row >= a.rows) return;
-    i = 0;
-    while (i < a.n && a.q_start[i + 1] <= row) ++i;
-    if (i == a.n || a.q_start[i] > row) return;
-    r = (int)row - a.q_start[i];
-    n_new = a.q_start[i + 1] - a.q_start[i];
-  } else {
-    if (row >= (long long)a.n * a.rows) return;
-    i = (int)(row / a.rows);
-    r = (int)(row % a.rows);
-    n_new = a.rows;
-  }
+  if (row >= a.rows) return;
+  int i = 0;
+  while (i < a.n && a.q_start[i + 1] <= row) ++i;
+  if (i == a.n || a.q_start[i] > row) return;
+  const int r = (int)row - a.q_start[i], n_new = a.q_start[i + 1] - a.q_start[i];
   const PgSeq s = pg_seq(c, a.seqs, a.lens, i);
-  const int base = s.len - n_new;
-  uint32_t anc[PROMPT ? 1 : PG_MAX_ROWS] = {};
-  uint32_t bits = 0;
-  if (!PROMPT) {
-    for (int t = 0; t < n_new; ++t) {
-      anc[t] = a.mask ? (uint32_t)a.mask[(long long)i * n_new + t] & ((1u << n_new) - 1) : (2u << t) - 1;
-      if (t == r) bits = anc[t];
-    }
-  }
-  const int end = base + r < 0 ? 0 : PROMPT ? base + r + 1 : s.len;
-  const int at = PROMPT ? base + r : 0;
-  const T* q = static_cast<const T*>(a.q) + (PROMPT ? row * a.q_row : i * a.q_seq + r * a.q_row) + h * a.q_head;
+  const int at = s.len - n_new + r, end = at < 0 ? 0 : at + 1;
+  const T* q = static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
   const int hk = h / (a.n_q / c.n_kv);
   float m = -INFINITY, l = 0.f, o[E] = {};
   for (int j0 = 0; j0 < end; j0 += 32) {
     const int j = j0 + lane;
-    bool see = j < end;
-    if (see) see = PROMPT ? !a.window || at - j < a.window || j < a.sinks
-                          : pg_sees(j, s.len, base, bits, anc, a.window, a.sinks);
+    const bool see = j < end && (!a.window || at - j < a.window || j < a.sinks);
     float sc = -INFINITY;
     int page = -1;
     if (see) {
@@ -196,7 +175,7 @@ __global__ void k_paged_attn(const vp_paged c, const vp_paged_attn a) {
       for (int e = 0; e < E; ++e) o[e] += pt * (float)v[lane + 32 * e];
     }
   }
-  T* out = static_cast<T*>(a.out) + (PROMPT ? row * a.out_row : i * a.out_seq + r * a.out_row) + h * a.out_head;
+  T* out = static_cast<T*>(a.out) + row * a.out_row + h * a.out_head;
   for (int e = 0; e < E; ++e) out[lane + 32 * e] = (T)(l > 0.f ? o[e] / l : 0.f);
   if (a.lse && lane == 0) a.lse[row * a.n_q + h] = l > 0.f ? m + logf(l) : -INFINITY;
 }
@@ -204,17 +183,6 @@ __global__ void k_paged_attn(const vp_paged c, const vp_paged_attn a) {
 }  // namespace vp
 
 namespace {
-
-int pfail(int code, const char* msg) {
-  vp_set_last_error(msg);
-  return code;
-}
-int launched(const char* what) {
-  const cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) return VP_OK;
-  vp_set_last_error(std::string(what) + ": " + cudaGetErrorString(e));
-  return VP_ERR_CUDA;
-}
 
 bool off16(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
 
@@ -266,12 +234,39 @@ int check_attn(const vp_paged* c, const vp_paged_attn* a) {
   return VP_OK;
 }
 
-template <typename T, bool PROMPT>
-void attn_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
-  const long long warps = (long long)(PROMPT ? 1 : a.n) * a.rows * a.n_q;
+template <typename T>
+void prompt_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
+  const long long warps = (long long)a.rows * a.n_q;
   const unsigned grid = (unsigned)((warps + 3) / 4);
-  if (c.head_dim == 64) k_paged_attn<T, 64, PROMPT><<<grid, 128, 0, st>>>(c, a);
-  else k_paged_attn<T, 128, PROMPT><<<grid, 128, 0, st>>>(c, a);
+  if (c.head_dim == 64) k_paged_prompt<T, 64><<<grid, 128, 0, st>>>(c, a);
+  else k_paged_prompt<T, 128><<<grid, 128, 0, st>>>(c, a);
+}
+
+template <typename T, int HD>
+int decode_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
+  using Sh = DcShape<HD>;
+  DcParams p;
+  p.c = c;
+  p.a = a;
+  p.group = a.n_q / c.n_kv;
+  const int m = p.group * a.rows;
+  p.blocks = (m + DC_BLOCK_ROWS - 1) / DC_BLOCK_ROWS;
+  p.block_rows = m < DC_BLOCK_ROWS ? m : DC_BLOCK_ROWS;
+  p.mt = (p.block_rows + 15) / 16;
+  p.min_tiles = 4;
+  p.tickets = static_cast<unsigned*>(a.work);
+  p.rec = reinterpret_cast<float*>(static_cast<char*>(a.work) + WORK_HEAD);
+  CUtensorMap mk, mv;
+  if (const int e = pool_maps(c, c.page_size < Sh::TS ? c.page_size : Sh::TS, &mk, &mv)) return e;
+  int sms = 0;
+  if (const int e = sm_count(&sms)) return e;
+  const int tiles = (int)(((long long)c.max_pages * c.page_size + Sh::TS - 1) / Sh::TS);
+  const long long most = (long long)a.n * c.n_kv * p.blocks * tiles;
+  const int grid = (int)(most < sms ? most : sms);
+  const cudaError_t e = cudaFuncSetAttribute(k_paged_decode<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM);
+  if (e != cudaSuccess) return pfail(VP_ERR_CUDA, cudaGetErrorString(e));
+  k_paged_decode<T, HD><<<grid, DC_THREADS, Sh::SMEM, st>>>(p, mk, mv);
+  return launched("vp_paged_decode");
 }
 
 }  // namespace
@@ -310,7 +305,9 @@ int vp_paged_append(const vp_paged* c, const vp_paged_rows* r, void* stream) try
 size_t vp_paged_work_bytes(int32_t head_dim, int32_t n_q, int32_t n_kv, int32_t rows) {
   if ((head_dim != 64 && head_dim != 128) || n_kv < 1 || n_q < 1 || n_q % n_kv || n_q / n_kv > PG_MAX_GROUP || rows < 1)
     return 0;
-  return 256;
+  const int m = n_q / n_kv * rows, block = m < DC_BLOCK_ROWS ? m : DC_BLOCK_ROWS;
+  const size_t record = head_dim == 64 ? DcShape<64>::record(block) : DcShape<128>::record(block);
+  return WORK_HEAD + (size_t)PG_MAX_CTAS * 2 * record * sizeof(float);
 }
 
 int vp_paged_decode(const vp_paged* c, const vp_paged_attn* a, void* stream) try {
@@ -318,9 +315,8 @@ int vp_paged_decode(const vp_paged* c, const vp_paged_attn* a, void* stream) try
   if (a->rows > PG_MAX_ROWS) return pfail(VP_ERR_ARG, "a decode call takes 1 to 16 rows per request");
   if (a->n == 0 || a->rows == 0) return VP_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (c->type == VP_T_F16) attn_launch<__half, false>(*c, *a, st);
-  else attn_launch<__nv_bfloat16, false>(*c, *a, st);
-  return launched("vp_paged_decode");
+  if (c->type == VP_T_F16) return c->head_dim == 64 ? decode_launch<__half, 64>(*c, *a, st) : decode_launch<__half, 128>(*c, *a, st);
+  return c->head_dim == 64 ? decode_launch<__nv_bfloat16, 64>(*c, *a, st) : decode_launch<__nv_bfloat16, 128>(*c, *a, st);
 } catch (const std::exception&) {
   return VP_ERR_NOMEM;
 }
@@ -330,8 +326,8 @@ int vp_paged_prefill(const vp_paged* c, const vp_paged_attn* a, void* stream) tr
   if (a->n == 0 || a->rows == 0) return VP_OK;
   if (!a->q_start) return pfail(VP_ERR_ARG, "null q_start");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (c->type == VP_T_F16) attn_launch<__half, true>(*c, *a, st);
-  else attn_launch<__nv_bfloat16, true>(*c, *a, st);
+  if (c->type == VP_T_F16) prompt_launch<__half>(*c, *a, st);
+  else prompt_launch<__nv_bfloat16>(*c, *a, st);
   return launched("vp_paged_prefill");
 } catch (const std::exception&) {
   return VP_ERR_NOMEM;

@@ -271,6 +271,22 @@ def test_decode_long_and_uneven(hd, nq, nkv, ps, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd,n,rows", [(64, 90001, 1), (128, 50001, 1), (64, 30011, 4), (64, 20001, 16)])
+def test_decode_very_long(hd, n, rows):
+    """Runs of many tiles per CTA: every stage of the ring is refilled many times."""
+    rng = np.random.default_rng(n)
+    nq, nkv, ps, dtype = 14, 2, 64, torch.float16
+    kv, k, v, table = make_cache(rng, [n, 70], nkv, hd, ps, dtype)
+    q = torch.from_numpy(rng.standard_normal((2, rows, nq, hd)).astype(np.float32)).to(dtype)
+    masks = tree_masks(rng, 2, rows)
+    out, lse = kv.decode(q.cuda(), torch.tensor([n, 70], dtype=torch.int32).cuda(), mask=torch.from_numpy(masks.astype(np.int32)).cuda(),
+                         return_lse=True)
+    kv.check()
+    want = want_decode(q.double().numpy(), k, v, table, [n, 70], masks, 0, 0, hd ** -0.5, ps)
+    compare(out, lse, want, dtype, hd)
+
+
+@pytest.mark.gpu
 def test_decode_large_scores_and_empty_masks():
     """Scores far past exp's range, rising and falling along the cache; rows whose mask has no bit see the old slots only, and
     nothing when there are none."""
