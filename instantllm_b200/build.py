@@ -7,8 +7,9 @@ from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
-SOURCES = [PKG / "csrc" / "vpass.cu", PKG / "csrc" / "vpdraft.cu", PKG / "csrc" / "vppaged.cu"]
-HEADERS = sorted((PKG / "csrc").glob("*.cuh")) + [ROOT / "include" / "vpass.h"]
+SOURCES = [PKG / "csrc" / "vpass.cu", PKG / "csrc" / "vpdraft.cu", PKG / "csrc" / "vppaged.cu",
+           PKG / "csrc" / "vpprefill.cu"]
+HEADERS = sorted((PKG / "csrc").glob("*.cuh")) + sorted((PKG / "csrc").glob("*.h")) + [ROOT / "include" / "vpass.h"]
 OUT = PKG / "libvpass.so"
 # the trace build (performance work only): the same kernels with %globaltimer stamps at every stage
 # step of one layer and of the lm_head (-DVP_TRACE_DETAIL), read by instantllm_b200.trace

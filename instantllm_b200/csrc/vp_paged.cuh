@@ -68,7 +68,7 @@ template <typename T>
 struct PgType;
 template <>
 struct PgType<__half> {
-  using Pair = __half2;
+  static constexpr bool BF16 = false;
   static __device__ __forceinline__ float2 up(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
   static __device__ __forceinline__ uint32_t down(float a, float b) {
     __half2 h = __floats2half2_rn(a, b);
@@ -82,7 +82,7 @@ struct PgType<__half> {
 };
 template <>
 struct PgType<__nv_bfloat16> {
-  using Pair = __nv_bfloat162;
+  static constexpr bool BF16 = true;
   static __device__ __forceinline__ float2 up(uint32_t w) {
     return {__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
   }

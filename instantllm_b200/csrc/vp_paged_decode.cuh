@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
     if (lane >= o) incl += v;
   }
   if (lane == 31) warp_sums[warp] = incl;
-  __syncthreads();
+  cta_sync();
   long long before = 0, N = 0;
 #pragma unroll
   for (int w = 0; w < DC_THREADS / 32; ++w) {
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
       at += n;
     }
   }
-  __syncthreads();
+  cta_sync();
 
   // the CTA's runs: (request, pair, tiles [u0, u1) of the pair), the same walk in every warp
   int seq = first_seq;
@@ -251,10 +251,12 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
           const uint32_t k_th = n_seen + b;
           const int st = k_th % ST, u = u0 + b;
           const int s0 = (u < sp.ns ? u : sp.ws + u - sp.ns) * TS;
-          if (!dead && !mbar_wait_warp(&full[st], (k_th / ST) & 1)) {
+          __syncwarp();
+          if (!*(volatile int*)&dead && !mbar_wait_warp(&full[st], (k_th / ST) & 1)) {
             pg_status(c.status, VP_DEV_ERR_TIMEOUT);
-            dead = 1;
+            *(volatile int*)&dead = 1;
           }
+          __syncwarp();
           const uint32_t kb = smem_u32(ring) + st * 2 * DC_TILE, vb = kb + DC_TILE;
           float s[NT][4];
           // lanes 0-7 .. 24-31 point at the lines of four 8 x 8 matrices: 8 slots, 32 elements

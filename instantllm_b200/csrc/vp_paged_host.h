@@ -5,11 +5,13 @@
 
 #include <string>
 
-#include "../../include/vpass.h"
+#include "vp_paged.cuh"
 
 void vp_set_last_error(const std::string& msg);
 
 namespace {
+
+using namespace vp;
 
 constexpr int PG_MAX_CTAS = 160;       // CTAs of an attention launch, one per SM (148 on a B200)
 constexpr size_t WORK_HEAD = 1024;     // counters at the head of the work buffer
@@ -24,6 +26,48 @@ int launched(const char* what) {
   if (e == cudaSuccess) return VP_OK;
   vp_set_last_error(std::string(what) + ": " + cudaGetErrorString(e));
   return VP_ERR_CUDA;
+}
+
+bool off16(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
+
+int check_cache(const vp_paged* c) {
+  if (!c) return pfail(VP_ERR_ARG, "null cache");
+  if (c->type != VP_T_F16 && c->type != VP_T_BF16) return pfail(VP_ERR_ARG, "the cache's type must be f16 or bf16");
+  if (c->head_dim != 64 && c->head_dim != 128) return pfail(VP_ERR_ARG, "head_dim must be 64 or 128");
+  if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
+    return pfail(VP_ERR_ARG, "page_size must be 16, 32, 64, 128 or 256");
+  if (c->n_kv < 1 || c->n_kv > 4096) return pfail(VP_ERR_ARG, "n_kv out of range");
+  if (c->n_pages < 1 || c->n_seqs < 0 || c->max_pages < 1 || (long long)c->max_pages * c->page_size > (1 << 30))
+    return pfail(VP_ERR_ARG, "n_pages, n_seqs or max_pages out of range");
+  if (!c->k || !c->v || !c->table) return pfail(VP_ERR_ARG, "null pool or table");
+  if (off16(c->k) || off16(c->v)) return pfail(VP_ERR_ARG, "pools must be 16-byte aligned");
+  const int64_t s[3] = {c->page_stride, c->head_stride, c->slot_stride};
+  for (int64_t x : s)
+    if (x <= 0 || x % 8 || x >= (1ll << 39)) return pfail(VP_ERR_ARG, "pool strides must be positive multiples of 8 elements below 2^39");
+  if (c->table_stride < c->max_pages) return pfail(VP_ERR_ARG, "table_stride below max_pages");
+  return VP_OK;
+}
+
+bool bad_strides(int64_t a, int64_t b, int unit) { return a % unit || b % unit; }
+
+int check_attn(const vp_paged* c, const vp_paged_attn* a) {
+  if (const int e = check_cache(c)) return e;
+  if (!a) return pfail(VP_ERR_ARG, "null arguments");
+  if (a->n < 0 || a->rows < 0 || a->n > (1 << 24)) return pfail(VP_ERR_ARG, "n or rows out of range");
+  if (a->n_q < 1 || a->n_q % c->n_kv) return pfail(VP_ERR_ARG, "n_q must be a multiple of n_kv");
+  if (a->n_q / c->n_kv > PG_MAX_GROUP) return pfail(VP_ERR_ARG, "more than 64 query heads per cache head");
+  if (a->window < 0 || a->sinks < 0) return pfail(VP_ERR_ARG, "window and sinks must not be negative");
+  if (!(a->scale > 0.f && a->scale < 3e38f)) return pfail(VP_ERR_ARG, "scale must be positive and finite");
+  if (a->n == 0 || a->rows == 0) return VP_OK;
+  if (!a->q || !a->out || !a->lens) return pfail(VP_ERR_ARG, "null q, out or lens");
+  if (off16(a->q) || off16(a->out)) return pfail(VP_ERR_ARG, "q and out must be 16-byte aligned");
+  if (bad_strides(a->q_row, a->q_head, 8) || bad_strides(a->out_row, a->out_head, 8) ||
+      bad_strides(a->q_seq, a->out_seq, 8))
+    return pfail(VP_ERR_ARG, "strides of q and out must be multiples of 8 elements");
+  if (!a->work || (reinterpret_cast<uintptr_t>(a->work) & 255)) return pfail(VP_ERR_ARG, "work must be 256-byte aligned");
+  if (a->work_bytes < vp_paged_work_bytes(c->head_dim, a->n_q, c->n_kv, a->rows < PG_MAX_ROWS ? a->rows : PG_MAX_ROWS))
+    return pfail(VP_ERR_ARG, "work is smaller than vp_paged_work_bytes");
+  return VP_OK;
 }
 
 // SMs of the current device, at most PG_MAX_CTAS.

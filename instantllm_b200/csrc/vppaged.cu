@@ -126,85 +126,9 @@ __global__ void __launch_bounds__(APPEND_THREADS) k_paged_append(const vp_paged 
   }
 }
 
-// ---- attention of prompts, one warp per row and query head ----
-// The running maximum and sum of the softmax over 32 slots at a time: lane i scores slot i, then
-// every lane adds the 32 weighted values of its own HD / 32 elements.
-template <typename T, int HD>
-__global__ void k_paged_prompt(const vp_paged c, const vp_paged_attn a) {
-  constexpr int E = HD / 32;
-  const int lane = threadIdx.x & 31;
-  const long long w = blockIdx.x * (long long)(blockDim.x / 32) + threadIdx.x / 32;
-  const int h = (int)(w % a.n_q);
-  const long long row = w / a.n_q;
-  if (row >= a.rows) return;
-  int i = 0;
-  while (i < a.n && a.q_start[i + 1] <= row) ++i;
-  if (i == a.n || a.q_start[i] > row) return;
-  const int r = (int)row - a.q_start[i], n_new = a.q_start[i + 1] - a.q_start[i];
-  const PgSeq s = pg_seq(c, a.seqs, a.lens, i);
-  const int at = s.len - n_new + r, end = at < 0 ? 0 : at + 1;
-  const T* q = static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
-  const int hk = h / (a.n_q / c.n_kv);
-  float m = -INFINITY, l = 0.f, o[E] = {};
-  for (int j0 = 0; j0 < end; j0 += 32) {
-    const int j = j0 + lane;
-    const bool see = j < end && (!a.window || at - j < a.window || j < a.sinks);
-    float sc = -INFINITY;
-    int page = -1;
-    if (see) {
-      page = s.pages[j / c.page_size];
-      if (page < 0 || page >= c.n_pages) pg_status(c.status, VP_DEV_ERR_PAGE), page = -1;
-      sc = 0.f;
-      if (page >= 0) {
-        const T* k = static_cast<const T*>(c.k) + page * c.page_stride + hk * c.head_stride + (j % c.page_size) * c.slot_stride;
-        for (int d = 0; d < HD; ++d) sc += (float)q[d] * (float)k[d];
-      }
-      sc *= a.scale;
-    }
-    const float mn = fmaxf(m, warp_max(sc));
-    if (mn == -INFINITY) continue;
-    const float f = expf(m - mn), p = expf(sc - mn);
-    l = l * f + warp_sum(p);
-    m = mn;
-    for (int e = 0; e < E; ++e) o[e] *= f;
-    for (int t = 0; t < 32; ++t) {
-      const float pt = __shfl_sync(0xffffffffu, p, t);
-      const int pg = __shfl_sync(0xffffffffu, see ? page : -1, t);
-      if (pg < 0) continue;
-      const T* v = static_cast<const T*>(c.v) + pg * c.page_stride + hk * c.head_stride + ((j0 + t) % c.page_size) * c.slot_stride;
-      for (int e = 0; e < E; ++e) o[e] += pt * (float)v[lane + 32 * e];
-    }
-  }
-  T* out = static_cast<T*>(a.out) + row * a.out_row + h * a.out_head;
-  for (int e = 0; e < E; ++e) out[lane + 32 * e] = (T)(l > 0.f ? o[e] / l : 0.f);
-  if (a.lse && lane == 0) a.lse[row * a.n_q + h] = l > 0.f ? m + logf(l) : -INFINITY;
-}
-
 }  // namespace vp
 
 namespace {
-
-bool off16(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
-
-int check_cache(const vp_paged* c) {
-  if (!c) return pfail(VP_ERR_ARG, "null cache");
-  if (c->type != VP_T_F16 && c->type != VP_T_BF16) return pfail(VP_ERR_ARG, "the cache's type must be f16 or bf16");
-  if (c->head_dim != 64 && c->head_dim != 128) return pfail(VP_ERR_ARG, "head_dim must be 64 or 128");
-  if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
-    return pfail(VP_ERR_ARG, "page_size must be 16, 32, 64, 128 or 256");
-  if (c->n_kv < 1 || c->n_kv > 4096) return pfail(VP_ERR_ARG, "n_kv out of range");
-  if (c->n_pages < 1 || c->n_seqs < 0 || c->max_pages < 1 || (long long)c->max_pages * c->page_size > (1 << 30))
-    return pfail(VP_ERR_ARG, "n_pages, n_seqs or max_pages out of range");
-  if (!c->k || !c->v || !c->table) return pfail(VP_ERR_ARG, "null pool or table");
-  if (off16(c->k) || off16(c->v)) return pfail(VP_ERR_ARG, "pools must be 16-byte aligned");
-  const int64_t s[3] = {c->page_stride, c->head_stride, c->slot_stride};
-  for (int64_t x : s)
-    if (x <= 0 || x % 8 || x >= (1ll << 39)) return pfail(VP_ERR_ARG, "pool strides must be positive multiples of 8 elements below 2^39");
-  if (c->table_stride < c->max_pages) return pfail(VP_ERR_ARG, "table_stride below max_pages");
-  return VP_OK;
-}
-
-bool bad_strides(int64_t a, int64_t b, int unit) { return a % unit || b % unit; }
 
 template <typename TI, typename T>
 void append_launch(const vp_paged& c, const vp_paged_rows& r, cudaStream_t st) {
@@ -212,34 +136,6 @@ void append_launch(const vp_paged& c, const vp_paged_rows& r, cudaStream_t st) {
   const int threads = want < APPEND_THREADS ? (want + 31) / 32 * 32 : APPEND_THREADS;
   if (c.head_dim == 64) k_paged_append<TI, T, 64><<<r.rows, threads, 0, st>>>(c, r);
   else k_paged_append<TI, T, 128><<<r.rows, threads, 0, st>>>(c, r);
-}
-
-int check_attn(const vp_paged* c, const vp_paged_attn* a) {
-  if (const int e = check_cache(c)) return e;
-  if (!a) return pfail(VP_ERR_ARG, "null arguments");
-  if (a->n < 0 || a->rows < 0 || a->n > (1 << 24)) return pfail(VP_ERR_ARG, "n or rows out of range");
-  if (a->n_q < 1 || a->n_q % c->n_kv) return pfail(VP_ERR_ARG, "n_q must be a multiple of n_kv");
-  if (a->n_q / c->n_kv > PG_MAX_GROUP) return pfail(VP_ERR_ARG, "more than 64 query heads per cache head");
-  if (a->window < 0 || a->sinks < 0) return pfail(VP_ERR_ARG, "window and sinks must not be negative");
-  if (!(a->scale > 0.f && a->scale < 3e38f)) return pfail(VP_ERR_ARG, "scale must be positive and finite");
-  if (a->n == 0 || a->rows == 0) return VP_OK;
-  if (!a->q || !a->out || !a->lens) return pfail(VP_ERR_ARG, "null q, out or lens");
-  if (off16(a->q) || off16(a->out)) return pfail(VP_ERR_ARG, "q and out must be 16-byte aligned");
-  if (bad_strides(a->q_row, a->q_head, 8) || bad_strides(a->out_row, a->out_head, 8) ||
-      bad_strides(a->q_seq, a->out_seq, 8))
-    return pfail(VP_ERR_ARG, "strides of q and out must be multiples of 8 elements");
-  if (!a->work || (reinterpret_cast<uintptr_t>(a->work) & 255)) return pfail(VP_ERR_ARG, "work must be 256-byte aligned");
-  if (a->work_bytes < vp_paged_work_bytes(c->head_dim, a->n_q, c->n_kv, a->rows < PG_MAX_ROWS ? a->rows : PG_MAX_ROWS))
-    return pfail(VP_ERR_ARG, "work is smaller than vp_paged_work_bytes");
-  return VP_OK;
-}
-
-template <typename T>
-void prompt_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
-  const long long warps = (long long)a.rows * a.n_q;
-  const unsigned grid = (unsigned)((warps + 3) / 4);
-  if (c.head_dim == 64) k_paged_prompt<T, 64><<<grid, 128, 0, st>>>(c, a);
-  else k_paged_prompt<T, 128><<<grid, 128, 0, st>>>(c, a);
 }
 
 template <typename T, int HD>
@@ -317,18 +213,6 @@ int vp_paged_decode(const vp_paged* c, const vp_paged_attn* a, void* stream) try
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (c->type == VP_T_F16) return c->head_dim == 64 ? decode_launch<__half, 64>(*c, *a, st) : decode_launch<__half, 128>(*c, *a, st);
   return c->head_dim == 64 ? decode_launch<__nv_bfloat16, 64>(*c, *a, st) : decode_launch<__nv_bfloat16, 128>(*c, *a, st);
-} catch (const std::exception&) {
-  return VP_ERR_NOMEM;
-}
-
-int vp_paged_prefill(const vp_paged* c, const vp_paged_attn* a, void* stream) try {
-  if (const int e = check_attn(c, a)) return e;
-  if (a->n == 0 || a->rows == 0) return VP_OK;
-  if (!a->q_start) return pfail(VP_ERR_ARG, "null q_start");
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (c->type == VP_T_F16) prompt_launch<__half>(*c, *a, st);
-  else prompt_launch<__nv_bfloat16>(*c, *a, st);
-  return launched("vp_paged_prefill");
 } catch (const std::exception&) {
   return VP_ERR_NOMEM;
 }
