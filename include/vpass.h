@@ -405,8 +405,9 @@ int vp_paged_append(const vp_paged* c, const vp_paged_rows* r, void* stream);
  *   to its own (all of them new, or a chunk over a cached prefix).
  * window > 0: a row at position p sees a slot at position j only if p - j < window or j < sinks.
  * seqs (NULL: i) names request i's row of the table. Rows before a request's first slot (more rows
- * than its length) see nothing. Strides as above; lse is dense. work: vp_paged_work_bytes(...) bytes,
- * 256-byte aligned, zeroed once before its first use (each call leaves it ready for the next); calls
+ * than its length) see nothing; rows of q that no request has are left alone in out. Strides as above;
+ * lse is dense. work: vp_paged_work_bytes(..., rows of the call) bytes, 256-byte aligned, the first
+ * VP_PAGED_WORK_ZEROED of them zeroed once before its first use (each call leaves them zero); calls
  * that share it must not overlap on the GPU. Results depend on the inputs alone, not on timing.
  *   limits   n_q a multiple of n_kv, n_q / n_kv <= 64; sinks >= 0, window >= 0. */
 typedef struct {
@@ -420,6 +421,7 @@ typedef struct {
   float scale;
   int32_t n, rows, n_q, window, sinks;
 } vp_paged_attn;
+#define VP_PAGED_WORK_ZEROED 8192
 size_t vp_paged_work_bytes(int32_t head_dim, int32_t n_q, int32_t n_kv, int32_t rows);
 int vp_paged_decode(const vp_paged* c, const vp_paged_attn* a, void* stream);
 int vp_paged_prefill(const vp_paged* c, const vp_paged_attn* a, void* stream);

@@ -46,14 +46,28 @@ __device__ __forceinline__ bool pg_sees(int slot, int len, int base, uint32_t bi
   return !window || base + __popc(bits) - 1 - place < window || place < sinks;
 }
 
-// One box of a pool into shared memory: 64 elements from d of `rows` slots from `slot` of a page (the
-// map's box), 128 bytes a slot with the 128-byte swizzle: the 16-byte piece i of line l lies at piece
-// i ^ (l & 7). Coordinates outside the pool fill zeros. All coordinates of d are multiples of 64.
-__device__ __forceinline__ void pg_box(void* dst, const CUtensorMap* map, int d, int slot, int head, int page, uint64_t* bar) {
+// One box of a pool into shared memory: the map's box of slots from `slot` of a page, in panels of 64
+// elements, 128 bytes a slot with the 128-byte swizzle: the 16-byte piece i of line l lies at piece
+// i ^ (l & 7). pg_box: one panel of the box; pg_box5: all its panels. A page outside the pool fills zeros.
+__device__ __forceinline__ void pg_box(void* dst, const CUtensorMap* map, int panel, int slot, int head, int page, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-      ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(d), "r"(slot), "r"(head), "r"(page)
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(0), "r"(slot), "r"(panel), "r"(head), "r"(page)
       : "memory");
+}
+__device__ __forceinline__ void pg_box5(void* dst, const CUtensorMap* map, int slot, int head, int page, uint64_t* bar) {
+  pg_box(dst, map, 0, slot, head, page, bar);
+}
+__device__ __forceinline__ void pg_prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+// 16 bytes global -> shared without a register; pg_cp_arrive: the barrier counts this thread once its
+// copies so far are there.
+__device__ __forceinline__ void pg_cp16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void pg_cp_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void pg_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");

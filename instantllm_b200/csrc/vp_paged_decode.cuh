@@ -1,52 +1,54 @@
-// Attention of the newest rows of many requests over the paged cache (vp_paged_decode).
+// Attention of the newest rows of many requests over the paged cache (vp_paged_decode), up to 16 query
+// rows (heads of a group x new rows) per cache head; more go to the tensor-memory kernel.
 //
-// Mathematics. Per request, cache head and block of query rows: S = scale q K^T over the visible slots,
+// Mathematics. Per request and cache head: S = scale q K^T over the visible slots,
 // p = 2^(S log2 e - m) with the running maximum m, l = sum p, o = sum p v; two such records (m, l, o)
 // over disjoint slots join as m* = max, l* = sum l 2^(m - m*), o* likewise, and out = o / l.
 //
-// Bound: the bytes of K and V, each read once. So the query rows of one cache head (G heads x R
-// rows, packed as m = r G + g, up to 128 per block) share one read of the cache, and the work is cut
-// into tiles of 16 KB (64 slots of 64, 32 of 128) dealt out evenly: the tiles of all (request, row
-// block, head) pairs are numbered in order, and CTA c of G' takes tiles [c N / G', (c + 1) N / G').
-// One CTA per SM: a producer warp keeps a ring of tiles in flight (TMA boxes of one page each), eight
-// consumer warps compute on mma.sync. MT warps hold the 16-row tiles of the block; the 8 / MT groups of
-// them take turns over the tiles, so that no CTA barrier stands in the loop: a warp waits for its
-// tile, computes and frees it. At the end of a pair's run the groups join in shared memory. A pair
-// that several CTAs share leaves records in the work buffer; the CTA that finishes last (a counter
-// per first CTA, back at zero afterwards) joins them in the order of the slots, so results do not
-// depend on which CTA that is.
+// Bound: the bytes of K and V, each read once, and for small calls the chain of dependent reads
+// (length, page, K, V). So the query rows of one cache head (G heads x R rows, packed as m = r G + g)
+// share one read of the cache, and the work is cut into tiles of 8 KB (32 slots of 64, 16 of 128)
+// dealt out evenly: the tiles of all (request, head) pairs are numbered in order and every CTA takes
+// the same number of consecutive ones. One CTA per SM, two roles:
+//  * eight consumer warps take turns over the tiles. Each has two stages of its own and refills a
+//    stage itself (TMA boxes of one page each) once it has computed on it (mma.sync), so the warps never
+//    wait for one another;
+//  * three joiner warps bring the queries of the next pair, and at the end of a pair's run add up the
+//    warps' records while the warps are on the next pair. A pair that several CTAs share leaves records
+//    in the work buffer; the CTA that finishes last (a counter per first CTA, back at zero afterwards)
+//    joins them in the order of the slots, so results do not depend on which CTA that is.
 #pragma once
 #include "vp_paged.cuh"
 
 namespace vp {
 
 constexpr int DC_WARPS = 8;                         // consumer warps
-constexpr int DC_THREADS = (DC_WARPS + 1) * 32;     // and the producer
-constexpr int DC_BLOCK_ROWS = DC_WARPS * 16;        // packed query rows per block
-constexpr int DC_TILE = 8192;                       // bytes of K (and of V) per tile
+constexpr int DC_JOINERS = 96;                      // threads
+constexpr int DC_THREADS = DC_WARPS * 32 + DC_JOINERS;
+constexpr int DC_ROWS = 16;                         // packed query rows of a pair
+constexpr int DC_TILE = 4096;                       // bytes of K (and of V) per tile
+constexpr int DC_STAGES = 2;                        // per warp
 constexpr int DC_LENS = 2048;                       // lengths kept in shared memory
 
 template <int HD>
 struct DcShape {
   static constexpr int TS = DC_TILE / (HD * 2);     // slots per tile
   static constexpr int PITCH = HD + 4;              // floats per row of the join buffer
-  // a multiple of every number of groups (8, 4, 2, 1): a stage then always goes to the same group,
-  // whose warps saw its previous tile. A warp that came to a stage whose previous tile, another
-  // group's, is still on its way would take that phase's parity for its own.
-  static constexpr int STAGES = DC_WARPS;
-  static constexpr size_t RING = (size_t)STAGES * 2 * DC_TILE;
-  static constexpr size_t JOIN = (size_t)DC_BLOCK_ROWS * PITCH * 4;
-  static constexpr size_t SMEM = 1024 + RING + JOIN + DC_BLOCK_ROWS * 8 + DC_LENS * 4;
-  // floats of one record: DC_BLOCK_ROWS rows at most, o then m then l; a multiple of 16 bytes
-  static __host__ __device__ constexpr size_t record(int rows) { return ((size_t)rows * (HD + 2) + 3) / 4 * 4; }
+  static constexpr int QBUF = DC_ROWS * HD * 2;
+  static constexpr size_t RING = (size_t)DC_WARPS * DC_STAGES * 2 * DC_TILE;
+  static constexpr size_t JOIN = (size_t)DC_WARPS * DC_ROWS * PITCH * 4;
+  static constexpr size_t SMEM = 1024 + RING + 2 * QBUF + JOIN + DC_WARPS * DC_ROWS * 8 + DC_LENS * 4;
 };
+
+// Floats of one record of `rows` rows: o, then m, then l; a multiple of 16 bytes.
+__host__ __device__ constexpr size_t pg_record(int rows, int hd) { return ((size_t)rows * (hd + 2) + 3) / 4 * 4; }
 
 struct DcParams {
   vp_paged c;
   vp_paged_attn a;
-  float* rec;         // [grid][2] records of min(M, 128) rows
+  float* rec;         // [grid][2] records of M rows
   unsigned* tickets;  // [grid]
-  int group, blocks, block_rows, mt, min_tiles;  // G, row blocks per pair, rows of a full block, 16-row tiles of one, tiles per CTA
+  int group, M, min_tiles, page_shift;  // G, G R, fewest tiles per CTA, log2 of the page size
 };
 
 // Slots of a request that the rows of a call see, as tiles: [0, ns) hold the sinks, [ws, end) the rest.
@@ -68,72 +70,138 @@ __device__ __forceinline__ DcSpan dc_span(int len, int rows, int window, int sin
   return s;
 }
 
-__device__ __forceinline__ void dc_bar() {  // the consumer warps
-  __syncwarp();
-  asm volatile("barrier.sync 1, 256;" ::: "memory");
+// Even shares of N tiles: the first N % G of G CTAs take one more.
+struct PgShare {
+  int per, more;
+  __device__ __forceinline__ PgShare(int N, int G) : per(N / G), more(N % G) {}
+  __device__ __forceinline__ int first(int c) const { return c * per + min(c, more); }
+  __device__ __forceinline__ int owner(int t) const {
+    const int big = more * (per + 1);
+    return t < big ? t / (per + 1) : more + (t - big) / per;
+  }
+};
+
+// Bits a .. b - 1 of a tile's 64 (all relative to its first slot).
+__device__ __forceinline__ uint64_t dc_bits(int a, int b) {
+  const uint64_t hi = b >= 64 ? ~0ull : b <= 0 ? 0ull : (1ull << b) - 1;
+  const uint64_t lo = a >= 64 ? ~0ull : a <= 0 ? 0ull : (1ull << a) - 1;
+  return hi & ~lo;
 }
+// Slots of a tile that a row sees: the old ones [lo, base) and the sinks, and its new ones.
+__device__ __forceinline__ uint64_t dc_seen(int s0, int base, int lo, int sinks, uint32_t bits) {
+  const int b = base - s0;
+  const uint64_t fresh = b >= 64 ? 0ull : b >= 0 ? (uint64_t)bits << b : b > -32 ? (uint64_t)(bits >> -b) : 0ull;
+  return dc_bits(lo - s0, b) | dc_bits(-s0, min(sinks - s0, b)) | fresh;
+}
+
+// Named barriers between consumers and joiners: the join buffer is filled, is free.
+constexpr int DC_FILLED = 2, DC_FREE = 3;
+__device__ __forceinline__ void dc_sync(int bar) {
+  __syncwarp();
+  asm volatile("barrier.sync %0, 352;" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void dc_arrive(int bar) {
+  __threadfence_block();
+  __syncwarp();
+  asm volatile("barrier.arrive %0, 352;" ::"r"(bar) : "memory");
+}
+static_assert(DC_THREADS == 352, "barrier counts");
+
+// A walk over the CTA's tiles [t, t1): the request and head that tile t belongs to.
+template <int TS>
+struct DcWalk {
+  const DcParams& p;
+  const int* lens_s;
+  int seq, seq_at, t, t1;  // seq_at: number of seq's first tile
+  DcSpan sp;
+  int head, u;             // tile t is tile u of this head
+  __device__ __forceinline__ DcWalk(const DcParams& p_, const int* l, int s, int at, int t_, int t1_)
+      : p(p_), lens_s(l), seq(s), seq_at(at), t(t_), t1(t1_) {
+    span();
+  }
+  __device__ __forceinline__ void span() {
+    const int len = seq < DC_LENS ? lens_s[seq] : pg_seq(p.c, p.a.seqs, p.a.lens, seq).len;
+    sp = dc_span<TS>(len, p.a.rows, p.a.window, p.a.sinks);
+  }
+  __device__ __forceinline__ bool find() {
+    if (t >= t1) return false;
+    while (t >= seq_at + sp.tiles * p.c.n_kv) {
+      seq_at += sp.tiles * p.c.n_kv;
+      ++seq;
+      span();
+    }
+    head = (t - seq_at) / sp.tiles;
+    u = t - seq_at - head * sp.tiles;
+    return true;
+  }
+  __device__ __forceinline__ int run() const { return min(sp.tiles - u, t1 - t); }  // tiles of this head from t on
+  __device__ __forceinline__ int slot(int v) const { return (v < sp.ns ? v : sp.ws + v - sp.ns) * TS; }
+};
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(DC_THREADS, 1)
     k_paged_decode(const __grid_constant__ DcParams p, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
   using Sh = DcShape<HD>;
-  constexpr int TS = Sh::TS, ST = Sh::STAGES, NT = TS / 8, KS = HD / 16, PITCH = Sh::PITCH;
+  constexpr int TS = Sh::TS, NT = TS / 8, KS = HD / 16, PITCH = Sh::PITCH, QP = DC_ROWS * 128;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* ring = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  float* join = reinterpret_cast<float*>(ring + Sh::RING);
-  float2* join_ml = reinterpret_cast<float2*>(join + DC_BLOCK_ROWS * PITCH);
-  int* lens_s = reinterpret_cast<int*>(join_ml + DC_BLOCK_ROWS);
-  __shared__ uint64_t full[ST], empty[ST];
-  __shared__ long long warp_sums[DC_THREADS / 32];
-  __shared__ int first_seq, dead, last_flag;
-  __shared__ long long first_tile;  // number of first_seq's first tile
+  unsigned char* qbuf = ring + Sh::RING;
+  float* join = reinterpret_cast<float*>(qbuf + 2 * Sh::QBUF);
+  float2* join_ml = reinterpret_cast<float2*>(join + DC_WARPS * DC_ROWS * PITCH);
+  int* lens_s = reinterpret_cast<int*>(join_ml + DC_WARPS * DC_ROWS);
+  __shared__ uint64_t full[DC_WARPS][DC_STAGES], q_full[2];
+  __shared__ int warp_sums[DC_THREADS / 32];
+  __shared__ int first_seq, first_tile, dead, last_flag;  // first_tile: number of first_seq's first tile
 
   const vp_paged& c = p.c;
   const vp_paged_attn& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rows = a.rows, per_seq = c.n_kv * p.blocks;  // pairs per request
+  const int rows = a.rows;
 
-  if (tid == 0) {
-    for (int i = 0; i < ST; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], p.mt);
-    }
-    fence_barrier_init();
-    dead = 0;
+  pdl_launch_dependents();
+  if (tid < DC_WARPS * DC_STAGES) mbar_init(&full[0][0] + tid, 1);
+  if (tid < 2) mbar_init(&q_full[tid], DC_JOINERS);
+  if (tid == 0) dead = 0;
+  if (tid < 32) fence_barrier_init();
+  for (int i = tid; i < 2 * Sh::QBUF / 16; i += DC_THREADS) reinterpret_cast<uint4*>(qbuf)[i] = make_uint4(0, 0, 0, 0);
+  if (tid == 32) {
+    pg_prefetch_map(&mk);
+    pg_prefetch_map(&mv);
   }
+  pdl_wait();
+
   // tiles of all requests: every thread counts a run of them, then a scan over the CTA
-  const int run = (a.n + DC_THREADS - 1) / DC_THREADS;
-  const int i0 = min(a.n, tid * run), i1 = min(a.n, i0 + run);
-  long long mine = 0;
+  const int chunk = (a.n + DC_THREADS - 1) / DC_THREADS;
+  const int i0 = min(a.n, tid * chunk), i1 = min(a.n, i0 + chunk);
+  int mine = 0;
   for (int i = i0; i < i1; ++i) {
     const int len = pg_seq(c, a.seqs, a.lens, i).len;
     if (i < DC_LENS) lens_s[i] = len;
-    mine += (long long)dc_span<TS>(len, rows, a.window, a.sinks).tiles * per_seq;
+    mine += dc_span<TS>(len, rows, a.window, a.sinks).tiles * c.n_kv;
   }
-  long long incl = mine;
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
   if (lane == 31) warp_sums[warp] = incl;
   cta_sync();
-  long long before = 0, N = 0;
+  int before = 0, N = 0;
 #pragma unroll
   for (int w = 0; w < DC_THREADS / 32; ++w) {
     if (w < warp) before += warp_sums[w];
     N += warp_sums[w];
   }
-  const long long want = (N + p.min_tiles - 1) / p.min_tiles;
-  const int G = (int)(want < (long long)gridDim.x ? want : (long long)gridDim.x);
-  const int cta = blockIdx.x;
+  const int G = min((N + p.min_tiles - 1) / p.min_tiles, (int)gridDim.x), cta = blockIdx.x;
   if (cta >= G) return;
-  const long long t0 = cta * N / G, t1 = (cta + 1) * N / G;
-  long long at = before + incl - mine;
+  const PgShare share(N, G);
+  const int t0 = share.first(cta), t1 = share.first(cta + 1);
+  int at = before + incl - mine;
   if (at <= t0 && t0 < at + mine) {
     for (int i = i0; i < i1; ++i) {
       const int len = i < DC_LENS ? lens_s[i] : pg_seq(c, a.seqs, a.lens, i).len;
-      const long long n = (long long)dc_span<TS>(len, rows, a.window, a.sinks).tiles * per_seq;
+      const int n = dc_span<TS>(len, rows, a.window, a.sinks).tiles * c.n_kv;
       if (t0 < at + n) {
         first_seq = i;
         first_tile = at;
@@ -144,305 +212,313 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
   }
   cta_sync();
 
-  // the CTA's runs: (request, pair, tiles [u0, u1) of the pair), the same walk in every warp
-  int seq = first_seq;
-  long long seq_at = first_tile, t = t0;
-  const int box = min(c.page_size, TS), boxes = TS / box;
-
-  if (warp == DC_WARPS) {  // producer
-    const int per_batch = 32 / boxes;
-    uint32_t n_issued = 0;
-    bool ok = true;
-    while (t < t1 && ok) {
-      const PgSeq s = pg_seq(c, a.seqs, a.lens, seq);
-      const DcSpan sp = dc_span<TS>(s.len, rows, a.window, a.sinks);
-      const long long end = seq_at + (long long)sp.tiles * per_seq;
-      while (t < t1 && t < end && ok) {
-        const int pair = (int)((t - seq_at) / sp.tiles), u0 = (int)((t - seq_at) % sp.tiles);
-        const int n = (int)min((long long)(sp.tiles - u0), t1 - t);
-        const int head = pair % c.n_kv;
-        for (int b = 0; b < n && ok; b += per_batch) {
-          // lane: tile b + lane / boxes of the run, box lane % boxes
-          const int u = u0 + b + lane / boxes;
-          const int slot = (u < sp.ns ? u : sp.ws + u - sp.ns) * TS + (lane % boxes) * box;
-          int page = c.n_pages;  // a box that nobody sees fills zeros
-          if (b + lane / boxes < n && slot < s.len && (slot + box > sp.lo || slot < a.sinks)) {
-            page = s.pages[slot / c.page_size];
-            if (page < 0 || page >= c.n_pages) {
-              pg_status(c.status, VP_DEV_ERR_PAGE);
-              page = c.n_pages;
-            }
-          }
-          const int m = min(per_batch, n - b);
-          for (int k = 0; k < m; ++k) {
-            const int st = n_issued % ST;
-            if (n_issued >= ST && !mbar_wait_warp(&empty[st], (n_issued / ST - 1) & 1)) {
-              pg_status(c.status, VP_DEV_ERR_TIMEOUT);
-              ok = false;
-              break;
-            }
-            if (lane == 0) mbar_arrive_expect_tx(&full[st], 2 * DC_TILE);
-            __syncwarp();
-            if (lane / boxes == k) {
-              unsigned char* dst = ring + (size_t)st * 2 * DC_TILE + (lane % boxes) * box * 128;
-#pragma unroll
-              for (int d = 0; d < HD / 64; ++d) {
-                pg_box(dst + d * TS * 128, &mk, d * 64, slot % c.page_size, head, page, &full[st]);
-                pg_box(dst + DC_TILE + d * TS * 128, &mv, d * 64, slot % c.page_size, head, page, &full[st]);
-              }
-            }
-            ++n_issued;
-          }
-        }
-        t += n;
-      }
-      seq_at = end;
-      ++seq;
+  // Waits of a whole warp; after one that ran out none waits any more, and the call ends with an error status.
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    __syncwarp();
+    if (!*(volatile int*)&dead && !mbar_wait_warp(bar, parity)) {
+      pg_status(c.status, VP_DEV_ERR_TIMEOUT);
+      *(volatile int*)&dead = 1;
     }
-    return;
-  }
+    __syncwarp();
+  };
 
-  // consumers
-  const int mt = warp % p.mt, ks = warp / p.mt, groups = DC_WARPS / p.mt;
-  const bool active = ks < groups;
-  const int g = lane >> 2, q4 = lane & 3;
-  const float cexp = a.scale * 1.4426950408889634f;
-  uint32_t n_seen = 0;  // tiles of the CTA so far
-  while (t < t1) {
-    const int len = seq < DC_LENS ? lens_s[seq] : pg_seq(c, a.seqs, a.lens, seq).len;
-    const DcSpan sp = dc_span<TS>(len, rows, a.window, a.sinks);
-    const long long end = seq_at + (long long)sp.tiles * per_seq;
-    while (t < t1 && t < end) {
-      const int pair = (int)((t - seq_at) / sp.tiles), u0 = (int)((t - seq_at) % sp.tiles);
-      const int n = (int)min((long long)(sp.tiles - u0), t1 - t);
-      const int head = pair % c.n_kv, m0 = pair / c.n_kv * DC_BLOCK_ROWS;
-      const int M = min(rows * p.group - m0, DC_BLOCK_ROWS);
-      // masks of the request's rows (lane r: row r), this thread's two rows
+  if (warp < DC_WARPS) {
+    // ---- consumers: warp w has tiles t0 + w, t0 + w + 8, ... ----
+    const int g = lane >> 2, q4 = lane & 3;
+    const float cexp = a.scale * 1.4426950408889634f;
+    const uint32_t stage0 = smem_u32(ring) + warp * DC_STAGES * 2 * DC_TILE;
+    // loads run ahead of the computation: `ahead` stands at the tile to fetch next, lane b < boxes has
+    // the page of its box b already
+    const int box = min(c.page_size, TS), boxes = TS / box;
+    DcWalk<TS> ahead(p, lens_s, first_seq, first_tile, t0 + warp, t1);
+    int page = c.n_pages, slot = 0;
+    auto look = [&] {  // page of this lane's box of the tile at `ahead`; one that nobody sees fills zeros
+      page = c.n_pages;
+      if (!ahead.find()) return;
+      slot = ahead.slot(ahead.u) + lane * box;
+      if (lane < boxes && slot < ahead.sp.len && (slot + box > ahead.sp.lo || slot < a.sinks)) {
+        const int s = a.seqs ? a.seqs[ahead.seq] : ahead.seq;  // a request outside the table has no slots
+        page = c.table[s * c.table_stride + (slot >> p.page_shift)];
+      }
+    };
+    auto fetch = [&](int st) {  // the tile at `ahead` into stage st
+      if (ahead.t >= t1) return;
+      if (lane == 0) mbar_arrive_expect_tx(&full[warp][st], 2 * DC_TILE);
+      __syncwarp();
+      if (lane < boxes) {
+        if (page < 0 || page > c.n_pages || (page == c.n_pages && slot < ahead.sp.len && (slot + box > ahead.sp.lo || slot < a.sinks))) {
+          pg_status(c.status, VP_DEV_ERR_PAGE);
+          page = c.n_pages;
+        }
+        unsigned char* dst = ring + (size_t)((warp * DC_STAGES + st) * 2) * DC_TILE + lane * box * 128;
+        pg_box5(dst, &mk, slot & (c.page_size - 1), ahead.head, page, &full[warp][st]);
+        pg_box5(dst + DC_TILE, &mv, slot & (c.page_size - 1), ahead.head, page, &full[warp][st]);
+      }
+      ahead.t += DC_WARPS;
+    };
+    look();
+#pragma unroll
+    for (int st = 0; st < DC_STAGES; ++st) {
+      fetch(st);
+      look();
+    }
+    uint32_t k_th = 0;  // tiles computed
+    int next = t0 + warp;
+    DcWalk<TS> w(p, lens_s, first_seq, first_tile, t0, t1);
+    for (int r = 0; w.find(); ++r) {
+      const DcSpan& sp = w.sp;
+      const int n = w.run(), seq = w.seq;
+      // masks of the request's rows (lane i: row i); this thread's two rows, and their union
       uint32_t anc = 0;
       if (lane < rows)
         anc = a.mask ? (uint32_t)a.mask[(long long)seq * rows + lane] & ((1u << rows) - 1) : (2u << lane) - 1;
-      uint32_t any = anc;
-      int least = lane < rows ? __popc(anc) : 32;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        any |= __shfl_xor_sync(0xffffffffu, any, o);
-        least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
-      }
-      const int first_seen = a.window ? sp.base + least - a.window : 0;  // beside the sinks, by any row
-      uint32_t qf[KS][4];
       uint32_t bits[2];
+      int lo[2];  // first old slot beside the sinks that the row sees
       bool there[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int m = mt * 16 + g + 8 * h, r = (m0 + m) / p.group;
-        there[h] = m < M && sp.base + r >= 0;
-        bits[h] = __shfl_sync(0xffffffffu, anc, min(r, 31));
-        const T* q = static_cast<const T*>(a.q) + seq * a.q_seq + r * a.q_row + (head * p.group + (m0 + m) % p.group) * a.q_head;
+        const int m = g + 8 * h, row = m / p.group;
+        there[h] = m < p.M && sp.base + row >= 0;
+        bits[h] = __shfl_sync(0xffffffffu, anc, min(row, 31));
+        lo[h] = a.window ? sp.base + __popc(bits[h]) - a.window : 0;
+      }
+      const uint32_t any = __reduce_or_sync(0xffffffffu, anc);
+      const int least = __reduce_min_sync(0xffffffffu, lane < rows ? __popc(anc) : 32);
+      const int first_seen = a.window ? sp.base + least - a.window : 0;  // beside the sinks, by any row
+      if (a.window) {  // new slots that have left a row's window
+        uint32_t keep[2] = {0, 0};
+        for (int j = 0; j < rows; ++j) {
+          const int place = sp.base + __popc(__shfl_sync(0xffffffffu, anc, j)) - 1;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          qf[k][h] = m < M ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 2 * q4) : 0u;
-          qf[k][2 + h] = m < M ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 8 + 2 * q4) : 0u;
+          for (int h = 0; h < 2; ++h)
+            if (place >= lo[h] || place < a.sinks) keep[h] |= 1u << j;
         }
+        bits[0] &= keep[0];
+        bits[1] &= keep[1];
+      }
+      uint32_t qf[KS][4];
+      wait(&q_full[r & 1], (r >> 1) & 1);
+      {
+        const int m = lane & 15;
+        const uint32_t qa = smem_u32(qbuf) + (r & 1) * Sh::QBUF + m * 128;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) pg_ldsm(qf[k], qa + (k / 4) * QP + ((((k & 3) * 2 + (lane >> 4)) ^ (m & 7)) << 4));
       }
       float o[HD / 8][4] = {};
       float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-      if (active) {
-        for (int b = (ks + groups - (int)(n_seen % groups)) % groups; b < n; b += groups) {
-          const uint32_t k_th = n_seen + b;
-          const int st = k_th % ST, u = u0 + b;
-          const int s0 = (u < sp.ns ? u : sp.ws + u - sp.ns) * TS;
-          __syncwarp();
-          if (!*(volatile int*)&dead && !mbar_wait_warp(&full[st], (k_th / ST) & 1)) {
-            pg_status(c.status, VP_DEV_ERR_TIMEOUT);
-            *(volatile int*)&dead = 1;
-          }
-          __syncwarp();
-          const uint32_t kb = smem_u32(ring) + st * 2 * DC_TILE, vb = kb + DC_TILE;
-          float s[NT][4];
-          // lanes 0-7 .. 24-31 point at the lines of four 8 x 8 matrices: 8 slots, 32 elements
+      for (; next < w.t + n; next += DC_WARPS, ++k_th) {
+        const int st = k_th % DC_STAGES, s0 = w.slot(w.u + next - w.t);
+        wait(&full[warp][st], (k_th / DC_STAGES) & 1);
+        const uint32_t kb = stage0 + st * 2 * DC_TILE, vb = kb + DC_TILE;
+        float s[NT][4], s2[NT][4];
+        // lanes 0-7 .. 24-31 point at the lines of four 8 x 8 matrices: 8 slots, 32 elements; two sums
+        // side by side halve the chain of dependent products
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-            const int line = nt * 8 + (lane & 7);
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int k = 0; k < KS; k += 2) {
-              uint32_t f[4];
-              pg_ldsm(f, kb + (k / 4) * TS * 128 + line * 128 + ((((k & 3) * 2 + (lane >> 3)) ^ (line & 7)) << 4));
-              PgType<T>::mma(s[nt], qf[k], f[0], f[1]);
-              PgType<T>::mma(s[nt], qf[k + 1], f[2], f[3]);
-            }
+          for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.f;
+          const int line = nt * 8 + (lane & 7);
+#pragma unroll
+          for (int k = 0; k < KS; k += 2) {
+            uint32_t f[4];
+            pg_ldsm(f, kb + (k / 4) * TS * 128 + line * 128 + ((((k & 3) * 2 + (lane >> 3)) ^ (line & 7)) << 4));
+            PgType<T>::mma(s[nt], qf[k], f[0], f[1]);
+            PgType<T>::mma(s2[nt], qf[k + 1], f[2], f[3]);
           }
-          const bool whole = s0 + TS <= sp.base && (s0 >= sp.lo_all || s0 + TS <= a.sinks);
-          if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] += s2[nt][e];
+        }
+        const bool whole = s0 + TS <= sp.base && (s0 >= sp.lo_all || s0 + TS <= a.sinks);
+        if (!whole) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t see = there[h] ? (uint32_t)dc_seen(s0, sp.base, lo[h], a.sinks, bits[h]) >> (2 * q4) : 0u;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int slot = s0 + nt * 8 + 2 * q4 + (e & 1), h = e >> 1;
-                bool see = there[h] && slot < len;
-                int place = slot;
-                const int j = slot - sp.base;
-                const uint32_t aj = __shfl_sync(0xffffffffu, anc, j & 15);
-                if (j >= 0) {
-                  see = see && ((bits[h] >> (j & 31)) & 1);
-                  place = sp.base + __popc(aj) - 1;
-                }
-                if (a.window) see = see && (sp.base + __popc(bits[h]) - 1 - place < a.window || place < a.sinks);
-                if (!see) s[nt][e] = -INFINITY;
-              }
+              for (int e = 0; e < 2; ++e)
+                if (!((see >> (nt * 8 + e)) & 1)) s[nt][2 * h + e] = -INFINITY;
           }
-          float mn[2] = {mx[0], mx[1]};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mn[0] = fmaxf(mn[0], fmaxf(s[nt][0], s[nt][1]) * cexp);
-            mn[1] = fmaxf(mn[1], fmaxf(s[nt][2], s[nt][3]) * cexp);
-          }
-          float use[2], f[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            mn[h] = fmaxf(mn[h], __shfl_xor_sync(0xffffffffu, mn[h], 1));
-            mn[h] = fmaxf(mn[h], __shfl_xor_sync(0xffffffffu, mn[h], 2));
-            use[h] = mn[h] == -INFINITY ? 0.f : mn[h];
-            f[h] = pg_exp2(mx[h] - use[h]);
-            mx[h] = mn[h];
-            sum[h] *= f[h];
-          }
-#pragma unroll
-          for (int d = 0; d < HD / 8; ++d) {
-            o[d][0] *= f[0], o[d][1] *= f[0];
-            o[d][2] *= f[1], o[d][3] *= f[1];
-          }
-          uint32_t pf[TS / 16][4];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float e[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) e[i] = pg_exp2(fmaf(s[nt][i], cexp, -use[i >> 1]));
-            sum[0] += e[0] + e[1];
-            sum[1] += e[2] + e[3];
-            pf[nt / 2][(nt & 1) * 2] = PgType<T>::down(e[0], e[1]);
-            pf[nt / 2][(nt & 1) * 2 + 1] = PgType<T>::down(e[2], e[3]);
-          }
-#pragma unroll
-          for (int kk = 0; kk < TS / 16; ++kk) {
-            uint32_t w0 = 0xffffffffu, w1 = 0xffffffffu;
-            if (!whole) {  // values of slots that no row sees may be NaN: a zero weight does not silence those
-              w0 = w1 = 0;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int slot = s0 + kk * 16 + 2 * q4 + (e & 1) + (e >> 1) * 8;
-                const bool live = slot < len && (slot >= first_seen || slot < a.sinks) &&
-                                  (slot < sp.base || ((any >> ((slot - sp.base) & 31)) & 1));
-                if (live) (e >> 1 ? w1 : w0) |= e & 1 ? 0xffff0000u : 0xffffu;
-              }
-            }
-            const int line = kk * 16 + (lane & 15);
-#pragma unroll
-            for (int d = 0; d < HD / 16; ++d) {
-              uint32_t f4[4];
-              pg_ldsm_t(f4, vb + (d / 4) * TS * 128 + line * 128 + ((((d & 3) * 2 + (lane >> 4)) ^ (line & 7)) << 4));
-              PgType<T>::mma(o[2 * d], pf[kk], f4[0] & w0, f4[1] & w1);
-              PgType<T>::mma(o[2 * d + 1], pf[kk], f4[2] & w0, f4[3] & w1);
-            }
-          }
-          __syncwarp();
-          if (lane == 0) pg_arrive(&empty[st]);
         }
+        float mn[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mn[0] = fmaxf(mn[0], fmaxf(s[nt][0], s[nt][1]));
+          mn[1] = fmaxf(mn[1], fmaxf(s[nt][2], s[nt][3]));
+        }
+        float use[2], f[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-          sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-          const int m = warp * 16 + g + 8 * h;
+          mn[h] = fmaxf(mn[h], __shfl_xor_sync(0xffffffffu, mn[h], 1));
+          mn[h] = fmaxf(mn[h], __shfl_xor_sync(0xffffffffu, mn[h], 2));
+          mn[h] = fmaxf(mx[h], mn[h] * cexp);
+          use[h] = mn[h] == -INFINITY ? 0.f : mn[h];
+          f[h] = pg_exp2(mx[h] - use[h]);
+          mx[h] = mn[h];
+          sum[h] *= f[h];
+        }
+#pragma unroll
+        for (int d = 0; d < HD / 8; ++d) {
+          o[d][0] *= f[0], o[d][1] *= f[0];
+          o[d][2] *= f[1], o[d][3] *= f[1];
+        }
+        uint32_t pf[TS / 16][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float e[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) e[i] = pg_exp2(fmaf(s[nt][i], cexp, -use[i >> 1]));
+          sum[0] += e[0] + e[1];
+          sum[1] += e[2] + e[3];
+          pf[nt / 2][(nt & 1) * 2] = PgType<T>::down(e[0], e[1]);
+          pf[nt / 2][(nt & 1) * 2 + 1] = PgType<T>::down(e[2], e[3]);
+        }
+        // values of slots that no row sees may be NaN, which a zero weight does not silence
+        const uint32_t live = whole ? ~0u : (uint32_t)dc_seen(s0, sp.base, first_seen, a.sinks, any) >> (2 * q4);
+#pragma unroll
+        for (int kk = 0; kk < TS / 16; ++kk) {
+          uint32_t w0 = 0xffffffffu, w1 = 0xffffffffu;
+          if (!whole) {
+            const uint32_t x = live >> (kk * 16);
+            w0 = (x & 1 ? 0xffffu : 0u) | (x & 2 ? 0xffff0000u : 0u);
+            w1 = (x & 0x100 ? 0xffffu : 0u) | (x & 0x200 ? 0xffff0000u : 0u);
+          }
+          const int line = kk * 16 + (lane & 15);
+#pragma unroll
+          for (int d = 0; d < HD / 16; ++d) {
+            uint32_t f4[4];
+            pg_ldsm_t(f4, vb + (d / 4) * TS * 128 + line * 128 + ((((d & 3) * 2 + (lane >> 4)) ^ (line & 7)) << 4));
+            PgType<T>::mma(o[2 * d], pf[kk], f4[0] & w0, f4[1] & w1);
+            PgType<T>::mma(o[2 * d + 1], pf[kk], f4[2] & w0, f4[3] & w1);
+          }
+        }
+        __syncwarp();
+        fetch(st);
+        look();
+      }
+      if (r > 0) dc_sync(DC_FREE);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+        if (g + 8 * h < p.M) {
+          const int m = warp * DC_ROWS + g + 8 * h;
 #pragma unroll
           for (int d = 0; d < HD / 8; ++d)
             *reinterpret_cast<float2*>(join + m * PITCH + d * 8 + 2 * q4) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
           if (q4 == 0) join_ml[m] = make_float2(mx[h], sum[h]);
         }
       }
-      n_seen += n;
-      dc_bar();
+      dc_arrive(DC_FILLED);
+      w.t += n;
+    }
+    return;
+  }
 
-      // join the groups: item (row m of the block, 4 elements); group k's rows lie p.mt * 16 further on
-      const bool alone = n == sp.tiles;
-      const long long pair_at = seq_at + (long long)pair * sp.tiles;
-      const int c0 = (int)(((pair_at + 1) * G - 1) / N), c1 = (int)(((pair_at + sp.tiles) * G - 1) / N);
-      const size_t rec_floats = Sh::record(p.block_rows);
-      float* rec = p.rec + (size_t)(u0 == 0 ? 2 * cta + 1 : 2 * cta) * rec_floats;
-      auto finish = [&](bool to_out) {
-        for (int it = tid; it < M * (HD / 4); it += DC_WARPS * 32) {
-          const int m = it / (HD / 4), d = it % (HD / 4) * 4;
-          float top = -INFINITY;
-          for (int k = 0; k < groups; ++k) top = fmaxf(top, join_ml[k * p.mt * 16 + m].x);
-          const float use = top == -INFINITY ? 0.f : top;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          float l = 0.f;
-          for (int k = 0; k < groups; ++k) {
-            const int mm = k * p.mt * 16 + m;
-            const float2 ml = join_ml[mm];
-            const float w = pg_exp2(ml.x - use);
-            const float4 v = *reinterpret_cast<const float4*>(join + mm * PITCH + d);
-            l += ml.y * w;
-            acc.x += v.x * w, acc.y += v.y * w, acc.z += v.z * w, acc.w += v.w * w;
-          }
-          if (!to_out) {
-            *reinterpret_cast<float4*>(rec + (size_t)m * HD + d) = acc;
-            if (d == 0) {
-              rec[(size_t)p.block_rows * HD + m] = top;
-              rec[(size_t)p.block_rows * (HD + 1) + m] = l;
-            }
-            continue;
-          }
-          const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-          const int r = (m0 + m) / p.group, h = head * p.group + (m0 + m) % p.group;
-          T* out = static_cast<T*>(a.out) + seq * a.out_seq + r * a.out_row + h * a.out_head + d;
-          uint2 w2;
-          w2.x = PgType<T>::down(acc.x * inv, acc.y * inv);
-          w2.y = PgType<T>::down(acc.z * inv, acc.w * inv);
-          *reinterpret_cast<uint2*>(out) = w2;
-          if (a.lse && d == 0)
-            a.lse[((long long)seq * rows + r) * a.n_q + h] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
-        }
-      };
-      finish(alone);
-      if (!alone) {
-        __threadfence();
-        dc_bar();
-        if (tid == 0) last_flag = atomicAdd(&p.tickets[c0], 1u) == (unsigned)(c1 - c0);
-        dc_bar();
-        if (last_flag) {  // all records of the pair are there: each group joins every groups-th of them
-          __threadfence();
-          if (active) {
-            const int rows_here = min(16, M - mt * 16);
-            for (int it = lane; it < rows_here * (HD / 4); it += 32) {
-              const int m = mt * 16 + it / (HD / 4), d = it % (HD / 4) * 4;
-              float top = -INFINITY, l = 0.f;
-              float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-              for (int k = c0 + ks; k <= c1; k += groups) {
-                const float* x = p.rec + (size_t)(k == c0 ? 2 * k + 1 : 2 * k) * rec_floats;
-                const float mk2 = __ldcg(x + (size_t)p.block_rows * HD + m), lk = __ldcg(x + (size_t)p.block_rows * (HD + 1) + m);
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(x + (size_t)m * HD + d));
-                const float nt = fmaxf(top, mk2), use = nt == -INFINITY ? 0.f : nt;
-                const float fo = pg_exp2(top - use), fn = pg_exp2(mk2 - use);
-                l = l * fo + lk * fn;
-                acc.x = acc.x * fo + v.x * fn, acc.y = acc.y * fo + v.y * fn;
-                acc.z = acc.z * fo + v.z * fn, acc.w = acc.w * fo + v.w * fn;
-                top = nt;
-              }
-              const int mm = warp * 16 + it / (HD / 4);
-              *reinterpret_cast<float4*>(join + mm * PITCH + d) = acc;
-              if (d == 0) join_ml[mm] = make_float2(top, l);
-            }
-          }
-          dc_bar();
-          finish(true);
-          if (tid == 0) p.tickets[c0] = 0;
+  // ---- joiners ----
+  const int jt = tid - DC_WARPS * 32;
+  const size_t rec_floats = pg_record(p.M, HD);
+  auto queries = [&](int seq, int head, int r) {
+    unsigned char* qd = qbuf + (r & 1) * Sh::QBUF;
+    for (int x = jt; x < p.M * (HD / 8); x += DC_JOINERS) {
+      const int m = x / (HD / 8), ch = x % (HD / 8);
+      const T* q = static_cast<const T*>(a.q) + seq * a.q_seq + m / p.group * a.q_row + (head * p.group + m % p.group) * a.q_head;
+      pg_cp16(qd + (ch / 8) * QP + m * 128 + (((ch & 7) ^ (m & 7)) << 4), q + ch * 8);
+    }
+    pg_cp_arrive(&q_full[r & 1]);
+  };
+  auto put = [&](int seq, int head, int m, int d, float top, float l, const float4& acc) {
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+    const int row = m / p.group, h = head * p.group + m % p.group;
+    T* out = static_cast<T*>(a.out) + seq * a.out_seq + row * a.out_row + h * a.out_head + d;
+    uint2 v;
+    v.x = PgType<T>::down(acc.x * inv, acc.y * inv);
+    v.y = PgType<T>::down(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(out) = v;
+    if (a.lse && d == 0) a.lse[((long long)seq * rows + row) * a.n_q + h] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+  };
+  DcWalk<TS> w(p, lens_s, first_seq, first_tile, t0, t1);
+  w.find();
+  queries(w.seq, w.head, 0);
+  bool more = true;
+  for (int r = 0; more; ++r) {
+    const int seq = w.seq, head = w.head, u0 = w.u, n = w.run(), tiles = w.sp.tiles, pair_at = w.t - w.u;
+    const bool alone = n == tiles;
+    w.t += n;
+    more = w.find();
+    if (more) queries(w.seq, w.head, r + 1);  // the warps are done with the queries of run r - 1
+    float* rec = p.rec + (size_t)(u0 == 0 ? 2 * cta + 1 : 2 * cta) * rec_floats;
+    dc_sync(DC_FILLED);
+    // item: row m, 4 elements
+    for (int it = jt; it < p.M * (HD / 4); it += DC_JOINERS) {
+      const int m = it / (HD / 4), d = it % (HD / 4) * 4;
+      float2 ml[DC_WARPS];
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < DC_WARPS; ++k) {
+        ml[k] = join_ml[k * DC_ROWS + m];
+        top = fmaxf(top, ml[k].x);
+      }
+      const float use = top == -INFINITY ? 0.f : top;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float l = 0.f;
+#pragma unroll
+      for (int k = 0; k < DC_WARPS; ++k) {
+        const float f = pg_exp2(ml[k].x - use);
+        const float4 v = *reinterpret_cast<const float4*>(join + (k * DC_ROWS + m) * PITCH + d);
+        l += ml[k].y * f;
+        acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+      }
+      if (alone) {
+        put(seq, head, m, d, top, l, acc);
+      } else {
+        *reinterpret_cast<float4*>(rec + (size_t)m * HD + d) = acc;
+        if (d == 0) {
+          rec[(size_t)p.M * HD + m] = top;
+          rec[(size_t)p.M * (HD + 1) + m] = l;
         }
       }
-      dc_bar();  // the join buffer is free
-      t += n;
     }
-    seq_at = end;
-    ++seq;
+    if (more) dc_arrive(DC_FREE);  // the warps come for it before each further run
+    if (alone) continue;
+    const int c0 = share.owner(pair_at), c1 = share.owner(pair_at + tiles - 1);
+    __threadfence();
+    __syncwarp();
+    asm volatile("barrier.sync 1, 96;" ::: "memory");
+    if (jt == 0) last_flag = atomicAdd(&p.tickets[c0], 1u) == (unsigned)(c1 - c0);
+    __syncwarp();
+    asm volatile("barrier.sync 1, 96;" ::: "memory");
+    if (!last_flag) continue;
+    __threadfence();
+    for (int it = jt; it < p.M * (HD / 4); it += DC_JOINERS) {
+      const int m = it / (HD / 4), d = it % (HD / 4) * 4;
+      float top = -INFINITY, l = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k0 = c0; k0 <= c1; k0 += 8) {  // 8 records at a time: their reads fly together
+        float mk8[8], l8[8];
+        float4 v8[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int cc = min(k0 + k, c1);
+          const float* x = p.rec + (size_t)(cc == c0 ? 2 * cc + 1 : 2 * cc) * rec_floats;
+          mk8[k] = __ldcg(x + (size_t)p.M * HD + m);
+          l8[k] = __ldcg(x + (size_t)p.M * (HD + 1) + m);
+          v8[k] = __ldcg(reinterpret_cast<const float4*>(x + (size_t)m * HD + d));
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (k0 + k > c1) continue;
+          const float nt = fmaxf(top, mk8[k]), use = nt == -INFINITY ? 0.f : nt;
+          const float fo = pg_exp2(top - use), fn = pg_exp2(mk8[k] - use);
+          l = l * fo + l8[k] * fn;
+          acc.x = acc.x * fo + v8[k].x * fn, acc.y = acc.y * fo + v8[k].y * fn;
+          acc.z = acc.z * fo + v8[k].z * fn, acc.w = acc.w * fo + v8[k].w * fn;
+          top = nt;
+        }
+      }
+      put(seq, head, m, d, top, l, acc);
+    }
+    if (jt == 0) p.tickets[c0] = 0;
   }
 }
 

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <string>
+#include <utility>
 
 #include "vp_paged.cuh"
 
@@ -14,20 +15,14 @@ namespace {
 using namespace vp;
 
 constexpr int PG_MAX_CTAS = 160;       // CTAs of an attention launch, one per SM (148 on a B200)
-constexpr size_t WORK_HEAD = 1024;     // counters at the head of the work buffer
-static_assert(PG_MAX_CTAS * sizeof(unsigned) <= WORK_HEAD, "counters");
+constexpr int PG_RECORDS = 4 * PG_MAX_CTAS;  // of cut blocks: a piece has half an even share of all tiles on average
+constexpr size_t WORK_HEAD = VP_PAGED_WORK_ZEROED;  // counters at the head of the work buffer
+static_assert(2 * PG_RECORDS * sizeof(unsigned) <= WORK_HEAD, "counters");
 
 int pfail(int code, const char* msg) {
   vp_set_last_error(msg);
   return code;
 }
-int launched(const char* what) {
-  const cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) return VP_OK;
-  vp_set_last_error(std::string(what) + ": " + cudaGetErrorString(e));
-  return VP_ERR_CUDA;
-}
-
 bool off16(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
 
 int check_cache(const vp_paged* c) {
@@ -65,9 +60,34 @@ int check_attn(const vp_paged* c, const vp_paged_attn* a) {
       bad_strides(a->q_seq, a->out_seq, 8))
     return pfail(VP_ERR_ARG, "strides of q and out must be multiples of 8 elements");
   if (!a->work || (reinterpret_cast<uintptr_t>(a->work) & 255)) return pfail(VP_ERR_ARG, "work must be 256-byte aligned");
-  if (a->work_bytes < vp_paged_work_bytes(c->head_dim, a->n_q, c->n_kv, a->rows < PG_MAX_ROWS ? a->rows : PG_MAX_ROWS))
+  if (a->work_bytes < vp_paged_work_bytes(c->head_dim, a->n_q, c->n_kv, a->rows))
     return pfail(VP_ERR_ARG, "work is smaller than vp_paged_work_bytes");
   return VP_OK;
+}
+
+// Launches a kernel whose prologue may run while the kernel before it in the stream ends
+// (griddepcontrol.wait in the kernel stands before its first access to global memory).
+template <typename... P, typename... A>
+int pg_launch(const char* what, void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, A&&... args) {
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return pfail(VP_ERR_CUDA, cudaGetErrorString(e));
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+  if (e == cudaSuccess) return VP_OK;
+  cudaGetLastError();
+  vp_set_last_error(std::string(what) + ": " + cudaGetErrorString(e));
+  return VP_ERR_CUDA;
 }
 
 // SMs of the current device, at most PG_MAX_CTAS.
@@ -80,9 +100,9 @@ int sm_count(int* out) {
   return VP_OK;
 }
 
-// Maps of both pools as [page][head][slot][element] with boxes of 64 elements x `rows` slots of one
-// page and head, 128-byte swizzle, zeros outside.
-int pool_maps(const vp_paged& c, int rows, CUtensorMap* mk, CUtensorMap* mv) {
+// Maps of both pools as [page][head][panel of 64 elements][slot][element] with boxes of `panels` panels
+// x `rows` slots of one page and head, 128-byte swizzle, zeros outside.
+int pool_maps(const vp_paged& c, int rows, int panels, CUtensorMap* mk, CUtensorMap* mv) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -93,12 +113,12 @@ int pool_maps(const vp_paged& c, int rows, CUtensorMap* mk, CUtensorMap* mv) {
     return reinterpret_cast<Encode>(f);
   }();
   if (!encode) return pfail(VP_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
-  const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.page_size, (cuuint64_t)c.n_kv, (cuuint64_t)c.n_pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)c.slot_stride * 2, (cuuint64_t)c.head_stride * 2, (cuuint64_t)c.page_stride * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, step[4] = {1, 1, 1, 1};
+  const cuuint64_t dims[5] = {64, (cuuint64_t)c.page_size, (cuuint64_t)c.head_dim / 64, (cuuint64_t)c.n_kv, (cuuint64_t)c.n_pages};
+  const cuuint64_t strides[4] = {(cuuint64_t)c.slot_stride * 2, 128, (cuuint64_t)c.head_stride * 2, (cuuint64_t)c.page_stride * 2};
+  const cuuint32_t box[5] = {64, (cuuint32_t)rows, (cuuint32_t)panels, 1, 1}, step[5] = {1, 1, 1, 1, 1};
   const CUtensorMapDataType type = c.type == VP_T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   for (int i = 0; i < 2; ++i)
-    if (encode(i ? mv : mk, type, 4, i ? c.v : c.k, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    if (encode(i ? mv : mk, type, 5, i ? c.v : c.k, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return pfail(VP_ERR_ARG, "the pools' strides or extents cannot be mapped");
   return VP_OK;

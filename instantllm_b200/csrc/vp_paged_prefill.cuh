@@ -1,25 +1,32 @@
-// Attention of prompt rows over the paged cache (vp_paged_prefill).
+// Attention of many query rows per cache head over the paged cache: prompts (vp_paged_prefill), and
+// vp_paged_decode where the new rows of a request and the heads of a group make more than 16.
 //
 // Mathematics as in vp_paged_decode.cuh: a running maximum m and sum l over tiles of 128 slots. The
 // maximum that the weights are taken against only moves when the tile's is more than 2^8 above it
 // (weights then reach 2^8 at most, and out = o / l does not depend on it), so o is rarely rescaled.
 //
 // Bound: the tensor cores at head_dim 128, the exponentials (16 a clock and SM against 4,096 products)
-// at 64. The query rows of one cache head are packed as row G + g, 256 of them to a CTA as two
+// at 64. The query rows of one cache head are packed as row G + g, 256 of them to a block as two
 // tiles of 128, so K and V are read once for 256 rows and the heads of a group share them. Tensor
 // memory holds S of both tiles (128 columns each, the weights P written over them as pairs) and both
 // o (head_dim columns each). One warp brings K and V tiles (TMA boxes of one page each), one thread
 // issues the products, and two warpgroups, one tile each and one row a thread, do the softmax: while
 // one of them works on its tile, the tensor cores work on the other's.
+//
+// Work: one piece per (request, block, head), dealt out to one CTA per SM, the blocks with the most slots
+// first. Where that gives a CTA more than its share, a block's tiles are cut into pieces of about an
+// even share of all tiles (PF_LEAST at least); the pieces leave records in the work buffer and the
+// one that finishes last (a counter per row tile, back at zero afterwards) joins them in order. A
+// scheduler warp looks up the next piece, and its K and V arrive, while the present one is computed.
 #pragma once
-#include "vp_paged.cuh"
+#include "vp_paged_decode.cuh"
 
 namespace vp {
 
 constexpr int PF_TS = 128;                 // slots per tile
 constexpr int PF_ROWS = 256;               // packed query rows per CTA
-constexpr int PF_THREADS = 384;            // two softmax warpgroups, then one: producer, issuer, two idle warps
-constexpr int PF_PRODUCER = 8, PF_ISSUER = 9;
+constexpr int PF_THREADS = 384;            // two softmax warpgroups, then one: producer, issuer, scheduler, an idle warp
+constexpr int PF_PRODUCER = 8, PF_ISSUER = 9, PF_SCHEDULER = 10;
 constexpr uint32_t PF_TMEM = 512;          // columns
 constexpr float PF_SLACK = 8.f;            // log2 of the largest weight
 
@@ -27,14 +34,18 @@ template <int HD>
 struct PfShape {
   static constexpr int PANELS = HD / 64;                        // 128-byte wide columns of a tile
   static constexpr int TILE = PF_TS * HD * 2;                   // bytes of a K, V or Q tile
-  static constexpr int SLOTS = HD == 64 ? 8 : 5;                // ring of K and V tiles
+  static constexpr int SLOTS = HD == 64 ? 8 : 4;                // ring of K and V tiles
   static constexpr size_t SMEM = 1024 + 2 * TILE + (size_t)SLOTS * TILE;
 };
+
+constexpr int PF_LEAST = 4;                // tiles of a piece, at least
 
 struct PfParams {
   vp_paged c;
   vp_paged_attn a;
-  int group;
+  float* rec;         // records of block_rows rows, one per piece of a cut block
+  unsigned* tickets;  // [records][2 row tiles]
+  int group, block_rows, sms, most;  // most: pieces that a call can have
 };
 
 __device__ __forceinline__ uint64_t pf_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
@@ -93,43 +104,103 @@ __device__ __forceinline__ void pf_st32(uint32_t addr, const uint32_t* r) {
       : "memory");
 }
 
-// Slots that a run of rows at positions [p0, p1] sees, as tiles: [0, ns) hold sinks, then [ws, end).
+// Slots [0, min(sinks, end)) and [lo, end) as tiles: [0, ns) hold the sinks, then [ws, ..).
 struct PfSpan {
   int ns, ws, tiles;
   __device__ __forceinline__ int at(int t) const { return t < ns ? t : ws + t - ns; }
-  // tiles of this list whose first slot is at or below p
-  __device__ __forceinline__ int upto(int p) const {
-    if (p < 0) return 0;
-    const int end = p / PF_TS + 1;
+  // tiles of the list that start below `stop`
+  __device__ __forceinline__ int upto(int stop) const {
+    const int end = stop <= 0 ? 0 : (stop - 1) / PF_TS + 1;
     return min(tiles, end <= ns ? end : ns + max(0, end - ws));
   }
 };
-__device__ __forceinline__ PfSpan pf_span(int p0, int p1, int window, int sinks) {
+__device__ __forceinline__ PfSpan pf_span(int lo, int end, int sinks) {
   PfSpan s;
-  const int end = p1 < 0 ? 0 : p1 / PF_TS + 1, lo = window ? max(0, p0 - window + 1) : 0;
-  s.ns = window ? min((min(sinks, p1 + 1) + PF_TS - 1) / PF_TS, end) : 0;
-  s.ws = lo / PF_TS;
+  const int all = end <= 0 ? 0 : (end - 1) / PF_TS + 1;
+  s.ns = lo > 0 ? min((min(sinks, max(end, 0)) + PF_TS - 1) / PF_TS, all) : 0;
+  s.ws = min(max(lo, 0) / PF_TS, all);
   if (s.ws <= s.ns) s.ws = s.ns = 0;
-  s.tiles = s.ns + end - s.ws;
+  s.tiles = s.ns + all - s.ws;
   return s;
+}
+// The request's part of a call: its new rows, and the slots that packed rows [f, g) of it see.
+struct PfSeq {
+  int first, n_new, len, base, blocks, least;  // least: fewest mask bits of a row (trees)
+  int lo, end;                                 // of the last range asked for
+  __device__ __forceinline__ void see(const PfParams& p, int f, int g) {
+    const bool tree = !p.a.q_start;
+    const int p_lo = tree ? base + least - 1 : base + f / p.group;
+    end = tree ? len : base + (g - 1) / p.group + 1;
+    lo = p.a.window ? max(0, p_lo - p.a.window + 1) : 0;
+  }
+  __device__ __forceinline__ int last_tiles(const PfParams& p) {  // of the last block, which has the most
+    see(p, (blocks - 1) * PF_ROWS, n_new * p.group);
+    return pf_span(lo, end, p.a.sinks).tiles;
+  }
+};
+__device__ __forceinline__ PfSeq pf_seq(const PfParams& p, int i) {
+  PfSeq s;
+  s.first = 0;
+  s.n_new = p.a.rows;
+  s.least = 1;
+  if (p.a.q_start) {
+    const int x = p.a.q_start[i], y = p.a.q_start[i + 1];
+    s.first = min(max(x, 0), p.a.rows);
+    const int next = min(max(y, 0), p.a.rows);
+    if (s.first != x || next != y || next < s.first) pg_status(p.c.status, VP_DEV_ERR_SLOT);
+    s.n_new = max(0, next - s.first);
+  } else if (p.a.window && p.a.mask) {
+    for (int r = 0; r < p.a.rows; ++r)
+      s.least = min(s.least, __popc((uint32_t)p.a.mask[(long long)i * p.a.rows + r] & ((1u << p.a.rows) - 1)));
+  }
+  s.len = pg_seq(p.c, p.a.seqs, p.a.lens, i).len;
+  s.base = s.len - s.n_new;
+  s.blocks = (int)(((unsigned)s.n_new * (unsigned)p.group + PF_ROWS - 1) / PF_ROWS);
+  return s;
+}
+__device__ __forceinline__ uint32_t pf_low(int x) { return x <= 0 ? 0u : x >= 32 ? ~0u : (1u << x) - 1; }
+
+// A piece as the scheduler hands it to the other roles.
+struct PfPiece {
+  int seq, head, f0, f_end, first, base, cut, cuts, live, record0, j0, n0, n1, see_lo, see_end, ns, ws;  // seq < 0: no more
+  uint32_t any;                 // trees: new slots that a row sees
+  uint32_t masks[PG_MAX_ROWS];  // bits 0-15: new slots that the row sees, 16-20: the row's mask bits
+};
+
+__device__ __forceinline__ float2 pf_fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 pf_add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
 }
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(PF_THREADS, 1)
-    k_paged_prefill(const __grid_constant__ PfParams p, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
+    k_paged_tiles(const __grid_constant__ PfParams p, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
   using Sh = PfShape<HD>;
   constexpr int TILE = Sh::TILE, SLOTS = Sh::SLOTS, PANELS = Sh::PANELS, PANEL = PF_TS * 128;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* qs = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   unsigned char* ring = qs + 2 * TILE;
-  __shared__ uint64_t kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_full[2], q_full, edge, drained;
+  // s_full: S of a buffer is there; p_full: its weights are; o_full: a product into o is done
+  __shared__ uint64_t kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_full[2], o_full[2], q_full, edge, drained, info_full[2], info_empty[2];
   __shared__ uint32_t tmem_base;
-  __shared__ int warp_sums[PF_THREADS / 32], my_seq, my_tile, dead;
+  __shared__ long long tile_sums[PF_THREADS / 32];
+  __shared__ int sums[PF_THREADS / 32][2], starts[PF_THREADS], rec_starts[PF_THREADS], dead, last_s[2];
+  __shared__ PfPiece info[2];
 
   const vp_paged& c = p.c;
   const vp_paged_attn& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const bool tree = !a.q_start;
 
+  pdl_launch_dependents();
   if (tid == 0) {
     for (int i = 0; i < SLOTS; ++i) {
       mbar_init(&kv_full[i], 1);
@@ -138,51 +209,19 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&info_full[i], 1);
+      mbar_init(&info_empty[i], 10);  // the softmax warps, the producer, the issuer
     }
-    mbar_init(&q_full, 8);
+    mbar_init(&q_full, 9);  // the softmax warps and the issuer
     mbar_init(&edge, 1);
     mbar_init(&drained, 1);
     fence_barrier_init();
     dead = 0;
-    my_seq = -1;
   }
-  // which request and block of rows: blocks are counted over the requests, the last ones (with the
-  // most slots to see) first
-  const int run = (a.n + PF_THREADS - 1) / PF_THREADS, i0 = min(a.n, tid * run), i1 = min(a.n, i0 + run);
-  auto new_rows = [&](int i) {
-    const int x = min(max(a.q_start[i], 0), a.rows), y = min(max(a.q_start[i + 1], 0), a.rows);
-    return max(0, y - x);
-  };
-  auto blocks_of = [&](int i) { return (int)(((long long)new_rows(i) * p.group + PF_ROWS - 1) / PF_ROWS); };
-  int mine = 0;
-  for (int i = i0; i < i1; ++i) mine += blocks_of(i);
-  int incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) warp_sums[warp] = incl;
-  cta_sync();
-  int before = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < PF_THREADS / 32; ++w) {
-    if (w < warp) before += warp_sums[w];
-    total += warp_sums[w];
-  }
-  const int block = total - 1 - (int)(blockIdx.x / c.n_kv), head = blockIdx.x % c.n_kv;
-  if (block < 0) return;
-  int at = before + incl - mine;
-  if (at <= block && block < at + mine) {
-    for (int i = i0; i < i1; ++i) {
-      const int n = blocks_of(i);
-      if (block < at + n) {
-        my_seq = i;
-        my_tile = block - at;
-        break;
-      }
-      at += n;
-    }
+  if (warp == PF_PRODUCER && lane == 0) {
+    pg_prefetch_map(&mk);
+    pg_prefetch_map(&mv);
   }
   __syncwarp();
   if (warp == PF_ISSUER) {
@@ -190,19 +229,62 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  pdl_wait();
+  // Pieces of all requests, in two sums: all tiles (which give the share of a CTA); pieces and records.
+  const int chunk = (a.n + PF_THREADS - 1) / PF_THREADS, i0 = min(a.n, tid * chunk), i1 = min(a.n, i0 + chunk);
+  long long tiles = 0;
+  int one_blocks = 0, one_last = 0;  // of the thread's last request
+  for (int i = i0; i < i1; ++i) {
+    PfSeq s = pf_seq(p, i);
+    one_blocks = s.blocks;
+    if (!s.blocks) continue;
+    one_last = s.last_tiles(p);
+    s.see(p, 0, min(PF_ROWS, s.n_new * p.group));
+    tiles += (long long)s.blocks * (one_last + pf_span(s.lo, s.end, a.sinks).tiles);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+  if (lane == 0) tile_sums[warp] = tiles;
   pf_fence_before();
   cta_sync();
   pf_fence_after();
+  long long all = 0;
+#pragma unroll
+  for (int w = 0; w < PF_THREADS / 32; ++w) all += tile_sums[w];
+  // the mean of its first and last block stands for a request's blocks: `all` is twice the tiles per
+  // cache head. Rounded up by two so that the float division cannot make it less than an even half.
+  const int share = max(PF_LEAST, (int)fminf((float)all * c.n_kv / (2 * p.sms), 1e9f) + 2);
+  int pieces = 0, records = 0;
+  for (int i = i0; i < i1; ++i) {
+    int blocks = one_blocks, last = one_last;
+    if (chunk > 1) {
+      PfSeq s = pf_seq(p, i);
+      blocks = s.blocks;
+      if (blocks) last = s.last_tiles(p);
+    }
+    if (!blocks) continue;
+    const int n = max(1, (last + share - 1) / share);
+    pieces += blocks * n * c.n_kv;
+    if (n > 1) records += blocks * n * c.n_kv;
+  }
+  int incl = pieces, incl_r = records;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, o), x = __shfl_up_sync(0xffffffffu, incl_r, o);
+    if (lane >= o) incl += v, incl_r += x;
+  }
+  if (lane == 31) sums[warp][0] = incl, sums[warp][1] = incl_r;
+  cta_sync();
+  int at0 = incl - pieces, at_r0 = incl_r - records, total = 0;
+#pragma unroll
+  for (int w = 0; w < PF_THREADS / 32; ++w) {
+    if (w < warp) at0 += sums[w][0], at_r0 += sums[w][1];
+    total += sums[w][0];
+  }
+  starts[tid] = at0;
+  rec_starts[tid] = at_r0;
+  cta_sync();
   const uint32_t tmem = tmem_base;
-  const int seq = my_seq, f0 = my_tile * PF_ROWS, n_new = new_rows(seq), first = min(max(a.q_start[seq], 0), a.rows);
-  const PgSeq sq = pg_seq(c, a.seqs, a.lens, seq);
-  const int base = sq.len - n_new;
-  const int f_end = (int)min((long long)n_new * p.group, (long long)f0 + PF_ROWS);
-  const int p_lo = base + f0 / p.group, p_hi = base + (f_end - 1) / p.group;
-  const PfSpan sp = pf_span(p_lo, p_hi, a.window, a.sinks);
-  // tiles of the two row tiles: the first ends earlier
-  const int p_hi0 = base + (min(f_end, f0 + 128) - 1) / p.group;
-  const int n0 = sp.upto(p_hi0), n1 = f_end > f0 + 128 ? sp.tiles : 0, n_max = max(n0, n1);
 
   auto wait_warp = [&](uint64_t* bar, uint32_t parity) {  // whole warp
     __syncwarp();
@@ -220,226 +302,469 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       *(volatile int*)&dead = 1;
     }
   };
+  auto is_dead = [&] { return *(volatile int*)&dead != 0; };
 
   if (warp < 8) {
     // ---- softmax: warpgroup i has row tile i, a thread row f ----
-    const int i = warp >> 2, row = tid & 127, f = f0 + tid;
-    const int n_t = i ? n1 : n0;
-    const bool valid = f < f_end;
-    const int qrow = f / p.group, h = head * p.group + f % p.group;
-    {
-      const T* q = static_cast<const T*>(a.q) + (long long)(first + qrow) * a.q_row + h * a.q_head;
-      unsigned char* dst = qs + i * TILE + row * 128;
-#pragma unroll
-      for (int d = 0; d < HD / 8; ++d) {
-        const uint4 v = valid ? *reinterpret_cast<const uint4*>(q + d * 8) : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(dst + (d / 8) * PANEL + (((d & 7) ^ (row & 7)) << 4)) = v;
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) pg_arrive(&q_full);
-    }
+    const int i = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 lanes of tensor memory
-    const uint32_t ts = tmem + lanes + i * 128, to = tmem + lanes + 256 + i * HD;
-    const int pos = base + qrow;
-    const int hi = valid ? pos + 1 : 1 << 30, lo = valid && a.window ? pos - a.window + 1 : 0;
-    // the tile of rows: every row sees below hi_all, and from lo_all on
-    const int hi_all = base + (f0 + i * 128) / p.group + 1, lo_all = a.window ? base + (f0 + i * 128 + 127) / p.group - a.window + 1 : 0;
+    const uint32_t to = tmem + lanes + 256 + i * HD;
     const float cexp = a.scale * 1.4426950408889634f;
-    float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < n_t; ++j) {
-      const int s0 = sp.at(j) * PF_TS;
-      wait_warp(&s_full[i], j & 1);
-      pf_fence_after();
-      uint32_t s[128];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) pf_ld32(s + 32 * k, ts + 32 * k);
-      pf_loaded(s);
-      if (s0 + PF_TS > hi_all || (s0 < lo_all && s0 + PF_TS > a.sinks)) {
-        const int h_r = hi - s0, l_r = lo - s0, k_r = a.sinks - s0;
-#pragma unroll
-        for (int k = 0; k < 128; ++k)
-          if (k >= h_r || (k < l_r && k >= k_r)) s[k] = 0xff800000u;
+    const size_t rec_floats = pg_record(p.block_rows, HD);
+    const int m_at = p.block_rows * HD, l_at = m_at + p.block_rows;
+    uint32_t n_s[2] = {0, 0}, n_o = 0;  // phases of s_full and p_full, of o_full so far
+    for (int r = 0;; ++r) {
+      wait_warp(&info_full[r & 1], (r >> 1) & 1);
+      const PfPiece& in = info[r & 1];
+      const int seq = in.seq, f = in.f0 + tid, f_end = in.f_end, f0 = in.f0, head = in.head, first = in.first, base = in.base;
+      if (seq < 0 || is_dead()) break;
+      const bool two = in.n1 > 0 || f_end > f0 + 128;  // two row tiles; else the first has both buffers of S
+      const int n_t = i ? in.n1 : in.n0, j0 = in.j0, cuts = in.cuts, cut = in.cut, live = in.live, record0 = in.record0;
+      const int n0 = in.n0, n1 = in.n1;
+      PfSpan sp;
+      sp.ns = in.ns;
+      sp.ws = in.ws;
+      const bool valid = f < f_end;
+      const int qrow = f / p.group, h = head * p.group + f % p.group;
+      // the row sees old slots [lo, hi), the sinks below hi, and new slot j of a tree where bit j is set
+      uint32_t bits = 0;
+      int hi = 0, lo = 0;
+      if (valid && base + qrow >= 0) {
+        const uint32_t mask = tree ? in.masks[qrow] : 0;
+        bits = mask & 0xffffu;
+        hi = tree ? base : base + qrow + 1;
+        if (a.window) lo = (tree ? base + (int)(mask >> 16) : base + qrow + 1) - a.window;
       }
-      float top = -INFINITY;
+      __syncwarp();
+      if (lane == 0) pg_arrive(&info_empty[r & 1]);
+      {  // queries: the products of the last piece that read the buffer are done
+        const T* q = static_cast<const T*>(a.q) + seq * a.q_seq + (long long)(first + qrow) * a.q_row + h * a.q_head;
+        unsigned char* dst = qs + i * TILE + row * 128;
+        if (valid) {
 #pragma unroll
-      for (int k = 0; k < 128; ++k) top = fmaxf(top, __uint_as_float(s[k]));
-      top *= cexp;
-      const bool move = top > m + PF_SLACK || (m == -INFINITY && top > m);
-      if (__any_sync(0xffffffffu, move)) {
-        const float mn = fmaxf(m, top), fac = m == -INFINITY ? 0.f : pg_exp2(m - mn);
-        l *= fac;
-        m = mn;
-        if (j > 0) {
+          for (int d = 0; d < HD / 8; ++d) pg_cp16(dst + (d / 8) * PANEL + (((d & 7) ^ (row & 7)) << 4), q + d * 8);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) pg_arrive(&q_full);
+        // Everybody starts the piece together: a warp ahead of the others would wait for phases of barriers
+        // whose earlier phases, the other warpgroup's, are still to come, and take one for another.
+        wait_warp(&q_full, r & 1);
+      }
+      // every row of the tile sees [lo_all, hi_all)
+      const int hi_all = tree ? base : base + (f0 + i * 128) / p.group + 1;
+      const int lo_all = !a.window ? 0 : tree ? base + a.rows - a.window : base + (f0 + i * 128 + 127) / p.group - a.window + 1;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < n_t; ++j) {
+        const int s0 = sp.at(j0 + j) * PF_TS, buf = two ? i : j & 1;
+        const uint32_t ts = tmem + lanes + buf * 128;
+        wait_warp(&s_full[buf], n_s[buf] & 1);
+        ++n_s[buf];
+        pf_fence_after();
+        uint32_t s[128];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) pf_ld32(s + 32 * k, ts + 32 * k);
+        pf_loaded(s);
+        if (s0 + PF_TS > hi_all || (s0 < lo_all && s0 + PF_TS > a.sinks)) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int b = s0 + 32 * k, fresh = base - b;
+            uint32_t see = (pf_low(hi - b) & ~pf_low(lo - b)) | pf_low(min(a.sinks, hi) - b);
+            if (bits) see |= fresh >= 32 || fresh <= -32 ? 0u : fresh >= 0 ? bits << fresh : bits >> -fresh;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((see >> e) & 1)) s[32 * k + e] = 0xff800000u;
+          }
+        }
+        float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains: a single one is 128 steps long
+#pragma unroll
+        for (int k = 0; k < 128; k += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            t4[e] = fmaxf(fmaxf(t4[e], __uint_as_float(s[k + 2 * e])), __uint_as_float(s[k + 2 * e + 1]));
+        const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * cexp;
+        const bool move = top > m + PF_SLACK || (m == -INFINITY && top > m);
+        if (__any_sync(0xffffffffu, move)) {
+          const float mn = fmaxf(m, top), fac = m == -INFINITY ? 0.f : pg_exp2(m - mn);
+          l *= fac;
+          m = mn;
+          if (j > 0) {
+            if (!two) {  // with two buffers of S the last product into o may be under way
+              wait_warp(&o_full[i], (n_o + j - 1) & 1);
+              pf_fence_after();
+            }
 #pragma unroll 1
-          for (int k = 0; k < HD; k += 32) {
-            uint32_t o[32];
+            for (int k = 0; k < HD; k += 32) {
+              uint32_t o[32];
+              pf_ld32(o, to + k);
+              pf_loaded(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fac);
+              pf_st32(to + k, o);
+            }
+            pf_wait_st();
+          }
+        }
+        const float use = m == -INFINITY ? 0.f : m;
+        const float2 c2 = make_float2(cexp, cexp), u2 = make_float2(-use, -use);
+        float2 sum[4] = {};
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          uint32_t w[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            float2 x = make_float2(__uint_as_float(s[64 * b + 2 * k]), __uint_as_float(s[64 * b + 2 * k + 1]));
+            x = pf_fma2(x, c2, u2);
+            x.x = pg_exp2(x.x);
+            x.y = pg_exp2(x.y);
+            sum[k & 3] = pf_add2(sum[k & 3], x);
+            w[k] = PgType<T>::down(x.x, x.y);
+          }
+          pf_st32(ts + 32 * b, w);
+        }
+        sum[0] = pf_add2(pf_add2(sum[0], sum[1]), pf_add2(sum[2], sum[3]));
+        l += sum[0].x + sum[0].y;
+        pf_wait_st();
+        pf_fence_before();
+        __syncwarp();
+        if (lane == 0) pg_arrive(&p_full[buf]);
+      }
+      // the last products into o, one phase after the other
+      if (n_t > 1 && !two) wait_warp(&o_full[i], (n_o + n_t - 2) & 1);
+      if (n_t > 0) {
+        wait_warp(&o_full[i], (n_o + n_t - 1) & 1);
+        pf_fence_after();
+      }
+      n_o += n_t;
+      if (two) {  // the other warpgroup's buffer
+        n_s[1 - i] += i ? n0 : n1;
+      } else if (i == 1) {  // both
+        n_s[0] += (n0 + 1) / 2;
+        n_s[1] += n0 / 2;
+      }
+      T* out = static_cast<T*>(a.out) + seq * a.out_seq + (long long)(first + qrow) * a.out_row + h * a.out_head;
+      float* lse = a.lse ? a.lse + ((tree ? (long long)seq * a.rows : (long long)first) + qrow) * a.n_q + h : nullptr;
+      float* rec = p.rec + (size_t)(record0 + cut) * rec_floats;
+      const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+      if (f_end > f0 + i * 128) {
+#pragma unroll 1
+        for (int k = 0; k < HD; k += 32) {
+          uint32_t o[32];
+          if (n_t > 0) {
             pf_ld32(o, to + k);
             pf_loaded(o);
+          } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fac);
-            pf_st32(to + k, o);
+            for (int e = 0; e < 32; ++e) o[e] = 0;
           }
-          pf_wait_st();
+          if (valid && cuts > 1) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4*>(rec + (size_t)tid * HD + k + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          } else if (valid) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint4 v;
+              uint32_t* w = &v.x;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float y0 = __uint_as_float(o[e + 2 * x]), y1 = __uint_as_float(o[e + 2 * x + 1]);
+                w[x] = PgType<T>::down(inv == 0.f ? 0.f : y0 * inv, inv == 0.f ? 0.f : y1 * inv);
+              }
+              *reinterpret_cast<uint4*>(out + k + e) = v;
+            }
+          }
+          __syncwarp();
+        }
+        if (valid && cuts > 1) rec[m_at + tid] = m, rec[l_at + tid] = l;
+        if (valid && cuts == 1 && lse) *lse = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        pf_fence_before();
+        if (cuts > 1) {
+          __threadfence();
+          __syncwarp();
+          asm volatile("barrier.sync %0, 128;" ::"r"(1 + i) : "memory");
+          unsigned* ticket = p.tickets + record0 * 2 + i;
+          if (row == 0) last_s[i] = atomicAdd(ticket, 1u) == (unsigned)(cuts - 1);
+          __syncwarp();
+          asm volatile("barrier.sync %0, 128;" ::"r"(1 + i) : "memory");
+          if (last_s[i]) {
+            // All pieces of the row tile are there. A warp takes rows in turn: its lanes first the weights
+            // of 32 pieces, then 4 elements each (two rows at head_dim 64).
+            __threadfence();
+            const float* rec0 = p.rec + (size_t)record0 * rec_floats;
+            const int n_rows = min(128, f_end - f0 - i * 128);
+            constexpr int LR = HD / 4, RW = 32 / LR;  // lanes per row, rows at a time
+            const int d = lane % LR * 4;
+            for (int x0 = (warp & 3) * RW; x0 < n_rows; x0 += 4 * RW) {
+              const int mm = i * 128 + min(x0 + lane / LR, n_rows - 1);
+              float top = -INFINITY;
+              for (int k = 0; k < live; ++k) top = fmaxf(top, __ldcg(rec0 + k * rec_floats + m_at + mm));
+              const float us = top == -INFINITY ? 0.f : top;
+              float sm = 0.f;
+              float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+              for (int k0 = 0; k0 < live; k0 += 8) {  // 8 records' reads fly together
+                float4 v8[8];
+                float m8[8], l8[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                  const float* x = rec0 + (size_t)min(k0 + k, live - 1) * rec_floats;
+                  v8[k] = __ldcg(reinterpret_cast<const float4*>(x + (size_t)mm * HD + d));
+                  m8[k] = __ldcg(x + m_at + mm);
+                  l8[k] = __ldcg(x + l_at + mm);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                  const float w = k0 + k < live ? pg_exp2(m8[k] - us) : 0.f;
+                  sm += l8[k] * w;
+                  acc.x += v8[k].x * w, acc.y += v8[k].y * w, acc.z += v8[k].z * w, acc.w += v8[k].w * w;
+                }
+              }
+              const float iv = sm > 0.f ? 1.f / sm : sm == 0.f ? 0.f : sm;
+              const int r2 = (f0 + mm) / p.group, h2 = head * p.group + (f0 + mm) % p.group;
+              uint2 v2;
+              v2.x = PgType<T>::down(acc.x * iv, acc.y * iv);
+              v2.y = PgType<T>::down(acc.z * iv, acc.w * iv);
+              *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + seq * a.out_seq + (long long)(first + r2) * a.out_row + h2 * a.out_head + d) = v2;
+              if (a.lse && d == 0)
+                a.lse[((tree ? (long long)seq * a.rows : (long long)first) + r2) * a.n_q + h2] =
+                    sm == 0.f ? -INFINITY : (top + log2f(sm)) * 0.6931471805599453f;
+            }
+            if (row == 0) *ticket = 0;
+          }
+          __syncwarp();
         }
       }
-      const float use = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        uint32_t w[32];
-#pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          const float x = pg_exp2(fmaf(__uint_as_float(s[64 * b + 2 * k]), cexp, -use));
-          const float y = pg_exp2(fmaf(__uint_as_float(s[64 * b + 2 * k + 1]), cexp, -use));
-          sum[k & 1] += x;
-          sum[2 + (k & 1)] += y;
-          w[k] = PgType<T>::down(x, y);
-        }
-        pf_st32(ts + 32 * b, w);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      pf_wait_st();
       pf_fence_before();
-      __syncwarp();
-      if (lane == 0) pg_arrive(&p_full[i]);
     }
-    if (n_t > 0) {
-      wait_warp(&s_full[i], n_t & 1);  // the last product into o
-      pf_fence_after();
-    }
-    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-    T* out = static_cast<T*>(a.out) + (long long)(first + qrow) * a.out_row + h * a.out_head;
-#pragma unroll 1
-    for (int k = 0; k < HD; k += 32) {
-      uint32_t o[32];
-      if (n_t > 0) {
-        pf_ld32(o, to + k);
-        pf_loaded(o);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = 0;
+  } else if (warp == PF_SCHEDULER) {
+    // ---- the CTA's pieces: in turns over the CTAs, there and back, from the last request's last block on ----
+    const int G = gridDim.x;
+    for (int r = 0;; ++r) {
+      if (r >= 2) wait_warp(&info_empty[r & 1], ((r >> 1) - 1) & 1);
+      const int idx = r * G + (r & 1 ? G - 1 - (int)blockIdx.x : (int)blockIdx.x);
+      int piece = total - 1 - idx;
+      if (total > p.most) {  // requests whose rows overlap
+        if (lane == 0) pg_status(c.status, VP_DEV_ERR_SLOT);
+        piece = -1;
       }
-      if (valid) {
+      PfPiece& in = info[r & 1];
+      if (piece < 0 || is_dead()) {
+        if (lane == 0) {
+          in.seq = -1;
+          pg_arrive(&info_full[r & 1]);
+        }
+        break;
+      }
+      // the thread whose run of requests has the piece: 32 threads at a time
+      int owner = 0;
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          uint4 v;
-          uint32_t* w = &v.x;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float y0 = __uint_as_float(o[e + 2 * x]), y1 = __uint_as_float(o[e + 2 * x + 1]);
-            w[x] = PgType<T>::down(inv == 0.f ? 0.f : y0 * inv, inv == 0.f ? 0.f : y1 * inv);
-          }
-          *reinterpret_cast<uint4*>(out + k + e) = v;
+      for (int b = 0; b < PF_THREADS; b += 32) {
+        const uint32_t under = __ballot_sync(0xffffffffu, starts[b + lane] <= piece);
+        owner += __popc(under);
+      }
+      owner -= 1;
+      int at = starts[owner], at_r = rec_starts[owner], seq = owner * chunk;
+      PfSeq s = pf_seq(p, seq);
+      int cuts = 1;
+      for (;; s = pf_seq(p, ++seq)) {
+        if (s.blocks) {
+          cuts = max(1, (s.last_tiles(p) + share - 1) / share);
+          const int k = s.blocks * cuts * c.n_kv;
+          if (piece < at + k) break;
+          at += k;
+          if (cuts > 1) at_r += k;
         }
       }
+      // pieces of a request: block, then head, then cut
+      const int mine = piece - at, pair = mine / cuts, cut = mine - pair * cuts, block = pair / c.n_kv;
+      const int f0 = block * PF_ROWS, f_end = min(s.n_new * p.group, f0 + PF_ROWS);
+      s.see(p, f0, f_end);
+      const PfSpan sp = pf_span(s.lo, s.end, a.sinks);
+      const int live = max(1, min(cuts, sp.tiles)), per = sp.tiles / live, odd = sp.tiles % live;
+      const int j0 = cut * per + min(cut, odd), j1 = cut < live ? j0 + per + (cut < odd) : j0;
+      const int stop0 = tree ? s.end : s.base + (min(f_end, f0 + 128) - 1) / p.group + 1;
+      if (tree) {
+        const uint32_t all_rows = (1u << a.rows) - 1;
+        uint32_t anc = 0, keep = 0;
+        if (lane < a.rows) anc = a.mask ? (uint32_t)a.mask[(long long)seq * a.rows + lane] & all_rows : (2u << lane) - 1;
+        const int pos = s.base + __popc(anc) - 1;
+        for (int j = 0; j < a.rows; ++j) {  // less the new slots that have left the row's window
+          const int place = s.base + __popc(__shfl_sync(0xffffffffu, anc, j)) - 1;
+          if (!a.window || pos - place < a.window || place < a.sinks) keep |= 1u << j;
+        }
+        const uint32_t any = __reduce_or_sync(0xffffffffu, anc);
+        if (lane < PG_MAX_ROWS) in.masks[lane] = (anc & keep) | (uint32_t)__popc(anc) << 16;
+        if (lane == 0) in.any = any;
+      }
+      if (lane == 0) {
+        in.seq = seq, in.head = pair - block * c.n_kv, in.f0 = f0, in.f_end = f_end, in.first = s.first, in.base = s.base;
+        in.cut = cut, in.cuts = cuts, in.live = live, in.record0 = at_r + mine - cut;
+        in.j0 = j0, in.n0 = max(0, min(j1, sp.upto(stop0)) - j0), in.n1 = f_end > f0 + 128 ? j1 - j0 : 0;
+        in.see_lo = s.lo, in.see_end = s.end, in.ns = sp.ns, in.ws = sp.ws;
+      }
+      __threadfence_block();
       __syncwarp();
+      if (lane == 0) pg_arrive(&info_full[r & 1]);
     }
-    if (a.lse && valid)
-      a.lse[(long long)(first + qrow) * a.n_q + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-    pf_fence_before();
   } else if (warp == PF_PRODUCER) {
     // ---- K and V tiles, in the order of their use: K0 V0 K1 V1 ... ----
     const int box = min(c.page_size, PF_TS), boxes = PF_TS / box;
-    int issued = 0;
-    uint32_t edges = 0;
-    for (int j = 0; j < n_max; ++j) {
-      const int s0 = sp.at(j) * PF_TS, slot = s0 + lane * box;
-      int page = c.n_pages;  // a box that nobody sees fills zeros
-      const int w_lo = a.window ? p_lo - a.window + 1 : 0;
-      if (lane < boxes && slot <= p_hi && (slot + box > w_lo || slot < a.sinks)) {
-        page = sq.pages[slot / c.page_size];
-        if (page < 0 || page >= c.n_pages) {
-          pg_status(c.status, VP_DEV_ERR_PAGE);
-          page = c.n_pages;
-        }
-      }
-      // slots of the tile that no row of the CTA sees: their values may be NaN, which a zero weight
-      // does not silence, so they are zeroed before the product may read them
-      const bool ragged = s0 + PF_TS > p_hi + 1 || (s0 < w_lo && s0 + PF_TS > a.sinks);
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv, ++issued) {
-        const int st = issued % SLOTS;
-        if (issued >= SLOTS) wait_warp(&kv_empty[st], (issued / SLOTS - 1) & 1);
-        if (*(volatile int*)&dead) break;
-        const bool patch = kv && ragged;
-        uint64_t* bar = patch ? &edge : &kv_full[st];
-        unsigned char* tile = ring + (size_t)st * TILE;
-        if (lane == 0) mbar_arrive_expect_tx(bar, TILE);
-        __syncwarp();
-        if (lane < boxes) {
-#pragma unroll
-          for (int d = 0; d < PANELS; ++d)
-            pg_box(tile + d * PANEL + lane * box * 128, kv ? &mv : &mk, d * 64, slot % c.page_size, head, page, bar);
-        }
-        if (patch) {
-          wait_warp(&edge, edges & 1);
-          ++edges;
-          for (int x = lane; x < PF_TS; x += 32) {
-            const int sl = s0 + x;
-            if (sl > p_hi || (sl < w_lo && sl >= a.sinks)) {
-#pragma unroll
-              for (int d = 0; d < PANELS; ++d)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) *reinterpret_cast<uint4*>(tile + d * PANEL + x * 128 + e * 16) = make_uint4(0, 0, 0, 0);
-            }
+    uint32_t issued = 0, edges = 0;
+    for (int r = 0;; ++r) {
+      wait_warp(&info_full[r & 1], (r >> 1) & 1);
+      const PfPiece& in = info[r & 1];
+      const int seq = in.seq, head = in.head, j0 = in.j0, n_max = max(in.n0, in.n1), see_lo = in.see_lo, see_end = in.see_end, base = in.base;
+      const uint32_t any = in.any;
+      PfSpan sp;
+      sp.ns = in.ns;
+      sp.ws = in.ws;
+      if (seq < 0 || is_dead()) break;
+      __syncwarp();
+      if (lane == 0) pg_arrive(&info_empty[r & 1]);
+      const int32_t* pages = pg_seq(c, a.seqs, a.lens, seq).pages;
+      for (int j = 0; j < n_max; ++j) {
+        const int s0 = sp.at(j0 + j) * PF_TS, slot = s0 + lane * box;
+        int page = c.n_pages;  // a box that nobody sees fills zeros
+        if (lane < boxes && slot < see_end && (slot + box > see_lo || slot < a.sinks)) {
+          page = pages[slot / c.page_size];
+          if (page < 0 || page >= c.n_pages) {
+            pg_status(c.status, VP_DEV_ERR_PAGE);
+            page = c.n_pages;
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) pg_arrive(&kv_full[st]);
         }
+        // slots of the tile that no row of the block sees: their values may be NaN, which a zero weight
+        // does not silence, so they are zeroed before the product may read them
+        const bool ragged = s0 + PF_TS > (tree ? base : see_end) || (s0 < see_lo && s0 + PF_TS > a.sinks);
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv, ++issued) {
+          const uint32_t st = issued % SLOTS;
+          if (issued >= SLOTS) wait_warp(&kv_empty[st], (issued / SLOTS - 1) & 1);
+          if (is_dead()) break;
+          const bool patch = kv && ragged;
+          uint64_t* bar = patch ? &edge : &kv_full[st];
+          unsigned char* tile = ring + (size_t)st * TILE;
+          if (lane == 0) mbar_arrive_expect_tx(bar, TILE);
+          __syncwarp();
+          if (lane < boxes) {
+#pragma unroll
+            for (int d = 0; d < PANELS; ++d)
+              pg_box(tile + d * PANEL + lane * box * 128, kv ? &mv : &mk, d, slot & (c.page_size - 1), head, page, bar);
+          }
+          if (patch) {
+            wait_warp(&edge, edges & 1);
+            ++edges;
+            for (int x = lane; x < PF_TS; x += 32) {
+              const int sl = s0 + x;
+              if (sl >= see_end || (sl < see_lo && sl >= a.sinks) || (tree && sl >= base && !((any >> (sl - base)) & 1))) {
+#pragma unroll
+                for (int d = 0; d < PANELS; ++d)
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) *reinterpret_cast<uint4*>(tile + d * PANEL + x * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+              }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) pg_arrive(&kv_full[st]);
+          }
+        }
+        if (is_dead()) break;
       }
-      if (*(volatile int*)&dead) break;
     }
     // copies still in flight land before the CTA may end (they have, unless a wait ran out)
-    for (int k = max(0, issued - SLOTS); k < issued; ++k) mbar_wait_warp(&kv_full[k % SLOTS], (k / SLOTS) & 1);
-  } else if (warp == PF_ISSUER && lane == 0 && n_max > 0) {
+    for (uint32_t k = issued > SLOTS ? issued - SLOTS : 0; k < issued; ++k) mbar_wait_warp(&kv_full[k % SLOTS], (k / SLOTS) & 1);
+  } else if (warp == PF_ISSUER && lane == 0) {
     // ---- products ----
     constexpr uint32_t FMT = PgType<T>::BF16 ? 1u : 0u;
     constexpr uint32_t ID_S = 1u << 4 | FMT << 7 | FMT << 10 | (PF_TS / 8) << 17 | (128 / 16) << 24;
     constexpr uint32_t ID_O = 1u << 4 | FMT << 7 | FMT << 10 | 1u << 16 | (HD / 8) << 17 | (128 / 16) << 24;
     const uint32_t qb = smem_u32(qs), rb = smem_u32(ring);
-    auto scores = [&](int i, int j) {  // S_i = Q_i K_j^T
-      const uint32_t kb = rb + (2 * j % SLOTS) * TILE, qa = qb + i * TILE;
+    auto scores = [&](int i, int buf, uint32_t st) {  // S buffer = Q_i K^T
+      const uint32_t kb = rb + st * TILE, qa = qb + i * TILE;
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k) {
         const uint32_t off = (k / 4) * PANEL + (k & 3) * 32;
-        pf_mma_ss(tmem + i * 128, pf_desc(qa + off, 16, 1024), pf_desc(kb + off, 16, 1024), ID_S, k > 0);
+        pf_mma_ss(tmem + buf * 128, pf_desc(qa + off, 16, 1024), pf_desc(kb + off, 16, 1024), ID_S, k > 0);
       }
-      pf_commit(&s_full[i]);
+      pf_commit(&s_full[buf]);
     };
-    wait_one(&q_full, 0);
-    wait_one(&kv_full[0], 0);
-    pf_fence_after();
-    if (n0 > 0) scores(0, 0);
-    if (n1 > 0) scores(1, 0);
-    pf_commit(&kv_empty[0]);
-    for (int j = 0; j < n_max; ++j) {
-      const int v = 2 * j + 1, vs = v % SLOTS, kn = 2 * j + 2;
-      wait_one(&kv_full[vs], (v / SLOTS) & 1);
-      bool k_there = false;
+    auto values = [&](int i, int buf, uint32_t st, bool add) {  // o_i += P buffer V
+      const uint32_t vb = rb + st * TILE;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int n_t = i ? n1 : n0;
-        if (j >= n_t) continue;
-        wait_one(&p_full[i], j & 1);
-        if (*(volatile int*)&dead) break;
-        pf_fence_after();
-        const uint32_t vb = rb + vs * TILE;
+      for (int k = 0; k < PF_TS / 16; ++k)
+        pf_mma_ts(tmem + 256 + i * HD, tmem + buf * 128 + k * 8, pf_desc(vb + k * 2048, PANEL, 1024), ID_O, add || k > 0);
+      pf_commit(&o_full[i]);
+    };
+    uint32_t used = 0, n_p[2] = {0, 0};  // K and V tiles so far, phases of p_full so far
+    auto ready = [&](uint32_t k) {        // tile k of the ring is there
+      wait_one(&kv_full[k % SLOTS], (k / SLOTS) & 1);
+      pf_fence_after();
+    };
+    for (int r = 0;; ++r) {
+      wait_one(&info_full[r & 1], (r >> 1) & 1);
+      const PfPiece& in = info[r & 1];
+      const int seq = in.seq, n0 = in.n0, n1 = in.n1, n_max = max(n0, n1);
+      const bool two = n1 > 0 || in.f_end > in.f0 + 128;
+      if (seq < 0 || is_dead()) break;
+      pg_arrive(&info_empty[r & 1]);
+      pg_arrive(&q_full);
+      wait_one(&q_full, r & 1);
+      pf_fence_after();
+      if (n_max > 0) ready(used);
+      if (two) {
+        if (n0 > 0) scores(0, 0, used % SLOTS);
+        if (n1 > 0) scores(1, 1, used % SLOTS);
+        if (n_max > 0) pf_commit(&kv_empty[used % SLOTS]);
+        for (int j = 0; j < n_max && !is_dead(); ++j) {
+          const uint32_t v = used + 2 * j + 1, kn = v + 1;
+          ready(v);
+          bool k_there = false;
 #pragma unroll
-        for (int k = 0; k < PF_TS / 16; ++k)
-          pf_mma_ts(tmem + 256 + i * HD, tmem + i * 128 + k * 8, pf_desc(vb + k * 2048, PANEL, 1024), ID_O, j > 0 || k > 0);
-        if (j + 1 < n_t) {
-          if (!k_there) wait_one(&kv_full[kn % SLOTS], (kn / SLOTS) & 1), k_there = true;
+          for (int i = 0; i < 2; ++i) {
+            const int n_t = i ? n1 : n0;
+            if (j >= n_t) continue;
+            wait_one(&p_full[i], n_p[i] & 1);
+            ++n_p[i];
+            if (is_dead()) break;
+            pf_fence_after();
+            values(i, i, v % SLOTS, j > 0);
+            if (i == 1 || j >= n1) pf_commit(&kv_empty[v % SLOTS]);
+            if (j + 1 < n_t) {
+              if (!k_there) ready(kn), k_there = true;
+              scores(i, i, kn % SLOTS);
+            }
+          }
+          if (j + 1 < n_max) pf_commit(&kv_empty[kn % SLOTS]);
+        }
+      } else {
+        // one row tile: S runs one tile ahead in the other buffer
+        if (n0 > 0) {
+          scores(0, 0, used % SLOTS);
+          pf_commit(&kv_empty[used % SLOTS]);
+        }
+        if (n0 > 1) {
+          ready(used + 2);
+          scores(0, 1, (used + 2) % SLOTS);
+          pf_commit(&kv_empty[(used + 2) % SLOTS]);
+        }
+        for (int j = 0; j < n0 && !is_dead(); ++j) {
+          const uint32_t v = used + 2 * j + 1, kn = v + 3;
+          const int buf = j & 1;
+          ready(v);
+          wait_one(&p_full[buf], n_p[buf] & 1);
+          ++n_p[buf];
+          if (is_dead()) break;
           pf_fence_after();
-          scores(i, j + 1);
-        } else {
-          pf_commit(&s_full[i]);
+          values(0, buf, v % SLOTS, j > 0);
+          pf_commit(&kv_empty[v % SLOTS]);
+          if (j + 2 < n0) {
+            ready(kn);
+            scores(0, buf, kn % SLOTS);
+            pf_commit(&kv_empty[kn % SLOTS]);
+          }
         }
       }
-      if (*(volatile int*)&dead) break;
-      pf_commit(&kv_empty[vs]);
-      if (j + 1 < n_max) pf_commit(&kv_empty[kn % SLOTS]);
+      used += 2 * n_max;
     }
     pf_commit(&drained);
     mbar_wait_bounded(&drained, 0);

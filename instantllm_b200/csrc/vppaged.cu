@@ -8,6 +8,9 @@
 #include "vp_paged.cuh"
 #include "vp_paged_decode.cuh"
 #include "vp_paged_host.h"
+#include "vp_paged_prefill.cuh"
+
+int pg_tiles(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st);  // vpprefill.cu
 
 using namespace vp;
 
@@ -48,6 +51,8 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 template <typename TI, typename T, int HD>
 __global__ void __launch_bounds__(APPEND_THREADS) k_paged_append(const vp_paged c, const vp_paged_rows r) {
   constexpr int J = HD / 16;
+  pdl_launch_dependents();
+  pdl_wait();
   const long long t = blockIdx.x;
   const int j = threadIdx.x % J;
   const int seq = r.seq[t], slot = r.slot[t];
@@ -131,11 +136,11 @@ __global__ void __launch_bounds__(APPEND_THREADS) k_paged_append(const vp_paged 
 namespace {
 
 template <typename TI, typename T>
-void append_launch(const vp_paged& c, const vp_paged_rows& r, cudaStream_t st) {
+int append_launch(const vp_paged& c, const vp_paged_rows& r, cudaStream_t st) {
   const int want = (r.n_q + 2 * c.n_kv) * (c.head_dim / 16);
   const int threads = want < APPEND_THREADS ? (want + 31) / 32 * 32 : APPEND_THREADS;
-  if (c.head_dim == 64) k_paged_append<TI, T, 64><<<r.rows, threads, 0, st>>>(c, r);
-  else k_paged_append<TI, T, 128><<<r.rows, threads, 0, st>>>(c, r);
+  return pg_launch("vp_paged_append", c.head_dim == 64 ? k_paged_append<TI, T, 64> : k_paged_append<TI, T, 128>, r.rows, threads, 0,
+                   st, c, r);
 }
 
 template <typename T, int HD>
@@ -145,24 +150,19 @@ int decode_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
   p.c = c;
   p.a = a;
   p.group = a.n_q / c.n_kv;
-  const int m = p.group * a.rows;
-  p.blocks = (m + DC_BLOCK_ROWS - 1) / DC_BLOCK_ROWS;
-  p.block_rows = m < DC_BLOCK_ROWS ? m : DC_BLOCK_ROWS;
-  p.mt = (p.block_rows + 15) / 16;
-  p.min_tiles = 4;
+  p.M = p.group * a.rows;
+  p.min_tiles = DC_WARPS * DC_STAGES;  // a CTA's ring: all of it flies at once
+  p.page_shift = __builtin_ctz(c.page_size);
   p.tickets = static_cast<unsigned*>(a.work);
   p.rec = reinterpret_cast<float*>(static_cast<char*>(a.work) + WORK_HEAD);
   CUtensorMap mk, mv;
-  if (const int e = pool_maps(c, c.page_size < Sh::TS ? c.page_size : Sh::TS, &mk, &mv)) return e;
+  if (const int e = pool_maps(c, c.page_size < Sh::TS ? c.page_size : Sh::TS, HD / 64, &mk, &mv)) return e;
   int sms = 0;
   if (const int e = sm_count(&sms)) return e;
   const int tiles = (int)(((long long)c.max_pages * c.page_size + Sh::TS - 1) / Sh::TS);
-  const long long most = (long long)a.n * c.n_kv * p.blocks * tiles;
-  const int grid = (int)(most < sms ? most : sms);
-  const cudaError_t e = cudaFuncSetAttribute(k_paged_decode<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM);
-  if (e != cudaSuccess) return pfail(VP_ERR_CUDA, cudaGetErrorString(e));
-  k_paged_decode<T, HD><<<grid, DC_THREADS, Sh::SMEM, st>>>(p, mk, mv);
-  return launched("vp_paged_decode");
+  const long long most = (long long)a.n * c.n_kv * tiles;
+  if (most > 0x7fffffff) return pfail(VP_ERR_ARG, "more slots than a launch holds");
+  return pg_launch("vp_paged_decode", k_paged_decode<T, HD>, (unsigned)(most < sms ? most : sms), DC_THREADS, Sh::SMEM, st, p, mk, mv);
 }
 
 }  // namespace
@@ -186,14 +186,9 @@ int vp_paged_append(const vp_paged* c, const vp_paged_rows* r, void* stream) try
       bad_strides(r->v_row, r->v_head, unit) || bad_strides(r->out_row, r->out_head, 8))
     return pfail(VP_ERR_ARG, "strides of rows must be multiples of 16 bytes");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (c->type == VP_T_F16) {
-    if (r->type == VP_T_F32) append_launch<float, __half>(*c, *r, st);
-    else append_launch<__half, __half>(*c, *r, st);
-  } else {
-    if (r->type == VP_T_F32) append_launch<float, __nv_bfloat16>(*c, *r, st);
-    else append_launch<__nv_bfloat16, __nv_bfloat16>(*c, *r, st);
-  }
-  return launched("vp_paged_append");
+  if (c->type == VP_T_F16)
+    return r->type == VP_T_F32 ? append_launch<float, __half>(*c, *r, st) : append_launch<__half, __half>(*c, *r, st);
+  return r->type == VP_T_F32 ? append_launch<float, __nv_bfloat16>(*c, *r, st) : append_launch<__nv_bfloat16, __nv_bfloat16>(*c, *r, st);
 } catch (const std::exception&) {
   return VP_ERR_NOMEM;
 }
@@ -201,9 +196,10 @@ int vp_paged_append(const vp_paged* c, const vp_paged_rows* r, void* stream) try
 size_t vp_paged_work_bytes(int32_t head_dim, int32_t n_q, int32_t n_kv, int32_t rows) {
   if ((head_dim != 64 && head_dim != 128) || n_kv < 1 || n_q < 1 || n_q % n_kv || n_q / n_kv > PG_MAX_GROUP || rows < 1)
     return 0;
-  const int m = n_q / n_kv * rows, block = m < DC_BLOCK_ROWS ? m : DC_BLOCK_ROWS;
-  const size_t record = head_dim == 64 ? DcShape<64>::record(block) : DcShape<128>::record(block);
-  return WORK_HEAD + (size_t)PG_MAX_CTAS * 2 * record * sizeof(float);
+  const long long m = (long long)n_q / n_kv * rows;
+  const size_t few = PG_MAX_CTAS * 2 * pg_record(m < DC_ROWS ? (int)m : DC_ROWS, head_dim);
+  const size_t many = PG_RECORDS * pg_record(m < PF_ROWS ? (int)m : PF_ROWS, head_dim);
+  return WORK_HEAD + (few > many ? few : many) * sizeof(float);
 }
 
 int vp_paged_decode(const vp_paged* c, const vp_paged_attn* a, void* stream) try {
@@ -211,6 +207,11 @@ int vp_paged_decode(const vp_paged* c, const vp_paged_attn* a, void* stream) try
   if (a->rows > PG_MAX_ROWS) return pfail(VP_ERR_ARG, "a decode call takes 1 to 16 rows per request");
   if (a->n == 0 || a->rows == 0) return VP_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->n_q / c->n_kv * a->rows > DC_ROWS) {
+    vp_paged_attn t = *a;
+    t.q_start = nullptr;
+    return pg_tiles(*c, t, st);
+  }
   if (c->type == VP_T_F16) return c->head_dim == 64 ? decode_launch<__half, 64>(*c, *a, st) : decode_launch<__half, 128>(*c, *a, st);
   return c->head_dim == 64 ? decode_launch<__nv_bfloat16, 64>(*c, *a, st) : decode_launch<__nv_bfloat16, 128>(*c, *a, st);
 } catch (const std::exception&) {

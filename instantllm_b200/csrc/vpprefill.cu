@@ -7,32 +7,44 @@
 namespace {
 
 template <typename T, int HD>
-int prefill_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
+int tiles_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
   using Sh = PfShape<HD>;
   PfParams p;
   p.c = c;
   p.a = a;
   p.group = a.n_q / c.n_kv;
+  const long long rows = (long long)a.rows * p.group;  // packed, of a request (tree) or of all
+  if (rows > 0x7fffff00ll) return pfail(VP_ERR_ARG, "more rows than a launch holds");
+  p.block_rows = rows < PF_ROWS ? (int)rows : PF_ROWS;
+  p.tickets = static_cast<unsigned*>(a.work);
+  p.rec = reinterpret_cast<float*>(static_cast<char*>(a.work) + WORK_HEAD);
+  if (const int e = sm_count(&p.sms)) return e;
   CUtensorMap mk, mv;
-  if (const int e = pool_maps(c, c.page_size < PF_TS ? c.page_size : PF_TS, &mk, &mv)) return e;
-  // every request's last block may be short
-  const long long blocks = ((long long)a.rows * p.group + PF_ROWS - 1) / PF_ROWS + a.n;
-  if (blocks * c.n_kv > 0x7fffffffll) return pfail(VP_ERR_ARG, "more rows than a launch holds");
-  const cudaError_t e = cudaFuncSetAttribute(k_paged_prefill<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM);
-  if (e != cudaSuccess) return pfail(VP_ERR_CUDA, cudaGetErrorString(e));
-  k_paged_prefill<T, HD><<<(unsigned)(blocks * c.n_kv), PF_THREADS, Sh::SMEM, st>>>(p, mk, mv);
-  return launched("vp_paged_prefill");
+  if (const int e = pool_maps(c, c.page_size < PF_TS ? c.page_size : PF_TS, 1, &mk, &mv)) return e;
+  // at most this many pieces: every request's last block may be short, and the cuts add two CTAs per
+  // SM at most, or as many as the table's longest request allows
+  const long long blocks = a.q_start ? rows / PF_ROWS + a.n : (rows + PF_ROWS - 1) / PF_ROWS * a.n;
+  const long long pairs = blocks * c.n_kv, tiles = ((long long)c.max_pages * c.page_size + PF_TS - 1) / PF_TS;
+  const long long cuts = (tiles + PF_LEAST - 1) / PF_LEAST - 1, more = pairs * cuts < 2 * p.sms ? pairs * cuts : 2 * p.sms;
+  if (pairs + more > 0x7fffffffll) return pfail(VP_ERR_ARG, "more rows than a launch holds");
+  p.most = (int)(pairs + more);
+  return pg_launch(a.q_start ? "vp_paged_prefill" : "vp_paged_decode", k_paged_tiles<T, HD>, p.most < p.sms ? p.most : p.sms, PF_THREADS,
+                   Sh::SMEM, st, p, mk, mv);
 }
 
 }  // namespace
+
+// Prompts (q_start set), or the new rows of vp_paged_decode.
+int pg_tiles(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
+  if (c.type == VP_T_F16) return c.head_dim == 64 ? tiles_launch<__half, 64>(c, a, st) : tiles_launch<__half, 128>(c, a, st);
+  return c.head_dim == 64 ? tiles_launch<__nv_bfloat16, 64>(c, a, st) : tiles_launch<__nv_bfloat16, 128>(c, a, st);
+}
 
 extern "C" int vp_paged_prefill(const vp_paged* c, const vp_paged_attn* a, void* stream) try {
   if (const int e = check_attn(c, a)) return e;
   if (a->n == 0 || a->rows == 0) return VP_OK;
   if (!a->q_start) return pfail(VP_ERR_ARG, "null q_start");
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (c->type == VP_T_F16) return c->head_dim == 64 ? prefill_launch<__half, 64>(*c, *a, st) : prefill_launch<__half, 128>(*c, *a, st);
-  return c->head_dim == 64 ? prefill_launch<__nv_bfloat16, 64>(*c, *a, st) : prefill_launch<__nv_bfloat16, 128>(*c, *a, st);
+  return pg_tiles(*c, *a, static_cast<cudaStream_t>(stream));
 } catch (const std::exception&) {
   return VP_ERR_NOMEM;
 }

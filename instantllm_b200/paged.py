@@ -25,6 +25,7 @@ from ._lib import VpError, VpPaged, VpPagedAttn, VpPagedRows, check
 TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 DEV_ERR_PAGE, DEV_ERR_SLOT = 16, 32
 MAX_ROWS = 16
+WORK_ZEROED = 8192
 
 
 def rope_table(rows: int, rot_dim: int = 64, theta: float = 1e6, device=0) -> torch.Tensor:
@@ -200,10 +201,11 @@ class PagedLayer:
             a.seqs = None
         else:
             a.seqs = _index(seqs, "seqs", (n,), self.device)
-        need = self.lib.vp_paged_work_bytes(self.head_dim, nq, self.n_kv, min(rows, MAX_ROWS))
+        need = self.lib.vp_paged_work_bytes(self.head_dim, nq, self.n_kv, rows)
         work = self._work[0]
         if work is None or work.numel() < need:
-            work = self._work[0] = torch.zeros(max(need, 256), dtype=torch.uint8, device=self.device)
+            work = self._work[0] = torch.empty(max(need, WORK_ZEROED), dtype=torch.uint8, device=self.device)
+            work[:WORK_ZEROED].zero_()
         a.work, a.work_bytes = work.data_ptr(), work.numel()
         a.scale = self.head_dim ** -0.5 if scale is None else scale
         a.n, a.rows, a.n_q, a.window, a.sinks = n, rows, nq, window, sinks
