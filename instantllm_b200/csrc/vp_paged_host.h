@@ -15,9 +15,7 @@ namespace {
 using namespace vp;
 
 constexpr int PG_MAX_CTAS = 160;       // CTAs of an attention launch, one per SM (148 on a B200)
-constexpr int PG_RECORDS = 4 * PG_MAX_CTAS;  // of cut blocks: a piece has half an even share of all tiles on average
 constexpr size_t WORK_HEAD = VP_PAGED_WORK_ZEROED;  // counters at the head of the work buffer
-static_assert(2 * PG_RECORDS * sizeof(unsigned) <= WORK_HEAD, "counters");
 
 int pfail(int code, const char* msg) {
   vp_set_last_error(msg);

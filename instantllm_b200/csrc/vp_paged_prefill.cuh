@@ -27,6 +27,7 @@ constexpr int PF_TS = 128;                 // slots per tile
 constexpr int PF_ROWS = 256;               // packed query rows per CTA
 constexpr int PF_THREADS = 384;            // two softmax warpgroups, then one: producer, issuer, scheduler, an idle warp
 constexpr int PF_PRODUCER = 8, PF_ISSUER = 9, PF_SCHEDULER = 10;
+constexpr int PF_SOFTMAX_REGS = 208, PF_OTHER_REGS = 88;  // of the 168 a thread that the block is launched with
 constexpr uint32_t PF_TMEM = 512;          // columns
 constexpr float PF_SLACK = 8.f;            // log2 of the largest weight
 
@@ -38,13 +39,14 @@ struct PfShape {
   static constexpr size_t SMEM = 1024 + 2 * TILE + (size_t)SLOTS * TILE;
 };
 
+constexpr int PF_RECORDS = 640;            // records at most: four per SM, for 160
 constexpr int PF_LEAST = 4;                // tiles of a piece, at least
 
 struct PfParams {
   vp_paged c;
   vp_paged_attn a;
   float* rec;         // records of block_rows rows, one per piece of a cut block
-  unsigned* tickets;  // [records][2 row tiles]
+  unsigned* tickets;  // [records][2 row tiles], then the scheduler's two
   int group, block_rows, sms, most;  // most: pieces that a call can have
 };
 
@@ -188,8 +190,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   extern __shared__ unsigned char smem_raw[];
   unsigned char* qs = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   unsigned char* ring = qs + 2 * TILE;
-  // s_full: S of a buffer is there; p_full: its weights are; o_full: a product into o is done
-  __shared__ uint64_t kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_full[2], o_full[2], q_full, edge, drained, info_full[2], info_empty[2];
+  // s_full: S of a buffer is there; p_full: its weights are; o_full: a product into o is done; o_last: the piece's last one is
+  __shared__ uint64_t kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_full[2], o_full[2], o_last[2], q_full, edge, drained, info_full[2], info_empty[2];
   __shared__ uint32_t tmem_base;
   __shared__ long long tile_sums[PF_THREADS / 32];
   __shared__ int sums[PF_THREADS / 32][2], starts[PF_THREADS], rec_starts[PF_THREADS], dead, last_s[2];
@@ -210,6 +212,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&o_full[i], 1);
+      mbar_init(&o_last[i], 1);
       mbar_init(&info_full[i], 1);
       mbar_init(&info_empty[i], 10);  // the softmax warps, the producer, the issuer
     }
@@ -286,17 +289,19 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   cta_sync();
   const uint32_t tmem = tmem_base;
 
-  auto wait_warp = [&](uint64_t* bar, uint32_t parity) {  // whole warp
+  // Waits of a whole warp, of one thread. After one that ran out none waits any more, and the call ends
+  // with an error status.
+  auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
     __syncwarp();
-    if (*(volatile int*)&dead) return;
-    if (!mbar_wait_warp(bar, parity)) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return;
+    if (!*(volatile int*)&dead && !mbar_wait_warp(bar, parity)) {
       pg_status(c.status, VP_DEV_ERR_TIMEOUT);
       *(volatile int*)&dead = 1;
     }
     __syncwarp();
   };
-  auto wait_one = [&](uint64_t* bar, uint32_t parity) {  // one thread
-    if (*(volatile int*)&dead) return;
+  auto wait_one = [&](uint64_t* bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity) || *(volatile int*)&dead) return;
     if (!mbar_wait_bounded(bar, parity)) {
       pg_status(c.status, VP_DEV_ERR_TIMEOUT);
       *(volatile int*)&dead = 1;
@@ -305,6 +310,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   auto is_dead = [&] { return *(volatile int*)&dead != 0; };
 
   if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PF_SOFTMAX_REGS));
     // ---- softmax: warpgroup i has row tile i, a thread row f ----
     const int i = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 lanes of tensor memory
@@ -312,9 +318,25 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     const float cexp = a.scale * 1.4426950408889634f;
     const size_t rec_floats = pg_record(p.block_rows, HD);
     const int m_at = p.block_rows * HD, l_at = m_at + p.block_rows;
-    uint32_t n_s[2] = {0, 0}, n_o = 0;  // phases of s_full and p_full, of o_full so far
-    for (int r = 0;; ++r) {
+    uint32_t n_s[2] = {0, 0}, n_o = 0, n_last = 0;  // phases of s_full and p_full, of o_full, of o_last so far
+    // Queries of piece r on their way into the row tile's buffer, once the last product that reads it is done.
+    auto fetch = [&](int r) {
       wait_warp(&info_full[r & 1], (r >> 1) & 1);
+      const PfPiece& in = info[r & 1];
+      const int f = in.f0 + tid;
+      if (in.seq >= 0 && f < in.f_end) {
+        const T* q = static_cast<const T*>(a.q) + in.seq * a.q_seq + (long long)(in.first + f / p.group) * a.q_row +
+                     (in.head * p.group + f % p.group) * a.q_head;
+        unsigned char* dst = qs + i * TILE + row * 128;
+#pragma unroll
+        for (int d = 0; d < HD / 8; ++d) pg_cp16(dst + (d / 8) * PANEL + (((d & 7) ^ (row & 7)) << 4), q + d * 8);
+      }
+      __syncwarp();
+    };
+    bool fetched = false;
+    for (int r = 0;; ++r) {
+      if (!fetched) fetch(r);
+      fetched = false;
       const PfPiece& in = info[r & 1];
       const int seq = in.seq, f = in.f0 + tid, f_end = in.f_end, f0 = in.f0, head = in.head, first = in.first, base = in.base;
       if (seq < 0 || is_dead()) break;
@@ -337,13 +359,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       }
       __syncwarp();
       if (lane == 0) pg_arrive(&info_empty[r & 1]);
-      {  // queries: the products of the last piece that read the buffer are done
-        const T* q = static_cast<const T*>(a.q) + seq * a.q_seq + (long long)(first + qrow) * a.q_row + h * a.q_head;
-        unsigned char* dst = qs + i * TILE + row * 128;
-        if (valid) {
-#pragma unroll
-          for (int d = 0; d < HD / 8; ++d) pg_cp16(dst + (d / 8) * PANEL + (((d & 7) ^ (row & 7)) << 4), q + d * 8);
-        }
+      {
         asm volatile("cp.async.wait_all;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -365,6 +381,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         uint32_t s[128];
 #pragma unroll
         for (int k = 0; k < 4; ++k) pf_ld32(s + 32 * k, ts + 32 * k);
+        if (j + 1 == n_t) {  // the last scores are there: the next piece's queries may come
+          fetch(r + 1);
+          fetched = true;
+        }
         pf_loaded(s);
         if (s0 + PF_TS > hi_all || (s0 < lo_all && s0 + PF_TS > a.sinks)) {
 #pragma unroll
@@ -430,10 +450,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         __syncwarp();
         if (lane == 0) pg_arrive(&p_full[buf]);
       }
-      // the last products into o, one phase after the other
-      if (n_t > 1 && !two) wait_warp(&o_full[i], (n_o + n_t - 2) & 1);
       if (n_t > 0) {
-        wait_warp(&o_full[i], (n_o + n_t - 1) & 1);
+        wait_warp(&o_last[i], n_last & 1);
+        ++n_last;
         pf_fence_after();
       }
       n_o += n_t;
@@ -489,46 +508,63 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           __syncwarp();
           asm volatile("barrier.sync %0, 128;" ::"r"(1 + i) : "memory");
           if (last_s[i]) {
-            // All pieces of the row tile are there. A warp takes rows in turn: its lanes first the weights
-            // of 32 pieces, then 4 elements each (two rows at head_dim 64).
+            // All pieces of the row tile are there: a thread a row, their weights in place of their maxima;
+            // then 4 elements a thread and turn, two turns' reads of 8 pieces in flight.
             __threadfence();
-            const float* rec0 = p.rec + (size_t)record0 * rec_floats;
+            float* rec0 = p.rec + (size_t)record0 * rec_floats;
             const int n_rows = min(128, f_end - f0 - i * 128);
-            constexpr int LR = HD / 4, RW = 32 / LR;  // lanes per row, rows at a time
-            const int d = lane % LR * 4;
-            for (int x0 = (warp & 3) * RW; x0 < n_rows; x0 += 4 * RW) {
-              const int mm = i * 128 + min(x0 + lane / LR, n_rows - 1);
-              float top = -INFINITY;
-              for (int k = 0; k < live; ++k) top = fmaxf(top, __ldcg(rec0 + k * rec_floats + m_at + mm));
+            if (row < n_rows) {
+              float top = -INFINITY, sm = 0.f;
+#pragma unroll 8
+              for (int k = 0; k < live; ++k) top = fmaxf(top, __ldcg(rec0 + k * rec_floats + m_at + tid));
               const float us = top == -INFINITY ? 0.f : top;
-              float sm = 0.f;
-              float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-              for (int k0 = 0; k0 < live; k0 += 8) {  // 8 records' reads fly together
-                float4 v8[8];
-                float m8[8], l8[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                  const float* x = rec0 + (size_t)min(k0 + k, live - 1) * rec_floats;
-                  v8[k] = __ldcg(reinterpret_cast<const float4*>(x + (size_t)mm * HD + d));
-                  m8[k] = __ldcg(x + m_at + mm);
-                  l8[k] = __ldcg(x + l_at + mm);
-                }
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                  const float w = k0 + k < live ? pg_exp2(m8[k] - us) : 0.f;
-                  sm += l8[k] * w;
-                  acc.x += v8[k].x * w, acc.y += v8[k].y * w, acc.z += v8[k].z * w, acc.w += v8[k].w * w;
-                }
-              }
+#pragma unroll 8
+              for (int k = 0; k < live; ++k)
+                sm += __ldcg(rec0 + k * rec_floats + l_at + tid) * pg_exp2(__ldcg(rec0 + k * rec_floats + m_at + tid) - us);
               const float iv = sm > 0.f ? 1.f / sm : sm == 0.f ? 0.f : sm;
-              const int r2 = (f0 + mm) / p.group, h2 = head * p.group + (f0 + mm) % p.group;
-              uint2 v2;
-              v2.x = PgType<T>::down(acc.x * iv, acc.y * iv);
-              v2.y = PgType<T>::down(acc.z * iv, acc.w * iv);
-              *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + seq * a.out_seq + (long long)(first + r2) * a.out_row + h2 * a.out_head + d) = v2;
-              if (a.lse && d == 0)
-                a.lse[((tree ? (long long)seq * a.rows : (long long)first) + r2) * a.n_q + h2] =
-                    sm == 0.f ? -INFINITY : (top + log2f(sm)) * 0.6931471805599453f;
+#pragma unroll 8
+              for (int k = 0; k < live; ++k) {
+                float* x = rec0 + k * rec_floats + m_at + tid;
+                *x = pg_exp2(__ldcg(x) - us) * iv;
+              }
+              if (lse) *lse = sm == 0.f ? -INFINITY : (top + log2f(sm)) * 0.6931471805599453f;
+            }
+            __threadfence();
+            __syncwarp();
+            asm volatile("barrier.sync %0, 128;" ::"r"(1 + i) : "memory");
+            for (int x0 = row; x0 < n_rows * (HD / 4); x0 += 256) {
+              float4 acc[2] = {};
+              const int x1 = min(x0 + 128, n_rows * (HD / 4) - 1);
+              const int mm[2] = {i * 128 + x0 / (HD / 4), i * 128 + x1 / (HD / 4)}, d[2] = {x0 % (HD / 4) * 4, x1 % (HD / 4) * 4};
+              for (int k0 = 0; k0 < live; k0 += 4) {
+                float4 v[2][4];
+                float w[2][4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const float* x = rec0 + (size_t)min(k0 + k, live - 1) * rec_floats;
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    v[e][k] = __ldcg(reinterpret_cast<const float4*>(x + (size_t)mm[e] * HD + d[e]));
+                    w[e][k] = __ldcg(x + m_at + mm[e]);
+                  }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const float f1 = k0 + k < live ? w[e][k] : 0.f;
+                    acc[e].x += v[e][k].x * f1, acc[e].y += v[e][k].y * f1, acc[e].z += v[e][k].z * f1, acc[e].w += v[e][k].w * f1;
+                  }
+              }
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                if (e && x0 + 128 >= n_rows * (HD / 4)) break;
+                const int r2 = (f0 + mm[e]) / p.group, h2 = head * p.group + (f0 + mm[e]) % p.group;
+                uint2 v2;
+                v2.x = PgType<T>::down(acc[e].x, acc[e].y);
+                v2.y = PgType<T>::down(acc[e].z, acc[e].w);
+                *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + seq * a.out_seq + (long long)(first + r2) * a.out_row + h2 * a.out_head + d[e]) = v2;
+              }
             }
             if (row == 0) *ticket = 0;
           }
@@ -537,13 +573,20 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       }
       pf_fence_before();
     }
-  } else if (warp == PF_SCHEDULER) {
-    // ---- the CTA's pieces: in turns over the CTAs, there and back, from the last request's last block on ----
-    const int G = gridDim.x;
+  } else {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_OTHER_REGS));
+  if (warp == PF_SCHEDULER) {
+    // ---- the CTA's pieces: one for each CTA, then whoever comes first has the next, from the last request's
+    // last block on. Which CTA has a piece does not show in the results. ----
+    unsigned* next = p.tickets + 2 * PF_RECORDS;  // and the number of CTAs that have come to the end
     for (int r = 0;; ++r) {
       if (r >= 2) wait_warp(&info_empty[r & 1], ((r >> 1) - 1) & 1);
-      const int idx = r * G + (r & 1 ? G - 1 - (int)blockIdx.x : (int)blockIdx.x);
-      int piece = total - 1 - idx;
+      unsigned idx = blockIdx.x;
+      if (r > 0) {
+        if (lane == 0) idx = gridDim.x + atomicAdd(next, 1u);
+        idx = __shfl_sync(0xffffffffu, idx, 0);
+      }
+      int piece = idx < (unsigned)total ? total - 1 - (int)idx : -1;
       if (total > p.most) {  // requests whose rows overlap
         if (lane == 0) pg_status(c.status, VP_DEV_ERR_SLOT);
         piece = -1;
@@ -553,6 +596,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         if (lane == 0) {
           in.seq = -1;
           pg_arrive(&info_full[r & 1]);
+          if (atomicAdd(next + 1, 1u) == gridDim.x - 1) next[0] = next[1] = 0;  // the last one leaves them as it found them
         }
         break;
       }
@@ -688,12 +732,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       }
       pf_commit(&s_full[buf]);
     };
-    auto values = [&](int i, int buf, uint32_t st, bool add) {  // o_i += P buffer V
+    auto values = [&](int i, int buf, uint32_t st, bool add, bool last) {  // o_i += P buffer V
       const uint32_t vb = rb + st * TILE;
 #pragma unroll
       for (int k = 0; k < PF_TS / 16; ++k)
         pf_mma_ts(tmem + 256 + i * HD, tmem + buf * 128 + k * 8, pf_desc(vb + k * 2048, PANEL, 1024), ID_O, add || k > 0);
       pf_commit(&o_full[i]);
+      if (last) pf_commit(&o_last[i]);
     };
     uint32_t used = 0, n_p[2] = {0, 0};  // K and V tiles so far, phases of p_full so far
     auto ready = [&](uint32_t k) {        // tile k of the ring is there
@@ -723,16 +768,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           for (int i = 0; i < 2; ++i) {
             const int n_t = i ? n1 : n0;
             if (j >= n_t) continue;
+            if (j + 1 < n_t && !k_there) ready(kn), k_there = true;
             wait_one(&p_full[i], n_p[i] & 1);
             ++n_p[i];
-            if (is_dead()) break;
             pf_fence_after();
-            values(i, i, v % SLOTS, j > 0);
+            values(i, i, v % SLOTS, j > 0, j + 1 == n_t);
+            if (j + 1 < n_t) scores(i, i, kn % SLOTS);
             if (i == 1 || j >= n1) pf_commit(&kv_empty[v % SLOTS]);
-            if (j + 1 < n_t) {
-              if (!k_there) ready(kn), k_there = true;
-              scores(i, i, kn % SLOTS);
-            }
           }
           if (j + 1 < n_max) pf_commit(&kv_empty[kn % SLOTS]);
         }
@@ -753,9 +795,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           ready(v);
           wait_one(&p_full[buf], n_p[buf] & 1);
           ++n_p[buf];
-          if (is_dead()) break;
           pf_fence_after();
-          values(0, buf, v % SLOTS, j > 0);
+          values(0, buf, v % SLOTS, j > 0, j + 1 == n0);
           pf_commit(&kv_empty[v % SLOTS]);
           if (j + 2 < n0) {
             ready(kn);
@@ -769,6 +810,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     pf_commit(&drained);
     mbar_wait_bounded(&drained, 0);
     pf_fence_before();
+  }
   }
   cta_sync();
   pf_fence_after();

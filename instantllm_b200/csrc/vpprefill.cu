@@ -6,6 +6,8 @@
 
 namespace {
 
+static_assert(PF_RECORDS >= 4 * PG_MAX_CTAS && (2 * PF_RECORDS + 2) * sizeof(unsigned) <= WORK_HEAD, "records and their counters");
+
 template <typename T, int HD>
 int tiles_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
   using Sh = PfShape<HD>;
@@ -19,6 +21,12 @@ int tiles_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
   p.tickets = static_cast<unsigned*>(a.work);
   p.rec = reinterpret_cast<float*>(static_cast<char*>(a.work) + WORK_HEAD);
   if (const int e = sm_count(&p.sms)) return e;
+  // the warpgroups trade registers: what the softmax takes on must have been launched with
+  static const int regs = [] {
+    cudaFuncAttributes f{};
+    return cudaFuncGetAttributes(&f, k_paged_tiles<T, HD>) == cudaSuccess ? f.numRegs : 0;
+  }();
+  if (regs * PF_THREADS < 2 * 128 * PF_SOFTMAX_REGS + 128 * PF_OTHER_REGS) return pfail(VP_ERR_CUDA, "the kernel was built with too few registers");
   CUtensorMap mk, mv;
   if (const int e = pool_maps(c, c.page_size < PF_TS ? c.page_size : PF_TS, 1, &mk, &mv)) return e;
   // at most this many pieces: every request's last block may be short, and the cuts add two CTAs per

@@ -23,7 +23,7 @@ from . import _lib
 from ._lib import VpError, VpPaged, VpPagedAttn, VpPagedRows, check
 
 TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
-DEV_ERR_PAGE, DEV_ERR_SLOT = 16, 32
+DEV_ERR_TIMEOUT, DEV_ERR_PAGE, DEV_ERR_SLOT = 4, 16, 32
 MAX_ROWS = 16
 WORK_ZEROED = 8192
 
@@ -212,13 +212,15 @@ class PagedLayer:
         return out, lse
 
     def check(self) -> None:
-        """Raises VpError if a call met a page or slot outside the table since the last check(); synchronises."""
+        """Raises VpError if a call met a page or slot outside the table, or gave up a wait, since the last check();
+        synchronises."""
         bits = int(self.status.item())
         if bits:
             self.status.zero_()
-            raise VpError("the cache was given " + " and ".join(
-                t for b, t in ((DEV_ERR_PAGE, "a page outside the pool"), (DEV_ERR_SLOT, "a request, slot, position or length outside the table"))
-                if bits & b))
+            raise VpError("the cache's calls met " + " and ".join(t for b, t in (
+                (DEV_ERR_PAGE, "a page outside the pool"),
+                (DEV_ERR_SLOT, "a request, slot, position or length outside the table"),
+                (DEV_ERR_TIMEOUT, "a wait that ran out: their results are void")) if bits & b))
 
 
 class PagedKV:

@@ -426,6 +426,44 @@ def test_prefill_long(nq, nkv, hd, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["trees", "prompts", "chunks"])
+def test_many_requests(kind):
+    """More work than CTAs: every CTA goes through several requests, some of them cut in pieces, calls follow one another
+    without a pause and give the same bits each time; rows are sampled."""
+    rng = np.random.default_rng(11)
+    nq, nkv, hd, ps, dtype = 14, 2, 64, 64, torch.float16
+    lens = [int(x) for x in np.exp(rng.uniform(np.log(20), np.log(2500), 70))]
+    lens[7], lens[40] = 6000, 0
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, ps, dtype, fill=float("nan"))
+    ln = torch.tensor(lens, dtype=torch.int32).cuda()
+    if kind == "trees":
+        q = torch.from_numpy(rng.standard_normal((70, 16, nq, hd)).astype(np.float32)).to(dtype)
+        masks = tree_masks(rng, 70, 16)
+        d, m = q.cuda(), torch.from_numpy(masks.astype(np.int32)).cuda()
+        outs = [kv.decode(d, ln, mask=m, return_lse=True) for _ in range(20)]
+        pick = [3, 7, 40, 69]
+        want = [((pick[at[0]],) + at[1:], o, n) for at, o, n in
+                want_decode(q[pick].double().numpy(), k, v, table[pick], [lens[i] for i in pick], masks[pick], 0, 0, hd ** -0.5, ps)]
+    else:
+        new = [n if kind == "prompts" else min(n, 50) for n in lens]
+        starts = np.concatenate([[0], np.cumsum(new)])
+        q = torch.from_numpy(rng.standard_normal((int(starts[-1]), nq, hd)).astype(np.float32)).to(dtype)
+        d, qs = q.cuda(), torch.from_numpy(starts.astype(np.int32)).cuda()
+        outs = [kv.prefill(d, qs, ln, return_lse=True) for _ in range(20)]
+        want = []
+        for t in rng.choice(int(starts[-1]), 30, replace=False):
+            i = int(np.searchsorted(starts, t, side="right") - 1)
+            p = lens[i] - new[i] + t - starts[i]
+            ks, vs = (O.slots(x, table[i], p + 1) for x in (k, v))
+            for h in (0, 6, 7, 13):
+                want.append(((t, h), O.attend(q[t, h].double().numpy(), ks[h // 7], vs[h // 7], np.ones(p + 1, dtype=bool), hd ** -0.5), p + 1))
+    kv.check()
+    for o, lse in outs[1:]:
+        assert torch.equal(o, outs[0][0]) and torch.equal(lse, outs[0][1])
+    compare(*outs[0], want, dtype, hd)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("src,dtype", [(torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16),
                                        (torch.float32, torch.float16), (torch.float32, torch.bfloat16)])
 @pytest.mark.parametrize("nq,nkv,hd,rot,interleaved,layout", [(14, 2, 64, 64, False, "hnd"), (8, 2, 128, 128, True, "nhd"),
