@@ -55,6 +55,11 @@ __device__ __forceinline__ uint64_t pf_desc(uint32_t addr, uint32_t lead, uint32
   return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((lead >> 4) & 0x3fff) << 16 | (uint64_t)((stride >> 4) & 0x3fff) << 32 |
          1ull << 46 | 2ull << 61;
 }
+__device__ __forceinline__ bool pf_elect() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void pf_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
@@ -289,7 +294,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   cta_sync();
   const uint32_t tmem = tmem_base;
 
-  // Waits of a whole warp, of one thread. After one that ran out none waits any more, and the call ends
+  // Waits of a whole warp. After one that ran out none waits any more, and the call ends
   // with an error status.
   auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
     __syncwarp();
@@ -299,13 +304,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       *(volatile int*)&dead = 1;
     }
     __syncwarp();
-  };
-  auto wait_one = [&](uint64_t* bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity) || *(volatile int*)&dead) return;
-    if (!mbar_wait_bounded(bar, parity)) {
-      pg_status(c.status, VP_DEV_ERR_TIMEOUT);
-      *(volatile int*)&dead = 1;
-    }
   };
   auto is_dead = [&] { return *(volatile int*)&dead != 0; };
 
@@ -406,7 +404,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * cexp;
         const bool move = top > m + PF_SLACK || (m == -INFINITY && top > m);
         if (__any_sync(0xffffffffu, move)) {
-          const float mn = fmaxf(m, top), fac = m == -INFINITY ? 0.f : pg_exp2(m - mn);
+          // a row's maximum moves by its own scores alone: what the other rows of the warp hold (rows past the
+          // block's end: anything) must not show in its bits
+          const float mn = move ? top : m, fac = m == -INFINITY ? 0.f : pg_exp2(m - mn);
           l *= fac;
           m = mn;
           if (j > 0) {
@@ -717,49 +717,61 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     }
     // copies still in flight land before the CTA may end (they have, unless a wait ran out)
     for (uint32_t k = issued > SLOTS ? issued - SLOTS : 0; k < issued; ++k) mbar_wait_warp(&kv_full[k % SLOTS], (k / SLOTS) & 1);
-  } else if (warp == PF_ISSUER && lane == 0) {
-    // ---- products ----
+  } else if (warp == PF_ISSUER) {
+    // ---- products. The whole warp walks, one elected lane issues: what the operands' descriptors come from
+    // is the same in every lane and known to be (shuffles), so that they live in uniform registers. With
+    // one lane walking alone every product took 100 clocks to issue, more than it takes to compute. ----
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const bool lead = pf_elect();
     constexpr uint32_t FMT = PgType<T>::BF16 ? 1u : 0u;
     constexpr uint32_t ID_S = 1u << 4 | FMT << 7 | FMT << 10 | (PF_TS / 8) << 17 | (128 / 16) << 24;
     constexpr uint32_t ID_O = 1u << 4 | FMT << 7 | FMT << 10 | 1u << 16 | (HD / 8) << 17 | (128 / 16) << 24;
-    const uint32_t qb = smem_u32(qs), rb = smem_u32(ring);
+    const uint32_t qb = __shfl_sync(0xffffffffu, smem_u32(qs), 0), rb = __shfl_sync(0xffffffffu, smem_u32(ring), 0);
     auto scores = [&](int i, int buf, uint32_t st) {  // S buffer = Q_i K^T
-      const uint32_t kb = rb + st * TILE, qa = qb + i * TILE;
+      const uint64_t kd = pf_desc(rb + st * TILE, 16, 1024), qd = pf_desc(qb + i * TILE, 16, 1024);
+      if (!lead) return;
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k) {
-        const uint32_t off = (k / 4) * PANEL + (k & 3) * 32;
-        pf_mma_ss(tmem + buf * 128, pf_desc(qa + off, 16, 1024), pf_desc(kb + off, 16, 1024), ID_S, k > 0);
+        const uint32_t off = ((k / 4) * PANEL + (k & 3) * 32) >> 4;
+        pf_mma_ss(tm + buf * 128, qd + off, kd + off, ID_S, k > 0);
       }
       pf_commit(&s_full[buf]);
     };
     auto values = [&](int i, int buf, uint32_t st, bool add, bool last) {  // o_i += P buffer V
-      const uint32_t vb = rb + st * TILE;
+      const uint64_t vd = pf_desc(rb + st * TILE, PANEL, 1024);
+      if (!lead) return;
 #pragma unroll
-      for (int k = 0; k < PF_TS / 16; ++k)
-        pf_mma_ts(tmem + 256 + i * HD, tmem + buf * 128 + k * 8, pf_desc(vb + k * 2048, PANEL, 1024), ID_O, add || k > 0);
+      for (int k = 0; k < PF_TS / 16; ++k) pf_mma_ts(tm + 256 + i * HD, tm + buf * 128 + k * 8, vd + k * 128, ID_O, add || k > 0);
       pf_commit(&o_full[i]);
       if (last) pf_commit(&o_last[i]);
     };
+    auto free_tile = [&](uint64_t* bar) {
+      if (lead) pf_commit(bar);
+    };
     uint32_t used = 0, n_p[2] = {0, 0};  // K and V tiles so far, phases of p_full so far
     auto ready = [&](uint32_t k) {        // tile k of the ring is there
-      wait_one(&kv_full[k % SLOTS], (k / SLOTS) & 1);
+      wait_warp(&kv_full[k % SLOTS], (k / SLOTS) & 1);
       pf_fence_after();
     };
     for (int r = 0;; ++r) {
-      wait_one(&info_full[r & 1], (r >> 1) & 1);
+      wait_warp(&info_full[r & 1], (r >> 1) & 1);
       const PfPiece& in = info[r & 1];
-      const int seq = in.seq, n0 = in.n0, n1 = in.n1, n_max = max(n0, n1);
-      const bool two = n1 > 0 || in.f_end > in.f0 + 128;
+      const int seq = __shfl_sync(0xffffffffu, in.seq, 0), n0 = __shfl_sync(0xffffffffu, in.n0, 0), n1 = __shfl_sync(0xffffffffu, in.n1, 0);
+      const int n_max = max(n0, n1);
+      const bool two = n1 > 0 || __shfl_sync(0xffffffffu, in.f_end - in.f0, 0) > 128;
       if (seq < 0 || is_dead()) break;
-      pg_arrive(&info_empty[r & 1]);
-      pg_arrive(&q_full);
-      wait_one(&q_full, r & 1);
+      __syncwarp();
+      if (lead) {
+        pg_arrive(&info_empty[r & 1]);
+        pg_arrive(&q_full);
+      }
+      wait_warp(&q_full, r & 1);
       pf_fence_after();
       if (n_max > 0) ready(used);
       if (two) {
         if (n0 > 0) scores(0, 0, used % SLOTS);
         if (n1 > 0) scores(1, 1, used % SLOTS);
-        if (n_max > 0) pf_commit(&kv_empty[used % SLOTS]);
+        if (n_max > 0) free_tile(&kv_empty[used % SLOTS]);
         for (int j = 0; j < n_max && !is_dead(); ++j) {
           const uint32_t v = used + 2 * j + 1, kn = v + 1;
           ready(v);
@@ -769,46 +781,46 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
             const int n_t = i ? n1 : n0;
             if (j >= n_t) continue;
             if (j + 1 < n_t && !k_there) ready(kn), k_there = true;
-            wait_one(&p_full[i], n_p[i] & 1);
+            wait_warp(&p_full[i], n_p[i] & 1);
             ++n_p[i];
             pf_fence_after();
             values(i, i, v % SLOTS, j > 0, j + 1 == n_t);
             if (j + 1 < n_t) scores(i, i, kn % SLOTS);
-            if (i == 1 || j >= n1) pf_commit(&kv_empty[v % SLOTS]);
+            if (i == 1 || j >= n1) free_tile(&kv_empty[v % SLOTS]);
           }
-          if (j + 1 < n_max) pf_commit(&kv_empty[kn % SLOTS]);
+          if (j + 1 < n_max) free_tile(&kv_empty[kn % SLOTS]);
         }
       } else {
         // one row tile: S runs one tile ahead in the other buffer
         if (n0 > 0) {
           scores(0, 0, used % SLOTS);
-          pf_commit(&kv_empty[used % SLOTS]);
+          free_tile(&kv_empty[used % SLOTS]);
         }
         if (n0 > 1) {
           ready(used + 2);
           scores(0, 1, (used + 2) % SLOTS);
-          pf_commit(&kv_empty[(used + 2) % SLOTS]);
+          free_tile(&kv_empty[(used + 2) % SLOTS]);
         }
         for (int j = 0; j < n0 && !is_dead(); ++j) {
           const uint32_t v = used + 2 * j + 1, kn = v + 3;
           const int buf = j & 1;
           ready(v);
-          wait_one(&p_full[buf], n_p[buf] & 1);
+          wait_warp(&p_full[buf], n_p[buf] & 1);
           ++n_p[buf];
           pf_fence_after();
           values(0, buf, v % SLOTS, j > 0, j + 1 == n0);
-          pf_commit(&kv_empty[v % SLOTS]);
+          free_tile(&kv_empty[v % SLOTS]);
           if (j + 2 < n0) {
             ready(kn);
             scores(0, buf, kn % SLOTS);
-            pf_commit(&kv_empty[kn % SLOTS]);
+            free_tile(&kv_empty[kn % SLOTS]);
           }
         }
       }
       used += 2 * n_max;
     }
-    pf_commit(&drained);
-    mbar_wait_bounded(&drained, 0);
+    if (lead) pf_commit(&drained);
+    mbar_wait_warp(&drained, 0);
     pf_fence_before();
   }
   }
