@@ -40,7 +40,7 @@ struct PfShape {
 };
 
 constexpr int PF_RECORDS = 640;            // records at most: four per SM, for 160
-constexpr int PF_LEAST = 4;                // tiles of a piece, at least
+constexpr int PF_LEAST = 16;               // tiles of a piece, at least
 
 struct PfParams {
   vp_paged c;
@@ -389,7 +389,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           for (int k = 0; k < 4; ++k) {
             const int b = s0 + 32 * k, fresh = base - b;
             uint32_t see = (pf_low(hi - b) & ~pf_low(lo - b)) | pf_low(min(a.sinks, hi) - b);
-            if (bits) see |= fresh >= 32 || fresh <= -32 ? 0u : fresh >= 0 ? bits << fresh : bits >> -fresh;
+            if (__any_sync(0xffffffffu, bits != 0)) see |= fresh >= 32 || fresh <= -32 ? 0u : fresh >= 0 ? bits << fresh : bits >> -fresh;
+            if (__all_sync(0xffffffffu, see == ~0u)) continue;
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (!((see >> e) & 1)) s[32 * k + e] = 0xff800000u;
@@ -436,8 +437,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           for (int k = 0; k < 32; ++k) {
             float2 x = make_float2(__uint_as_float(s[64 * b + 2 * k]), __uint_as_float(s[64 * b + 2 * k + 1]));
             x = pf_fma2(x, c2, u2);
-            x.x = pg_exp2(x.x);
-            x.y = pg_exp2(x.y);
+            x = make_float2(pg_exp2(x.x), pg_exp2(x.y));
             sum[k & 3] = pf_add2(sum[k & 3], x);
             w[k] = PgType<T>::down(x.x, x.y);
           }
@@ -532,18 +532,23 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
             __threadfence();
             __syncwarp();
             asm volatile("barrier.sync %0, 128;" ::"r"(1 + i) : "memory");
-            for (int x0 = row; x0 < n_rows * (HD / 4); x0 += 256) {
-              float4 acc[2] = {};
-              const int x1 = min(x0 + 128, n_rows * (HD / 4) - 1);
-              const int mm[2] = {i * 128 + x0 / (HD / 4), i * 128 + x1 / (HD / 4)}, d[2] = {x0 % (HD / 4) * 4, x1 % (HD / 4) * 4};
+            constexpr int W = 4;  // turns whose reads fly together
+            for (int x0 = row; x0 < n_rows * (HD / 4); x0 += 128 * W) {
+              float4 acc[W] = {};
+              int mm[W], d[W];
+#pragma unroll
+              for (int e = 0; e < W; ++e) {
+                const int x = min(x0 + 128 * e, n_rows * (HD / 4) - 1);
+                mm[e] = i * 128 + x / (HD / 4), d[e] = x % (HD / 4) * 4;
+              }
               for (int k0 = 0; k0 < live; k0 += 4) {
-                float4 v[2][4];
-                float w[2][4];
+                float4 v[W][4];
+                float w[W][4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                   const float* x = rec0 + (size_t)min(k0 + k, live - 1) * rec_floats;
 #pragma unroll
-                  for (int e = 0; e < 2; ++e) {
+                  for (int e = 0; e < W; ++e) {
                     v[e][k] = __ldcg(reinterpret_cast<const float4*>(x + (size_t)mm[e] * HD + d[e]));
                     w[e][k] = __ldcg(x + m_at + mm[e]);
                   }
@@ -551,14 +556,14 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
 #pragma unroll
-                  for (int e = 0; e < 2; ++e) {
+                  for (int e = 0; e < W; ++e) {
                     const float f1 = k0 + k < live ? w[e][k] : 0.f;
                     acc[e].x += v[e][k].x * f1, acc[e].y += v[e][k].y * f1, acc[e].z += v[e][k].z * f1, acc[e].w += v[e][k].w * f1;
                   }
               }
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                if (e && x0 + 128 >= n_rows * (HD / 4)) break;
+              for (int e = 0; e < W; ++e) {
+                if (x0 + 128 * e >= n_rows * (HD / 4)) break;
                 const int r2 = (f0 + mm[e]) / p.group, h2 = head * p.group + (f0 + mm[e]) % p.group;
                 uint2 v2;
                 v2.x = PgType<T>::down(acc[e].x, acc[e].y);
