@@ -15,6 +15,7 @@ table) is told by `check()`. The reference keeps one contiguous cache of one req
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import torch
@@ -26,6 +27,13 @@ TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 DEV_ERR_TIMEOUT, DEV_ERR_PAGE, DEV_ERR_SLOT = 4, 16, 32
 MAX_ROWS = 16
 WORK_ZEROED = 8192
+
+# The argument structs (VpPagedRows, VpPagedAttn) are packed in one go: a call of a few microseconds on the GPU should
+# not take longer to prepare, and setting two dozen ctypes fields takes 2 us.
+_ROWS = struct.Struct("8P8q6i")
+_ATTN = struct.Struct("8PQ6qf5i")
+assert _ROWS.size == ctypes.sizeof(VpPagedRows) and _ATTN.size <= ctypes.sizeof(VpPagedAttn)
+_I32, _F32 = torch.int32, torch.float32
 
 
 def rope_table(rows: int, rot_dim: int = 64, theta: float = 1e6, device=0) -> torch.Tensor:
@@ -47,9 +55,13 @@ def ancestor_masks(trees) -> torch.Tensor:
     return out
 
 
-def _index(t: torch.Tensor, what: str, shape, device) -> int:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous int32 tensor of shape {shape} on {device}")
+# the current stream's handle without a Stream object around it (2 us), where torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _index(t: torch.Tensor, what: str, shape, device: int) -> int:
+    if t.dtype is not _I32 or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 tensor of shape {shape} on cuda:{device}")
     return t.data_ptr()
 
 
@@ -85,11 +97,21 @@ class PagedLayer:
                           self.pages, n, width)
         self._r, self._a = VpPagedRows(), VpPagedAttn()
         self._cp, self._rp, self._ap = (ctypes.addressof(x) for x in (self._c, self._r, self._a))
+        self._index_of_device, self._need = self.device.index, {}
 
     def _stream(self) -> int:
-        if torch.cuda.current_device() != self.device.index:
+        if torch.cuda.current_device() != self._index_of_device:
             raise ValueError(f"the cache lives on {self.device}: make it the current device")
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return _raw_stream(self._index_of_device)
+
+    def _out(self, like: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
+        if out is None:
+            if like.dtype is self.dtype and like.is_contiguous():
+                return torch.empty_like(like)
+            return torch.empty(like.shape, dtype=self.dtype, device=self.device)
+        if out.shape != like.shape or out.dtype is not self.dtype or out.get_device() != self._index_of_device or out.stride(-1) != 1:
+            raise ValueError("out must have q's shape and the cache's type, elements of a head adjacent")
+        return out
 
     def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq: torch.Tensor, slot: torch.Tensor,
                pos: Optional[torch.Tensor], rope: Optional[torch.Tensor], interleaved: bool = False,
@@ -108,30 +130,27 @@ class PagedLayer:
         qs, ks, vs = q.stride(), k.stride(), v.stride()
         if qs[2] != 1 or ks[2] != 1 or vs[2] != 1:
             raise ValueError("the elements of a head must be adjacent")
-        if q.device != self.device or k.device != self.device or v.device != self.device:
-            raise ValueError(f"rows must be on {self.device}")
-        if out is None:
-            out = torch.empty((n, nq, hd), dtype=self.dtype, device=self.device)
-        elif out.shape != q.shape or out.dtype is not self.dtype or out.device != self.device or out.stride(2) != 1:
-            raise ValueError("out must have q's shape and the cache's type, elements of a head adjacent")
-        r, os = self._r, out.stride()
-        r.q, r.k, r.v, r.q_out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+        dev = self._index_of_device
+        if q.get_device() != dev or k.get_device() != dev or v.get_device() != dev:
+            raise ValueError(f"rows must be on cuda:{dev}")
         shape = (n,)
-        r.seq, r.slot = _index(seq, "seq", shape, self.device), _index(slot, "slot", shape, self.device)
+        places = _index(seq, "seq", shape, dev), _index(slot, "slot", shape, dev)
         if rope is None:
-            r.pos = r.rope = None
-            r.rope_rows = r.rot_dim = 0
+            places += None, None
+            turns = 0, 0
         else:
             if pos is None:
                 raise ValueError("a rotation needs pos")
-            if rope.dim() != 3 or rope.shape[2] != 2 or rope.dtype is not torch.float32 or not rope.is_contiguous() \
-                    or rope.device != self.device:
-                raise ValueError(f"rope must be a contiguous fp32 [positions][rot_dim / 2][2] tensor on {self.device}")
-            r.pos, r.rope = _index(pos, "pos", shape, self.device), rope.data_ptr()
-            r.rope_rows, r.rot_dim = rope.shape[0], 2 * rope.shape[1]
-        r.q_row, r.q_head, r.k_row, r.k_head, r.v_row, r.v_head = qs[0], qs[1], ks[0], ks[1], vs[0], vs[1]
-        r.out_row, r.out_head = os[0], os[1]
-        r.type, r.rows, r.n_q, r.interleaved = TYPES[q.dtype], n, nq, 1 if interleaved else 0
+            rs = rope.shape
+            if len(rs) != 3 or rs[2] != 2 or rope.dtype is not _F32 or not rope.is_contiguous() or rope.get_device() != dev:
+                raise ValueError(f"rope must be a contiguous fp32 [positions][rot_dim / 2][2] tensor on cuda:{dev}")
+            places += _index(pos, "pos", shape, dev), rope.data_ptr()
+            turns = rs[0], 2 * rs[1]
+        out = self._out(q, out)
+        os = out.stride()
+        _ROWS.pack_into(self._r, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *(x or 0 for x in places),
+                        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
+                        TYPES[q.dtype], n, nq, *turns, 1 if interleaved else 0)
         rc = self.lib.vp_paged_append(self._cp, self._rp, self._stream())
         if rc:
             check(rc, "vp_paged_append")
@@ -145,25 +164,16 @@ class PagedLayer:
         slot j (its own bit included; ancestor_masks), None for a causal chain. seqs: int32 [n], the requests' rows of the
         table (None: 0 .. n - 1). window > 0: a row sees the last `window` positions and the first `sinks`. Returns out
         like q, and with return_lse the log sum exp fp32 [n][rows][query heads]."""
-        one = q.dim() == 3
-        if not one and q.dim() != 4:
-            raise ValueError("q must be [n][rows][query heads][head_dim] or [n][query heads][head_dim]")
-        n, nq = q.shape[0], q.shape[-2]
-        rows = 1 if one else q.shape[1]
-        a = self._a
-        if mask is None:
-            a.mask = None
+        shape, qs = q.shape, q.stride()
+        if len(shape) == 4:
+            n, rows, nq, _ = shape
+        elif len(shape) == 3:
+            (n, nq, _), rows, qs = shape, 1, (qs[0], 0, qs[1], qs[2])
         else:
-            a.mask = _index(mask, "mask", (n, rows), self.device)
-        out, lse = self._attend(q, n, rows, nq, lens, seqs, window, sinks, scale, out, return_lse)
-        qs, os = q.stride(), out.stride()
-        a.q_seq, a.q_head, a.out_seq, a.out_head = qs[0], qs[-2], os[0], os[-2]
-        a.q_row, a.out_row = (0, 0) if one else (qs[1], os[1])
-        a.q_start = None
-        rc = self.lib.vp_paged_decode(self._cp, self._ap, self._stream())
-        if rc:
-            check(rc, "vp_paged_decode")
-        return (out, lse) if return_lse else out
+            raise ValueError("q must be [n][rows][query heads][head_dim] or [n][query heads][head_dim]")
+        masks = 0 if mask is None else _index(mask, "mask", (n, rows), self._index_of_device)
+        return self._attend(self.lib.vp_paged_decode, "vp_paged_decode", q, qs, n, rows, nq, lens, seqs, masks, 0, window, sinks,
+                            scale, out, return_lse)
 
     def prefill(self, q: torch.Tensor, q_start: torch.Tensor, lens: torch.Tensor, seqs: Optional[torch.Tensor] = None,
                 window: int = 0, sinks: int = 0, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
@@ -172,44 +182,39 @@ class PagedLayer:
         slots of lens[i] (already appended). Other arguments and results as in decode."""
         if q.dim() != 3:
             raise ValueError("q must be [rows][query heads][head_dim]")
-        n, a = lens.shape[0], self._a
-        a.q_start = _index(q_start, "q_start", (n + 1,), self.device)
-        out, lse = self._attend(q, n, q.shape[0], q.shape[1], lens, seqs, window, sinks, scale, out, return_lse)
-        qs, os = q.stride(), out.stride()
-        a.q_seq = a.out_seq = 0
-        a.q_row, a.q_head, a.out_row, a.out_head = qs[0], qs[1], os[0], os[1]
-        a.mask = None
-        rc = self.lib.vp_paged_prefill(self._cp, self._ap, self._stream())
-        if rc:
-            check(rc, "vp_paged_prefill")
-        return (out, lse) if return_lse else out
+        n, qs = lens.shape[0], q.stride()
+        starts = _index(q_start, "q_start", (n + 1,), self._index_of_device)
+        return self._attend(self.lib.vp_paged_prefill, "vp_paged_prefill", q, (0, *qs), n, q.shape[0], q.shape[1], lens, seqs, 0,
+                            starts, window, sinks, scale, out, return_lse)
 
-    def _attend(self, q, n, rows, nq, lens, seqs, window, sinks, scale, out, return_lse):
-        if q.shape[-1] != self.head_dim or q.dtype is not self.dtype or q.device != self.device or q.stride(-1) != 1:
+    def _attend(self, call, name, q, qs, n, rows, nq, lens, seqs, masks, starts, window, sinks, scale, out, return_lse):
+        dev = self._index_of_device
+        if q.shape[-1] != self.head_dim or q.dtype is not self.dtype or q.get_device() != dev or qs[3] != 1:
             raise ValueError(f"q must be {self.dtype} heads of {self.head_dim} on {self.device}, elements of a head adjacent")
-        a = self._a
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        elif out.shape != q.shape or out.dtype is not q.dtype or out.device != self.device or out.stride(-1) != 1:
-            raise ValueError("out must have q's shape and type, elements of a head adjacent")
-        lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=self.device) if return_lse else None
-        a.q, a.out, a.lse = q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None
-        a.lens = _index(lens, "lens", (n,), self.device)
-        if seqs is None:
-            if n > self.table.shape[0]:
-                raise ValueError(f"{n} requests, and a table of {self.table.shape[0]}")
-            a.seqs = None
-        else:
-            a.seqs = _index(seqs, "seqs", (n,), self.device)
-        need = self.lib.vp_paged_work_bytes(self.head_dim, nq, self.n_kv, rows)
+        places = _index(lens, "lens", (n,), dev)
+        if seqs is not None:
+            seqs = _index(seqs, "seqs", (n,), dev)
+        elif n > self._c.n_seqs:
+            raise ValueError(f"{n} requests, and a table of {self._c.n_seqs}")
+        out = self._out(q, out)
+        os = out.stride()
+        if len(os) == 3:
+            os = (0, *os) if starts else (os[0], 0, *os[1:])
+        lse = torch.empty(q.shape[:-1], dtype=_F32, device=self.device) if return_lse else None
+        need = self._need.get((nq, rows))
+        if need is None:
+            need = self._need[nq, rows] = self.lib.vp_paged_work_bytes(self.head_dim, nq, self.n_kv, rows)
         work = self._work[0]
         if work is None or work.numel() < need:
             work = self._work[0] = torch.empty(max(need, WORK_ZEROED), dtype=torch.uint8, device=self.device)
             work[:WORK_ZEROED].zero_()
-        a.work, a.work_bytes = work.data_ptr(), work.numel()
-        a.scale = self.head_dim ** -0.5 if scale is None else scale
-        a.n, a.rows, a.n_q, a.window, a.sinks = n, rows, nq, window, sinks
-        return out, lse
+        _ATTN.pack_into(self._a, 0, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, places, seqs or 0, masks, starts,
+                        work.data_ptr(), work.numel(), qs[0], qs[1], qs[2], os[0], os[1], os[2],
+                        self.head_dim ** -0.5 if scale is None else scale, n, rows, nq, window, sinks)
+        rc = call(self._cp, self._ap, self._stream())
+        if rc:
+            check(rc, name)
+        return (out, lse) if return_lse else out
 
     def check(self) -> None:
         """Raises VpError if a call met a page or slot outside the table, or gave up a wait, since the last check();
