@@ -13,7 +13,7 @@
 //  * eight consumer warps take turns over the tiles. Each has two stages of its own and refills a
 //    stage itself (TMA boxes of one page each) once it has computed on it (mma.sync), so the warps never
 //    wait for one another;
-//  * three joiner warps bring the queries of the next pair, and at the end of a pair's run add up the
+//  * four joiner warps bring the queries of the next pair, and at the end of a pair's run add up the
 //    warps' records while the warps are on the next pair. A pair that several CTAs share leaves records
 //    in the work buffer; the CTA that finishes last (a counter per first CTA, back at zero afterwards)
 //    joins them in the order of the slots, so results do not depend on which CTA that is.
@@ -23,7 +23,7 @@
 namespace vp {
 
 constexpr int DC_WARPS = 8;                         // consumer warps
-constexpr int DC_JOINERS = 96;                      // threads
+constexpr int DC_JOINERS = 128;                     // threads
 constexpr int DC_THREADS = DC_WARPS * 32 + DC_JOINERS;
 constexpr int DC_ROWS = 16;                         // packed query rows of a pair
 constexpr int DC_TILE = 4096;                       // bytes of K (and of V) per tile
@@ -98,41 +98,52 @@ __device__ __forceinline__ uint64_t dc_seen(int s0, int base, int lo, int sinks,
 constexpr int DC_FILLED = 2, DC_FREE = 3;
 __device__ __forceinline__ void dc_sync(int bar) {
   __syncwarp();
-  asm volatile("barrier.sync %0, 352;" ::"r"(bar) : "memory");
+  asm volatile("barrier.sync %0, 384;" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void dc_arrive(int bar) {
   __threadfence_block();
   __syncwarp();
-  asm volatile("barrier.arrive %0, 352;" ::"r"(bar) : "memory");
+  asm volatile("barrier.arrive %0, 384;" ::"r"(bar) : "memory");
 }
-static_assert(DC_THREADS == 352, "barrier counts");
+static_assert(DC_THREADS == 384, "barrier counts");
 
-// A walk over the CTA's tiles [t, t1): the request and head that tile t belongs to.
+// A walk over the CTA's tiles: the request and head that tile t belongs to.
 template <int TS>
 struct DcWalk {
   const DcParams& p;
   const int* lens_s;
-  int seq, seq_at, t, t1;  // seq_at: number of seq's first tile
+  int seq, head, u, t, t1;  // tile t is tile u of this head
   DcSpan sp;
-  int head, u;             // tile t is tile u of this head
+  // at: the number of seq's first tile
   __device__ __forceinline__ DcWalk(const DcParams& p_, const int* l, int s, int at, int t_, int t1_)
-      : p(p_), lens_s(l), seq(s), seq_at(at), t(t_), t1(t1_) {
+      : p(p_), lens_s(l), seq(s), t(at), t1(t1_) {
     span();
+    const int skip = t_ - at;  // seq has the CTA's first tile, so few requests are passed over
+    head = 0;
+    u = 0;
+    if (skip >= sp.tiles && t_ < t1) {
+      head = min(skip / sp.tiles, p.c.n_kv - 1);
+      t += head * sp.tiles;
+    }
+    advance(t_ - t);
   }
   __device__ __forceinline__ void span() {
     const int len = seq < DC_LENS ? lens_s[seq] : pg_seq(p.c, p.a.seqs, p.a.lens, seq).len;
     sp = dc_span<TS>(len, p.a.rows, p.a.window, p.a.sinks);
   }
-  __device__ __forceinline__ bool find() {
-    if (t >= t1) return false;
-    while (t >= seq_at + sp.tiles * p.c.n_kv) {
-      seq_at += sp.tiles * p.c.n_kv;
-      ++seq;
-      span();
+  __device__ __forceinline__ bool more() const { return t < t1; }
+  __device__ __forceinline__ void advance(int k) {
+    t += k;
+    if (t >= t1) return;
+    u += k;
+    while (u >= sp.tiles) {
+      u -= sp.tiles;
+      if (++head == p.c.n_kv) {
+        head = 0;
+        ++seq;
+        span();
+      }
     }
-    head = (t - seq_at) / sp.tiles;
-    u = t - seq_at - head * sp.tiles;
-    return true;
   }
   __device__ __forceinline__ int run() const { return min(sp.tiles - u, t1 - t); }  // tiles of this head from t on
   __device__ __forceinline__ int slot(int v) const { return (v < sp.ns ? v : sp.ws + v - sp.ns) * TS; }
@@ -227,75 +238,92 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
     const int g = lane >> 2, q4 = lane & 3;
     const float cexp = a.scale * 1.4426950408889634f;
     const uint32_t stage0 = smem_u32(ring) + warp * DC_STAGES * 2 * DC_TILE;
-    // loads run ahead of the computation: `ahead` stands at the tile to fetch next, lane b < boxes has
-    // the page of its box b already
+    // Loads run ahead of the computation. A tile is looked up (lane b < boxes: the page of box b) well
+    // before it is fetched, so that the table's answer is there.
     const int box = min(c.page_size, TS), boxes = TS / box;
-    DcWalk<TS> ahead(p, lens_s, first_seq, first_tile, t0 + warp, t1);
-    int page = c.n_pages, slot = 0;
-    auto look = [&] {  // page of this lane's box of the tile at `ahead`; one that nobody sees fills zeros
-      page = c.n_pages;
-      if (!ahead.find()) return;
-      slot = ahead.slot(ahead.u) + lane * box;
-      if (lane < boxes && slot < ahead.sp.len && (slot + box > ahead.sp.lo || slot < a.sinks)) {
-        const int s = a.seqs ? a.seqs[ahead.seq] : ahead.seq;  // a request outside the table has no slots
-        page = c.table[s * c.table_stride + (slot >> p.page_shift)];
-      }
+    struct Tile {
+      int page, slot, head;
+      bool any, seen;
     };
-    auto fetch = [&](int st) {  // the tile at `ahead` into stage st
-      if (ahead.t >= t1) return;
+    DcWalk<TS> ahead(p, lens_s, first_seq, first_tile, t0 + warp, t1);
+    auto look = [&] {
+      Tile x;
+      x.any = ahead.more();
+      x.page = c.n_pages;  // a box that nobody sees fills zeros
+      x.slot = ahead.slot(ahead.u) + lane * box;
+      x.head = ahead.head;
+      x.seen = x.any && lane < boxes && x.slot < ahead.sp.len && (x.slot + box > ahead.sp.lo || x.slot < a.sinks);
+      if (x.seen) {
+        const int s = a.seqs ? a.seqs[ahead.seq] : ahead.seq;  // a request outside the table has no slots
+        x.page = c.table[s * c.table_stride + (x.slot >> p.page_shift)];
+      }
+      ahead.advance(DC_WARPS);
+      return x;
+    };
+    auto fetch = [&](const Tile& x, int st) {
+      if (!x.any) return;
       if (lane == 0) mbar_arrive_expect_tx(&full[warp][st], 2 * DC_TILE);
       __syncwarp();
       if (lane < boxes) {
-        if (page < 0 || page > c.n_pages || (page == c.n_pages && slot < ahead.sp.len && (slot + box > ahead.sp.lo || slot < a.sinks))) {
+        int page = x.page;
+        if (x.seen && (page < 0 || page >= c.n_pages)) {
           pg_status(c.status, VP_DEV_ERR_PAGE);
           page = c.n_pages;
         }
         unsigned char* dst = ring + (size_t)((warp * DC_STAGES + st) * 2) * DC_TILE + lane * box * 128;
-        pg_box5(dst, &mk, slot & (c.page_size - 1), ahead.head, page, &full[warp][st]);
-        pg_box5(dst + DC_TILE, &mv, slot & (c.page_size - 1), ahead.head, page, &full[warp][st]);
+        pg_box5(dst, &mk, x.slot & (c.page_size - 1), x.head, page, &full[warp][st]);
+        pg_box5(dst + DC_TILE, &mv, x.slot & (c.page_size - 1), x.head, page, &full[warp][st]);
       }
-      ahead.t += DC_WARPS;
     };
-    look();
-#pragma unroll
-    for (int st = 0; st < DC_STAGES; ++st) {
-      fetch(st);
-      look();
+    Tile coming;
+    {
+      const Tile x = look(), y = look();
+      fetch(x, 0);
+      fetch(y, 1);
+      coming = look();
     }
+    static_assert(DC_STAGES == 2, "first tiles");
+    const int row_of[2] = {g / p.group, (g + 8) / p.group};
+    const bool plain = rows == 1 && !a.mask;  // one row that sees all up to its own slot
     uint32_t k_th = 0;  // tiles computed
     int next = t0 + warp;
     DcWalk<TS> w(p, lens_s, first_seq, first_tile, t0, t1);
-    for (int r = 0; w.find(); ++r) {
+    for (int r = 0; w.more(); ++r) {
       const DcSpan& sp = w.sp;
       const int n = w.run(), seq = w.seq;
       // masks of the request's rows (lane i: row i); this thread's two rows, and their union
-      uint32_t anc = 0;
-      if (lane < rows)
-        anc = a.mask ? (uint32_t)a.mask[(long long)seq * rows + lane] & ((1u << rows) - 1) : (2u << lane) - 1;
-      uint32_t bits[2];
+      uint32_t bits[2] = {1, 1}, any = 1;
       int lo[2];  // first old slot beside the sinks that the row sees
+      int least = 1;
       bool there[2];
+      if (plain) {
+        lo[0] = lo[1] = a.window ? sp.base + 1 - a.window : 0;
+      } else {
+        uint32_t anc = 0;
+        if (lane < rows)
+          anc = a.mask ? (uint32_t)a.mask[(long long)seq * rows + lane] & ((1u << rows) - 1) : (2u << lane) - 1;
+        any = __reduce_or_sync(0xffffffffu, anc);
+        least = __reduce_min_sync(0xffffffffu, lane < rows ? __popc(anc) : 32);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int m = g + 8 * h, row = m / p.group;
-        there[h] = m < p.M && sp.base + row >= 0;
-        bits[h] = __shfl_sync(0xffffffffu, anc, min(row, 31));
-        lo[h] = a.window ? sp.base + __popc(bits[h]) - a.window : 0;
-      }
-      const uint32_t any = __reduce_or_sync(0xffffffffu, anc);
-      const int least = __reduce_min_sync(0xffffffffu, lane < rows ? __popc(anc) : 32);
-      const int first_seen = a.window ? sp.base + least - a.window : 0;  // beside the sinks, by any row
-      if (a.window) {  // new slots that have left a row's window
-        uint32_t keep[2] = {0, 0};
-        for (int j = 0; j < rows; ++j) {
-          const int place = sp.base + __popc(__shfl_sync(0xffffffffu, anc, j)) - 1;
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (place >= lo[h] || place < a.sinks) keep[h] |= 1u << j;
+        for (int h = 0; h < 2; ++h) {
+          bits[h] = __shfl_sync(0xffffffffu, anc, min(row_of[h], 31));
+          lo[h] = a.window ? sp.base + __popc(bits[h]) - a.window : 0;
         }
-        bits[0] &= keep[0];
-        bits[1] &= keep[1];
+        if (a.window) {  // new slots that have left a row's window
+          uint32_t keep[2] = {0, 0};
+          for (int j = 0; j < rows; ++j) {
+            const int place = sp.base + __popc(__shfl_sync(0xffffffffu, anc, j)) - 1;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (place >= lo[h] || place < a.sinks) keep[h] |= 1u << j;
+          }
+          bits[0] &= keep[0];
+          bits[1] &= keep[1];
+        }
       }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) there[h] = g + 8 * h < p.M && sp.base + row_of[h] >= 0;
+      const int first_seen = a.window ? sp.base + least - a.window : 0;  // beside the sinks, by any row
       uint32_t qf[KS][4];
       wait(&q_full[r & 1], (r >> 1) & 1);
       {
@@ -393,8 +421,8 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
           }
         }
         __syncwarp();
-        fetch(st);
-        look();
+        fetch(coming, st);
+        coming = look();
       }
       if (r > 0) dc_sync(DC_FREE);
 #pragma unroll
@@ -410,7 +438,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
         }
       }
       dc_arrive(DC_FILLED);
-      w.t += n;
+      w.advance(n);
     }
     return;
   }
@@ -438,14 +466,13 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
     if (a.lse && d == 0) a.lse[((long long)seq * rows + row) * a.n_q + h] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
   };
   DcWalk<TS> w(p, lens_s, first_seq, first_tile, t0, t1);
-  w.find();
   queries(w.seq, w.head, 0);
   bool more = true;
   for (int r = 0; more; ++r) {
     const int seq = w.seq, head = w.head, u0 = w.u, n = w.run(), tiles = w.sp.tiles, pair_at = w.t - w.u;
     const bool alone = n == tiles;
-    w.t += n;
-    more = w.find();
+    w.advance(n);
+    more = w.more();
     if (more) queries(w.seq, w.head, r + 1);  // the warps are done with the queries of run r - 1
     float* rec = p.rec + (size_t)(u0 == 0 ? 2 * cta + 1 : 2 * cta) * rec_floats;
     dc_sync(DC_FILLED);
@@ -484,10 +511,10 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
     const int c0 = share.owner(pair_at), c1 = share.owner(pair_at + tiles - 1);
     __threadfence();
     __syncwarp();
-    asm volatile("barrier.sync 1, 96;" ::: "memory");
+    asm volatile("barrier.sync 1, 128;" ::: "memory");
     if (jt == 0) last_flag = atomicAdd(&p.tickets[c0], 1u) == (unsigned)(c1 - c0);
     __syncwarp();
-    asm volatile("barrier.sync 1, 96;" ::: "memory");
+    asm volatile("barrier.sync 1, 128;" ::: "memory");
     if (!last_flag) continue;
     __threadfence();
     for (int it = jt; it < p.M * (HD / 4); it += DC_JOINERS) {
