@@ -8,8 +8,10 @@
 // Bound: the tensor cores at head_dim 128, the exponentials (16 a clock and SM against 4,096 products)
 // at 64. The query rows of one cache head are packed as row G + g, 256 of them to a block as two
 // tiles of 128, so K and V are read once for 256 rows and the heads of a group share them. Tensor
-// memory holds S of both tiles (128 columns each, the weights P written over them as pairs) and both
-// o (head_dim columns each). One warp brings K and V tiles (TMA boxes of one page each), one thread
+// memory holds three buffers of S (two at head_dim 128; 128 columns each, the weights P written over
+// them as pairs) and both o (head_dim columns each). A unit is a row tile with a tile of slots; units go
+// round the buffers in order, first row tile, second row tile, next slots, so with three buffers the
+// next S of a row tile is there before its present weights are. One warp brings K and V tiles (TMA boxes of one page each), one thread
 // issues the products, and two warpgroups, one tile each and one row a thread, do the softmax: while
 // one of them works on its tile, the tensor cores work on the other's.
 //
@@ -36,6 +38,7 @@ struct PfShape {
   static constexpr int PANELS = HD / 64;                        // 128-byte wide columns of a tile
   static constexpr int TILE = PF_TS * HD * 2;                   // bytes of a K, V or Q tile
   static constexpr int SLOTS = HD == 64 ? 8 : 4;                // ring of K and V tiles
+  static constexpr int BUFS = HD == 64 ? 3 : 2;                 // buffers of S in tensor memory, beside both o
   static constexpr size_t SMEM = 1024 + 2 * TILE + (size_t)SLOTS * TILE;
 };
 
@@ -48,6 +51,8 @@ struct PfParams {
   float* rec;         // records of block_rows rows, one per piece of a cut block
   unsigned* tickets;  // [records][2 row tiles], then the scheduler's two
   int group, block_rows, sms, most;  // most: pieces that a call can have
+  int rows;                          // packed rows of a block: 256, or 128 where there are few blocks
+  int cuts;                          // whether the table's longest request may be cut
 };
 
 __device__ __forceinline__ uint64_t pf_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
@@ -132,7 +137,7 @@ __device__ __forceinline__ PfSpan pf_span(int lo, int end, int sinks) {
 }
 // The request's part of a call: its new rows, and the slots that packed rows [f, g) of it see.
 struct PfSeq {
-  int first, n_new, len, base, blocks, least;  // least: fewest mask bits of a row (trees)
+  int first, n_new, len, base, blocks, least, row;  // least: fewest mask bits of a row (trees); row: of the table
   int lo, end;                                 // of the last range asked for
   __device__ __forceinline__ void see(const PfParams& p, int f, int g) {
     const bool tree = !p.a.q_start;
@@ -141,7 +146,7 @@ struct PfSeq {
     lo = p.a.window ? max(0, p_lo - p.a.window + 1) : 0;
   }
   __device__ __forceinline__ int last_tiles(const PfParams& p) {  // of the last block, which has the most
-    see(p, (blocks - 1) * PF_ROWS, n_new * p.group);
+    see(p, (blocks - 1) * p.rows, n_new * p.group);
     return pf_span(lo, end, p.a.sinks).tiles;
   }
 };
@@ -161,15 +166,18 @@ __device__ __forceinline__ PfSeq pf_seq(const PfParams& p, int i) {
       s.least = min(s.least, __popc((uint32_t)p.a.mask[(long long)i * p.a.rows + r] & ((1u << p.a.rows) - 1)));
   }
   s.len = pg_seq(p.c, p.a.seqs, p.a.lens, i).len;
+  s.row = p.a.seqs ? p.a.seqs[i] : i;
   s.base = s.len - s.n_new;
-  s.blocks = (int)(((unsigned)s.n_new * (unsigned)p.group + PF_ROWS - 1) / PF_ROWS);
+  s.blocks = (int)(((unsigned)s.n_new * (unsigned)p.group + p.rows - 1) / p.rows);
   return s;
 }
+// Cuts of each of a request's blocks: none as long as the largest is not half as much again as the share.
+__device__ __forceinline__ int pf_cuts(int last, int share) { return 2 * last > 3 * share ? (last + share - 1) / share : 1; }
 __device__ __forceinline__ uint32_t pf_low(int x) { return x <= 0 ? 0u : x >= 32 ? ~0u : (1u << x) - 1; }
 
 // A piece as the scheduler hands it to the other roles.
 struct PfPiece {
-  int seq, head, f0, f_end, first, base, cut, cuts, live, record0, j0, n0, n1, see_lo, see_end, ns, ws;  // seq < 0: no more
+  int seq, row, head, f0, f_end, first, base, cut, cuts, live, record0, j0, n0, n1, see_lo, see_end, ns, ws;  // seq < 0: no more
   uint32_t any;                 // trees: new slots that a row sees
   uint32_t masks[PG_MAX_ROWS];  // bits 0-15: new slots that the row sees, 16-20: the row's mask bits
 };
@@ -187,20 +195,25 @@ __device__ __forceinline__ float2 pf_add2(float2 a, float2 b) {
   return *reinterpret_cast<float2*>(&d);
 }
 
+// Number of the unit (row tile i, j-th tile of slots) in its piece; the first row tile has n0 tiles, the second as
+// many or more.
+__device__ __forceinline__ int pf_unit(bool two, int i, int j, int n0) { return !two ? j : j < n0 ? 2 * j + i : n0 + j; }
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(PF_THREADS, 1)
     k_paged_tiles(const __grid_constant__ PfParams p, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
   using Sh = PfShape<HD>;
-  constexpr int TILE = Sh::TILE, SLOTS = Sh::SLOTS, PANELS = Sh::PANELS, PANEL = PF_TS * 128;
+  constexpr int TILE = Sh::TILE, SLOTS = Sh::SLOTS, PANELS = Sh::PANELS, PANEL = PF_TS * 128, BUFS = Sh::BUFS;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* qs = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   unsigned char* ring = qs + 2 * TILE;
-  // s_full: S of a buffer is there; p_full: its weights are; o_full: a product into o is done; o_last: the piece's last one is
-  __shared__ uint64_t kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_full[2], o_full[2], o_last[2], q_full, edge, drained, info_full[2], info_empty[2];
+  // of a buffer: its S is there, its weights are, its product into o is done; of a row tile: the piece's last product is
+  __shared__ uint64_t kv_full[SLOTS], kv_empty[SLOTS], s_full[BUFS], p_full[BUFS], o_done[BUFS], o_last[2], q_full, edge, drained, info_full[2], info_empty[2];
   __shared__ uint32_t tmem_base;
   __shared__ long long tile_sums[PF_THREADS / 32];
   __shared__ int sums[PF_THREADS / 32][2], starts[PF_THREADS], rec_starts[PF_THREADS], dead, last_s[2];
   __shared__ PfPiece info[2];
+  __shared__ PfSeq seqs_s[PF_THREADS];  // the requests, where there are no more than threads
 
   const vp_paged& c = p.c;
   const vp_paged_attn& a = p.a;
@@ -213,10 +226,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < BUFS; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
-      mbar_init(&o_full[i], 1);
+      mbar_init(&o_done[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&o_last[i], 1);
       mbar_init(&info_full[i], 1);
       mbar_init(&info_empty[i], 10);  // the softmax warps, the producer, the issuer
@@ -238,40 +253,43 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait();
-  // Pieces of all requests, in two sums: all tiles (which give the share of a CTA); pieces and records.
+  // Pieces of all requests, in two sums: all tiles, which give the share of a CTA (left out where no
+  // request can be long enough to be cut); pieces and records.
   const int chunk = (a.n + PF_THREADS - 1) / PF_THREADS, i0 = min(a.n, tid * chunk), i1 = min(a.n, i0 + chunk);
   long long tiles = 0;
   int one_blocks = 0, one_last = 0;  // of the thread's last request
   for (int i = i0; i < i1; ++i) {
     PfSeq s = pf_seq(p, i);
+    if (chunk == 1) seqs_s[i] = s;
     one_blocks = s.blocks;
-    if (!s.blocks) continue;
+    if (!s.blocks || !p.cuts) continue;
     one_last = s.last_tiles(p);
-    s.see(p, 0, min(PF_ROWS, s.n_new * p.group));
+    s.see(p, 0, min(p.rows, s.n_new * p.group));
     tiles += (long long)s.blocks * (one_last + pf_span(s.lo, s.end, a.sinks).tiles);
   }
+  int share = 1 << 30;
+  if (p.cuts) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
-  if (lane == 0) tile_sums[warp] = tiles;
-  pf_fence_before();
-  cta_sync();
-  pf_fence_after();
-  long long all = 0;
+    for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    if (lane == 0) tile_sums[warp] = tiles;
+    cta_sync();
+    long long all = 0;
 #pragma unroll
-  for (int w = 0; w < PF_THREADS / 32; ++w) all += tile_sums[w];
-  // the mean of its first and last block stands for a request's blocks: `all` is twice the tiles per
-  // cache head. Rounded up by two so that the float division cannot make it less than an even half.
-  const int share = max(PF_LEAST, (int)fminf((float)all * c.n_kv / (2 * p.sms), 1e9f) + 2);
+    for (int w = 0; w < PF_THREADS / 32; ++w) all += tile_sums[w];
+    // the mean of its first and last block stands for a request's blocks: `all` is twice the tiles per
+    // cache head. Rounded up by two so that the float division cannot make it less than an even half.
+    share = max(PF_LEAST, (int)fminf((float)all * c.n_kv / (2 * p.sms), 1e8f) + 2);
+  }
   int pieces = 0, records = 0;
   for (int i = i0; i < i1; ++i) {
     int blocks = one_blocks, last = one_last;
     if (chunk > 1) {
       PfSeq s = pf_seq(p, i);
       blocks = s.blocks;
-      if (blocks) last = s.last_tiles(p);
+      if (blocks && p.cuts) last = s.last_tiles(p);
     }
     if (!blocks) continue;
-    const int n = max(1, (last + share - 1) / share);
+    const int n = p.cuts ? pf_cuts(last, share) : 1;
     pieces += blocks * n * c.n_kv;
     if (n > 1) records += blocks * n * c.n_kv;
   }
@@ -291,7 +309,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   }
   starts[tid] = at0;
   rec_starts[tid] = at_r0;
+  pf_fence_before();
   cta_sync();
+  pf_fence_after();
   const uint32_t tmem = tmem_base;
 
   // Waits of a whole warp. After one that ran out none waits any more, and the call ends
@@ -312,11 +332,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     // ---- softmax: warpgroup i has row tile i, a thread row f ----
     const int i = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 lanes of tensor memory
-    const uint32_t to = tmem + lanes + 256 + i * HD;
+    const uint32_t to = tmem + lanes + BUFS * 128 + i * HD;
     const float cexp = a.scale * 1.4426950408889634f;
     const size_t rec_floats = pg_record(p.block_rows, HD);
     const int m_at = p.block_rows * HD, l_at = m_at + p.block_rows;
-    uint32_t n_s[2] = {0, 0}, n_o = 0, n_last = 0;  // phases of s_full and p_full, of o_full, of o_last so far
+    uint32_t units = 0, n_last = 0;  // units of all pieces so far, phases of o_last so far
     // Queries of piece r on their way into the row tile's buffer, once the last product that reads it is done.
     auto fetch = [&](int r) {
       wait_warp(&info_full[r & 1], (r >> 1) & 1);
@@ -338,7 +358,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       const PfPiece& in = info[r & 1];
       const int seq = in.seq, f = in.f0 + tid, f_end = in.f_end, f0 = in.f0, head = in.head, first = in.first, base = in.base;
       if (seq < 0 || is_dead()) break;
-      const bool two = in.n1 > 0 || f_end > f0 + 128;  // two row tiles; else the first has both buffers of S
+      const bool two = f_end > f0 + 128;  // row tiles
       const int n_t = i ? in.n1 : in.n0, j0 = in.j0, cuts = in.cuts, cut = in.cut, live = in.live, record0 = in.record0;
       const int n0 = in.n0, n1 = in.n1;
       PfSpan sp;
@@ -371,10 +391,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       const int lo_all = !a.window ? 0 : tree ? base + a.rows - a.window : base + (f0 + i * 128 + 127) / p.group - a.window + 1;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n_t; ++j) {
-        const int s0 = sp.at(j0 + j) * PF_TS, buf = two ? i : j & 1;
+        const int s0 = sp.at(j0 + j) * PF_TS;
+        const uint32_t u = units + pf_unit(two, i, j, n0), buf = u % BUFS;
         const uint32_t ts = tmem + lanes + buf * 128;
-        wait_warp(&s_full[buf], n_s[buf] & 1);
-        ++n_s[buf];
+        wait_warp(&s_full[buf], (u / BUFS) & 1);
         pf_fence_after();
         uint32_t s[128];
 #pragma unroll
@@ -411,8 +431,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           l *= fac;
           m = mn;
           if (j > 0) {
-            if (!two) {  // with two buffers of S the last product into o may be under way
-              wait_warp(&o_full[i], (n_o + j - 1) & 1);
+            const uint32_t before = units + pf_unit(two, i, j - 1, n0);
+            if (u - before < BUFS) {  // the last product into o may be under way: this S did not wait for it
+              wait_warp(&o_done[before % BUFS], (before / BUFS) & 1);
               pf_fence_after();
             }
 #pragma unroll 1
@@ -455,13 +476,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         ++n_last;
         pf_fence_after();
       }
-      n_o += n_t;
-      if (two) {  // the other warpgroup's buffer
-        n_s[1 - i] += i ? n0 : n1;
-      } else if (i == 1) {  // both
-        n_s[0] += (n0 + 1) / 2;
-        n_s[1] += n0 / 2;
-      }
+      units += two ? n0 + n1 : n0;
       T* out = static_cast<T*>(a.out) + seq * a.out_seq + (long long)(first + qrow) * a.out_row + h * a.out_head;
       float* lse = a.lse ? a.lse + ((tree ? (long long)seq * a.rows : (long long)first) + qrow) * a.n_q + h : nullptr;
       float* rec = p.rec + (size_t)(record0 + cut) * rec_floats;
@@ -614,11 +629,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       }
       owner -= 1;
       int at = starts[owner], at_r = rec_starts[owner], seq = owner * chunk;
-      PfSeq s = pf_seq(p, seq);
+      PfSeq s = chunk == 1 ? seqs_s[seq] : pf_seq(p, seq);
       int cuts = 1;
       for (;; s = pf_seq(p, ++seq)) {
         if (s.blocks) {
-          cuts = max(1, (s.last_tiles(p) + share - 1) / share);
+          cuts = p.cuts ? pf_cuts(s.last_tiles(p), share) : 1;
           const int k = s.blocks * cuts * c.n_kv;
           if (piece < at + k) break;
           at += k;
@@ -627,7 +642,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       }
       // pieces of a request: block, then head, then cut
       const int mine = piece - at, pair = mine / cuts, cut = mine - pair * cuts, block = pair / c.n_kv;
-      const int f0 = block * PF_ROWS, f_end = min(s.n_new * p.group, f0 + PF_ROWS);
+      const int f0 = block * p.rows, f_end = min(s.n_new * p.group, f0 + p.rows);
       s.see(p, f0, f_end);
       const PfSpan sp = pf_span(s.lo, s.end, a.sinks);
       const int live = max(1, min(cuts, sp.tiles)), per = sp.tiles / live, odd = sp.tiles % live;
@@ -647,7 +662,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         if (lane == 0) in.any = any;
       }
       if (lane == 0) {
-        in.seq = seq, in.head = pair - block * c.n_kv, in.f0 = f0, in.f_end = f_end, in.first = s.first, in.base = s.base;
+        in.seq = seq, in.row = s.row, in.head = pair - block * c.n_kv, in.f0 = f0, in.f_end = f_end, in.first = s.first, in.base = s.base;
         in.cut = cut, in.cuts = cuts, in.live = live, in.record0 = at_r + mine - cut;
         in.j0 = j0, in.n0 = max(0, min(j1, sp.upto(stop0)) - j0), in.n1 = f_end > f0 + 128 ? j1 - j0 : 0;
         in.see_lo = s.lo, in.see_end = s.end, in.ns = sp.ns, in.ws = sp.ws;
@@ -663,7 +678,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     for (int r = 0;; ++r) {
       wait_warp(&info_full[r & 1], (r >> 1) & 1);
       const PfPiece& in = info[r & 1];
-      const int seq = in.seq, head = in.head, j0 = in.j0, n_max = max(in.n0, in.n1), see_lo = in.see_lo, see_end = in.see_end, base = in.base;
+      const int seq = in.seq, table_row = in.row, head = in.head, j0 = in.j0, n_max = max(in.n0, in.n1), see_lo = in.see_lo, see_end = in.see_end, base = in.base;
       const uint32_t any = in.any;
       PfSpan sp;
       sp.ns = in.ns;
@@ -671,7 +686,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       if (seq < 0 || is_dead()) break;
       __syncwarp();
       if (lane == 0) pg_arrive(&info_empty[r & 1]);
-      const int32_t* pages = pg_seq(c, a.seqs, a.lens, seq).pages;
+      // a request outside the table has no slots, and no page is looked up for it
+      const int32_t* pages = c.table + table_row * c.table_stride;
       for (int j = 0; j < n_max; ++j) {
         const int s0 = sp.at(j0 + j) * PF_TS, slot = s0 + lane * box;
         int page = c.n_pages;  // a box that nobody sees fills zeros
@@ -746,24 +762,19 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       const uint64_t vd = pf_desc(rb + st * TILE, PANEL, 1024);
       if (!lead) return;
 #pragma unroll
-      for (int k = 0; k < PF_TS / 16; ++k) pf_mma_ts(tm + 256 + i * HD, tm + buf * 128 + k * 8, vd + k * 128, ID_O, add || k > 0);
-      pf_commit(&o_full[i]);
+      for (int k = 0; k < PF_TS / 16; ++k) pf_mma_ts(tm + BUFS * 128 + i * HD, tm + buf * 128 + k * 8, vd + k * 128, ID_O, add || k > 0);
+      pf_commit(&o_done[buf]);
       if (last) pf_commit(&o_last[i]);
     };
-    auto free_tile = [&](uint64_t* bar) {
-      if (lead) pf_commit(bar);
+    auto free_tile = [&](uint32_t k) {
+      if (lead) pf_commit(&kv_empty[k % SLOTS]);
     };
-    uint32_t used = 0, n_p[2] = {0, 0};  // K and V tiles so far, phases of p_full so far
-    auto ready = [&](uint32_t k) {        // tile k of the ring is there
-      wait_warp(&kv_full[k % SLOTS], (k / SLOTS) & 1);
-      pf_fence_after();
-    };
+    uint32_t used = 0, units = 0;  // K and V tiles, and units, of all pieces so far
     for (int r = 0;; ++r) {
       wait_warp(&info_full[r & 1], (r >> 1) & 1);
       const PfPiece& in = info[r & 1];
       const int seq = __shfl_sync(0xffffffffu, in.seq, 0), n0 = __shfl_sync(0xffffffffu, in.n0, 0), n1 = __shfl_sync(0xffffffffu, in.n1, 0);
-      const int n_max = max(n0, n1);
-      const bool two = n1 > 0 || __shfl_sync(0xffffffffu, in.f_end - in.f0, 0) > 128;
+      const bool two = __shfl_sync(0xffffffffu, in.f_end - in.f0, 0) > 128;
       if (seq < 0 || is_dead()) break;
       __syncwarp();
       if (lead) {
@@ -772,57 +783,41 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       }
       wait_warp(&q_full, r & 1);
       pf_fence_after();
-      if (n_max > 0) ready(used);
-      if (two) {
-        if (n0 > 0) scores(0, 0, used % SLOTS);
-        if (n1 > 0) scores(1, 1, used % SLOTS);
-        if (n_max > 0) free_tile(&kv_empty[used % SLOTS]);
-        for (int j = 0; j < n_max && !is_dead(); ++j) {
-          const uint32_t v = used + 2 * j + 1, kn = v + 1;
-          ready(v);
-          bool k_there = false;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int n_t = i ? n1 : n0;
-            if (j >= n_t) continue;
-            if (j + 1 < n_t && !k_there) ready(kn), k_there = true;
-            wait_warp(&p_full[i], n_p[i] & 1);
-            ++n_p[i];
-            pf_fence_after();
-            values(i, i, v % SLOTS, j > 0, j + 1 == n_t);
-            if (j + 1 < n_t) scores(i, i, kn % SLOTS);
-            if (i == 1 || j >= n1) free_tile(&kv_empty[v % SLOTS]);
-          }
-          if (j + 1 < n_max) free_tile(&kv_empty[kn % SLOTS]);
-        }
-      } else {
-        // one row tile: S runs one tile ahead in the other buffer
-        if (n0 > 0) {
-          scores(0, 0, used % SLOTS);
-          free_tile(&kv_empty[used % SLOTS]);
-        }
-        if (n0 > 1) {
-          ready(used + 2);
-          scores(0, 1, (used + 2) % SLOTS);
-          free_tile(&kv_empty[(used + 2) % SLOTS]);
-        }
-        for (int j = 0; j < n0 && !is_dead(); ++j) {
-          const uint32_t v = used + 2 * j + 1, kn = v + 3;
-          const int buf = j & 1;
-          ready(v);
-          wait_warp(&p_full[buf], n_p[buf] & 1);
-          ++n_p[buf];
+      const int n = two ? n0 + n1 : n0;
+      int next_k = 0, next_v = 0;  // tiles of slots whose K, whose V, have been waited for
+      auto tile_of = [&](int u, int& i) {
+        i = two && (u >= 2 * n0 || (u & 1));
+        return !two ? u : u < 2 * n0 ? u >> 1 : u - n0;
+      };
+      auto start = [&](int u) {  // S of unit u
+        int i;
+        const int j = tile_of(u, i);
+        const uint32_t k = used + 2 * j;
+        if (j >= next_k) {
+          wait_warp(&kv_full[k % SLOTS], (k / SLOTS) & 1);
           pf_fence_after();
-          values(0, buf, v % SLOTS, j > 0, j + 1 == n0);
-          free_tile(&kv_empty[v % SLOTS]);
-          if (j + 2 < n0) {
-            ready(kn);
-            scores(0, buf, kn % SLOTS);
-            free_tile(&kv_empty[kn % SLOTS]);
-          }
+          next_k = j + 1;
         }
+        scores(i, (units + u) % BUFS, k % SLOTS);
+        if (!two || i) free_tile(k);  // the second row tile sees every tile of slots that the first does
+      };
+      for (int u = 0; u < min(n, BUFS); ++u) start(u);
+      for (int u = 0; u < n && !is_dead(); ++u) {
+        int i;
+        const int j = tile_of(u, i);
+        const uint32_t g = units + u, v = used + 2 * j + 1;
+        if (j >= next_v) {
+          wait_warp(&kv_full[v % SLOTS], (v / SLOTS) & 1);
+          next_v = j + 1;
+        }
+        wait_warp(&p_full[g % BUFS], (g / BUFS) & 1);
+        pf_fence_after();
+        values(i, g % BUFS, v % SLOTS, j > 0, j + 1 == (i ? n1 : n0));
+        if (!two || i) free_tile(v);
+        if (u + BUFS < n) start(u + BUFS);
       }
-      used += 2 * n_max;
+      units += n;
+      used += 2 * max(n0, n1);
     }
     if (lead) pf_commit(&drained);
     mbar_wait_warp(&drained, 0);

@@ -17,10 +17,15 @@ int tiles_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
   p.group = a.n_q / c.n_kv;
   const long long rows = (long long)a.rows * p.group;  // packed, of a request (tree) or of all
   if (rows > 0x7fffff00ll) return pfail(VP_ERR_ARG, "more rows than a launch holds");
-  p.block_rows = rows < PF_ROWS ? (int)rows : PF_ROWS;
+  if (const int e = sm_count(&p.sms)) return e;
+  // at most this many blocks of 256 rows: every request's last block may be short. Where they leave half of
+  // the SMs idle, 128 rows make a block: twice the CTAs, each with one row tile (a prompt of 1,024 rows
+  // of 14 query and 2 key-value heads: 28 us with 256, 19 us with 128).
+  auto blocks_of = [&](int of) { return (a.q_start ? rows / of + a.n : (rows + of - 1) / of * a.n) * c.n_kv; };
+  p.rows = blocks_of(PF_ROWS) * 2 <= p.sms ? PF_ROWS / 2 : PF_ROWS;
+  p.block_rows = rows < p.rows ? (int)rows : p.rows;
   p.tickets = static_cast<unsigned*>(a.work);
   p.rec = reinterpret_cast<float*>(static_cast<char*>(a.work) + WORK_HEAD);
-  if (const int e = sm_count(&p.sms)) return e;
   // the warpgroups trade registers: what the softmax takes on must have been launched with
   static const int regs = [] {
     cudaFuncAttributes f{};
@@ -29,11 +34,12 @@ int tiles_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
   if (regs * PF_THREADS < 2 * 128 * PF_SOFTMAX_REGS + 128 * PF_OTHER_REGS) return pfail(VP_ERR_CUDA, "the kernel was built with too few registers");
   CUtensorMap mk, mv;
   if (const int e = pool_maps(c, c.page_size < PF_TS ? c.page_size : PF_TS, 1, &mk, &mv)) return e;
-  // at most this many pieces: every request's last block may be short, and the cuts add two CTAs per
-  // SM at most, or as many as the table's longest request allows
-  const long long blocks = a.q_start ? rows / PF_ROWS + a.n : (rows + PF_ROWS - 1) / PF_ROWS * a.n;
-  const long long pairs = blocks * c.n_kv, tiles = ((long long)c.max_pages * c.page_size + PF_TS - 1) / PF_TS;
-  const long long cuts = (tiles + PF_LEAST - 1) / PF_LEAST - 1, more = pairs * cuts < 2 * p.sms ? pairs * cuts : 2 * p.sms;
+  // at most this many pieces: the cuts add two CTAs per SM at most, or as many as the table's longest request
+  // allows
+  const long long pairs = blocks_of(p.rows), tiles = ((long long)c.max_pages * c.page_size + PF_TS - 1) / PF_TS;
+  const long long cuts = (tiles + PF_LEAST - 1) / PF_LEAST - 1;
+  p.cuts = 2 * tiles > 3 * PF_LEAST;
+  const long long more = !p.cuts ? 0 : pairs * cuts < 2 * p.sms ? pairs * cuts : 2 * p.sms;
   if (pairs + more > 0x7fffffffll) return pfail(VP_ERR_ARG, "more rows than a launch holds");
   p.most = (int)(pairs + more);
   return pg_launch(a.q_start ? "vp_paged_prefill" : "vp_paged_decode", k_paged_tiles<T, HD>, p.most < p.sms ? p.most : p.sms, PF_THREADS,
