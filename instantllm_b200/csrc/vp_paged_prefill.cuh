@@ -43,6 +43,7 @@ struct PfShape {
 };
 
 constexpr int PF_RECORDS = 640;            // records at most: four per SM, for 160
+constexpr int PF_SORT = 128;               // requests that are sorted by length, at most
 constexpr int PF_LEAST = 16;               // tiles of a piece, at least
 
 struct PfParams {
@@ -137,7 +138,7 @@ __device__ __forceinline__ PfSpan pf_span(int lo, int end, int sinks) {
 }
 // The request's part of a call: its new rows, and the slots that packed rows [f, g) of it see.
 struct PfSeq {
-  int first, n_new, len, base, blocks, least, row;  // least: fewest mask bits of a row (trees); row: of the table
+  int index, first, n_new, len, base, blocks, least, row;  // index: of the request; least: fewest mask bits of a row (trees); row: of the table
   int lo, end;                                 // of the last range asked for
   __device__ __forceinline__ void see(const PfParams& p, int f, int g) {
     const bool tree = !p.a.q_start;
@@ -152,6 +153,7 @@ struct PfSeq {
 };
 __device__ __forceinline__ PfSeq pf_seq(const PfParams& p, int i) {
   PfSeq s;
+  s.index = i;
   s.first = 0;
   s.n_new = p.a.rows;
   s.least = 1;
@@ -258,9 +260,21 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   const int chunk = (a.n + PF_THREADS - 1) / PF_THREADS, i0 = min(a.n, tid * chunk), i1 = min(a.n, i0 + chunk);
   long long tiles = 0;
   int one_blocks = 0, one_last = 0;  // of the thread's last request
+  if (chunk == 1 && i0 < i1) seqs_s[tid] = pf_seq(p, tid);
+  if (a.n > 1 && a.n <= PF_SORT) {  // longest requests last: pieces are taken from the end
+    __shared__ int ranks_s[PF_SORT];
+    if (i0 < i1) ranks_s[tid] = seqs_s[tid].blocks ? seqs_s[tid].last_tiles(p) : 0;
+    const PfSeq s = seqs_s[min(tid, a.n - 1)];
+    cta_sync();
+    if (i0 < i1) {
+      int rank = 0;
+      for (int k = 0; k < a.n; ++k) rank += ranks_s[k] < ranks_s[tid] || (ranks_s[k] == ranks_s[tid] && k < tid);
+      seqs_s[rank] = s;
+    }
+    cta_sync();
+  }
   for (int i = i0; i < i1; ++i) {
-    PfSeq s = pf_seq(p, i);
-    if (chunk == 1) seqs_s[i] = s;
+    PfSeq s = chunk == 1 ? seqs_s[tid] : pf_seq(p, i);
     one_blocks = s.blocks;
     if (!s.blocks || !p.cuts) continue;
     one_last = s.last_tiles(p);
@@ -351,7 +365,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       }
       __syncwarp();
     };
-    bool fetched = false;
+    auto hand_over = [&] {  // they are there: the issuer may start the piece
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) pg_arrive(&q_full);
+    };
+    bool fetched = false, handed = false;
     for (int r = 0;; ++r) {
       if (!fetched) fetch(r);
       fetched = false;
@@ -377,11 +397,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       }
       __syncwarp();
       if (lane == 0) pg_arrive(&info_empty[r & 1]);
+      if (!handed) hand_over();
+      handed = false;
       {
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) pg_arrive(&q_full);
         // Everybody starts the piece together: a warp ahead of the others would wait for phases of barriers
         // whose earlier phases, the other warpgroup's, are still to come, and take one for another.
         wait_warp(&q_full, r & 1);
@@ -475,6 +493,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         wait_warp(&o_last[i], n_last & 1);
         ++n_last;
         pf_fence_after();
+        hand_over();  // the next piece's first scores are made beside this one's epilogue
+        handed = true;
       }
       units += two ? n0 + n1 : n0;
       T* out = static_cast<T*>(a.out) + seq * a.out_seq + (long long)(first + qrow) * a.out_row + h * a.out_head;
@@ -651,7 +671,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       if (tree) {
         const uint32_t all_rows = (1u << a.rows) - 1;
         uint32_t anc = 0, keep = 0;
-        if (lane < a.rows) anc = a.mask ? (uint32_t)a.mask[(long long)seq * a.rows + lane] & all_rows : (2u << lane) - 1;
+        if (lane < a.rows) anc = a.mask ? (uint32_t)a.mask[(long long)s.index * a.rows + lane] & all_rows : (2u << lane) - 1;
         const int pos = s.base + __popc(anc) - 1;
         for (int j = 0; j < a.rows; ++j) {  // less the new slots that have left the row's window
           const int place = s.base + __popc(__shfl_sync(0xffffffffu, anc, j)) - 1;
@@ -662,7 +682,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         if (lane == 0) in.any = any;
       }
       if (lane == 0) {
-        in.seq = seq, in.row = s.row, in.head = pair - block * c.n_kv, in.f0 = f0, in.f_end = f_end, in.first = s.first, in.base = s.base;
+        in.seq = s.index, in.row = s.row, in.head = pair - block * c.n_kv, in.f0 = f0, in.f_end = f_end, in.first = s.first, in.base = s.base;
         in.cut = cut, in.cuts = cuts, in.live = live, in.record0 = at_r + mine - cut;
         in.j0 = j0, in.n0 = max(0, min(j1, sp.upto(stop0)) - j0), in.n1 = f_end > f0 + 128 ? j1 - j0 : 0;
         in.see_lo = s.lo, in.see_end = s.end, in.ns = sp.ns, in.ws = sp.ws;
