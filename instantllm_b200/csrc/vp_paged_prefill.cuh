@@ -11,7 +11,8 @@
 // memory holds three buffers of S (two at head_dim 128; 128 columns each, the weights P written over
 // them as pairs) and both o (head_dim columns each). A unit is a row tile with a tile of slots; units go
 // round the buffers in order, first row tile, second row tile, next slots, so with three buffers the
-// next S of a row tile is there before its present weights are. One warp brings K and V tiles (TMA boxes of one page each), one thread
+// next S of a row tile is there before its present weights are. A block of one row tile has both
+// warpgroups too: they take its tiles of slots in turns and join their two records at the end. One warp brings K and V tiles (TMA boxes of one page each), one thread
 // issues the products, and two warpgroups, one tile each and one row a thread, do the softmax: while
 // one of them works on its tile, the tensor cores work on the other's.
 //
@@ -197,9 +198,21 @@ __device__ __forceinline__ float2 pf_add2(float2 a, float2 b) {
   return *reinterpret_cast<float2*>(&d);
 }
 
-// Number of the unit (row tile i, j-th tile of slots) in its piece; the first row tile has n0 tiles, the second as
-// many or more.
-__device__ __forceinline__ int pf_unit(bool two, int i, int j, int n0) { return !two ? j : j < n0 ? 2 * j + i : n0 + j; }
+// Number of the unit (warpgroup i, its j-th tile of slots) in its piece. Two row tiles: one to a warpgroup, the
+// first has n0 tiles of slots, the second as many or more. One: the warpgroups take turns.
+__device__ __forceinline__ int pf_unit(bool two, int i, int j, int n0) { return !two || j < n0 ? 2 * j + i : n0 + j; }
+
+// Named barriers of the warpgroups with one row tile: the second one's part of o is there, is taken.
+constexpr int PF_PART = 3, PF_TAKEN = 4;
+__device__ __forceinline__ void pf_sync(int bar) {
+  __syncwarp();
+  asm volatile("barrier.sync %0, 256;" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void pf_arrive(int bar) {
+  __threadfence_block();
+  __syncwarp();
+  asm volatile("barrier.arrive %0, 256;" ::"r"(bar) : "memory");
+}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(PF_THREADS, 1)
@@ -215,6 +228,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   __shared__ long long tile_sums[PF_THREADS / 32];
   __shared__ int sums[PF_THREADS / 32][2], starts[PF_THREADS], rec_starts[PF_THREADS], dead, last_s[2];
   __shared__ PfPiece info[2];
+  __shared__ float2 part_ml[128];  // m and l of the second warpgroup's records
   __shared__ PfSeq seqs_s[PF_THREADS];  // the requests, where there are no more than threads
 
   const vp_paged& c = p.c;
@@ -343,7 +357,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
 
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PF_SOFTMAX_REGS));
-    // ---- softmax: warpgroup i has row tile i, a thread row f ----
+    // ---- softmax: warpgroup i has row tile i (or every other tile of slots), a thread row f ----
     const int i = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 lanes of tensor memory
     const uint32_t to = tmem + lanes + BUFS * 128 + i * HD;
@@ -355,7 +369,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     auto fetch = [&](int r) {
       wait_warp(&info_full[r & 1], (r >> 1) & 1);
       const PfPiece& in = info[r & 1];
-      const int f = in.f0 + tid;
+      const int f = in.f0 + tid;  // with one row tile the second warpgroup has none to bring
       if (in.seq >= 0 && f < in.f_end) {
         const T* q = static_cast<const T*>(a.q) + in.seq * a.q_seq + (long long)(in.first + f / p.group) * a.q_row +
                      (in.head * p.group + f % p.group) * a.q_head;
@@ -371,15 +385,18 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       __syncwarp();
       if (lane == 0) pg_arrive(&q_full);
     };
-    bool fetched = false, handed = false;
+    bool fetched = false, handed = false, lent = false;  // lent: the row tile's buffer holds a part of o
     for (int r = 0;; ++r) {
+      if (lent) pf_sync(PF_TAKEN);  // the buffer is the queries' again
+      lent = false;
       if (!fetched) fetch(r);
       fetched = false;
       const PfPiece& in = info[r & 1];
-      const int seq = in.seq, f = in.f0 + tid, f_end = in.f_end, f0 = in.f0, head = in.head, first = in.first, base = in.base;
+      const int seq = in.seq, f_end = in.f_end, f0 = in.f0, head = in.head, first = in.first, base = in.base;
       if (seq < 0 || is_dead()) break;
       const bool two = f_end > f0 + 128;  // row tiles
-      const int n_t = i ? in.n1 : in.n0, j0 = in.j0, cuts = in.cuts, cut = in.cut, live = in.live, record0 = in.record0;
+      const int i_row = two ? i : 0, f = f0 + i_row * 128 + row;
+      const int n_t = !two ? (in.n0 + 1 - i) / 2 : i ? in.n1 : in.n0, j0 = in.j0, cuts = in.cuts, cut = in.cut, live = in.live, record0 = in.record0;
       const int n0 = in.n0, n1 = in.n1;
       PfSpan sp;
       sp.ns = in.ns;
@@ -405,11 +422,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         wait_warp(&q_full, r & 1);
       }
       // every row of the tile sees [lo_all, hi_all)
-      const int hi_all = tree ? base : base + (f0 + i * 128) / p.group + 1;
-      const int lo_all = !a.window ? 0 : tree ? base + a.rows - a.window : base + (f0 + i * 128 + 127) / p.group - a.window + 1;
+      const int hi_all = tree ? base : base + (f0 + i_row * 128) / p.group + 1;
+      const int lo_all = !a.window ? 0 : tree ? base + a.rows - a.window : base + (f0 + i_row * 128 + 127) / p.group - a.window + 1;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n_t; ++j) {
-        const int s0 = sp.at(j0 + j) * PF_TS;
+        const int s0 = sp.at(j0 + (two ? j : 2 * j + i)) * PF_TS;
         const uint32_t u = units + pf_unit(two, i, j, n0), buf = u % BUFS;
         const uint32_t ts = tmem + lanes + buf * 128;
         wait_warp(&s_full[buf], (u / BUFS) & 1);
@@ -417,7 +434,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         uint32_t s[128];
 #pragma unroll
         for (int k = 0; k < 4; ++k) pf_ld32(s + 32 * k, ts + 32 * k);
-        if (j + 1 == n_t) {  // the last scores are there: the next piece's queries may come
+        if (j + 1 == n_t && two) {  // the row tile's last scores are there: the next piece's queries may come
           fetch(r + 1);
           fetched = true;
         }
@@ -493,15 +510,23 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         wait_warp(&o_last[i], n_last & 1);
         ++n_last;
         pf_fence_after();
-        hand_over();  // the next piece's first scores are made beside this one's epilogue
-        handed = true;
+        if (fetched) {
+          hand_over();  // the next piece's first scores are made beside this one's epilogue
+          handed = true;
+        } else if (i == 0) {  // one row tile: before this product the other warpgroup's last scores were made too
+          fetch(r + 1);
+          fetched = true;
+        }
       }
       units += two ? n0 + n1 : n0;
       T* out = static_cast<T*>(a.out) + seq * a.out_seq + (long long)(first + qrow) * a.out_row + h * a.out_head;
       float* lse = a.lse ? a.lse + ((tree ? (long long)seq * a.rows : (long long)first) + qrow) * a.n_q + h : nullptr;
       float* rec = p.rec + (size_t)(record0 + cut) * rec_floats;
-      const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-      if (f_end > f0 + i * 128) {
+      // one row tile: the second warpgroup hands its record over, 32 elements at a time, in its row tile's buffer
+      unsigned char* part = qs + TILE + row * 128;
+      float mine = 1.f, other = 0.f;
+      if (!two && i == 1) {
+        part_ml[row] = make_float2(m, l);
 #pragma unroll 1
         for (int k = 0; k < HD; k += 32) {
           uint32_t o[32];
@@ -511,6 +536,47 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0;
+          }
+          if (k > 0) pf_sync(PF_TAKEN);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<uint4*>(part + ((e ^ (row & 7)) << 4)) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          pf_arrive(PF_PART);
+        }
+        lent = true;
+      }
+      if (f_end > f0 + i * 128) {
+        float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+#pragma unroll 1
+        for (int k = 0; k < HD; k += 32) {
+          uint32_t o[32];
+          if (n_t > 0) {
+            pf_ld32(o, to + k);
+            pf_loaded(o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0;
+          }
+          if (!two) {
+            pf_sync(PF_PART);
+            if (k == 0) {
+              const float2 ml = part_ml[row];
+              const float top = fmaxf(m, ml.x), use = top == -INFINITY ? 0.f : top;
+              mine = pg_exp2(m - use);
+              other = pg_exp2(ml.x - use);
+              l = l * mine + ml.y * other;
+              m = top;
+              inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float4 v = *reinterpret_cast<const float4*>(part + ((e ^ (row & 7)) << 4));
+              o[4 * e] = __float_as_uint(__uint_as_float(o[4 * e]) * mine + v.x * other);
+              o[4 * e + 1] = __float_as_uint(__uint_as_float(o[4 * e + 1]) * mine + v.y * other);
+              o[4 * e + 2] = __float_as_uint(__uint_as_float(o[4 * e + 2]) * mine + v.z * other);
+              o[4 * e + 3] = __float_as_uint(__uint_as_float(o[4 * e + 3]) * mine + v.w * other);
+            }
+            pf_arrive(PF_TAKEN);
           }
           if (valid && cuts > 1) {
 #pragma unroll
@@ -805,8 +871,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       pf_fence_after();
       const int n = two ? n0 + n1 : n0;
       int next_k = 0, next_v = 0;  // tiles of slots whose K, whose V, have been waited for
-      auto tile_of = [&](int u, int& i) {
-        i = two && (u >= 2 * n0 || (u & 1));
+      auto tile_of = [&](int u, int& i) {  // warpgroup and tile of slots of unit u
+        i = two && u >= 2 * n0 ? 1 : u & 1;
         return !two ? u : u < 2 * n0 ? u >> 1 : u - n0;
       };
       auto start = [&](int u) {  // S of unit u
@@ -818,7 +884,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           pf_fence_after();
           next_k = j + 1;
         }
-        scores(i, (units + u) % BUFS, k % SLOTS);
+        scores(two ? i : 0, (units + u) % BUFS, k % SLOTS);
         if (!two || i) free_tile(k);  // the second row tile sees every tile of slots that the first does
       };
       for (int u = 0; u < min(n, BUFS); ++u) start(u);
@@ -832,7 +898,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         }
         wait_warp(&p_full[g % BUFS], (g / BUFS) & 1);
         pf_fence_after();
-        values(i, g % BUFS, v % SLOTS, j > 0, j + 1 == (i ? n1 : n0));
+        values(i, g % BUFS, v % SLOTS, two ? j > 0 : u > 1, two ? j + 1 == (i ? n1 : n0) : u + 2 >= n);
         if (!two || i) free_tile(v);
         if (u + BUFS < n) start(u + BUFS);
       }
