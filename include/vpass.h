@@ -421,7 +421,7 @@ typedef struct {
   float scale;
   int32_t n, rows, n_q, window, sinks;
 } vp_paged_attn;
-#define VP_PAGED_WORK_ZEROED 8192
+#define VP_PAGED_WORK_ZEROED 16384
 size_t vp_paged_work_bytes(int32_t head_dim, int32_t n_q, int32_t n_kv, int32_t rows);
 int vp_paged_decode(const vp_paged* c, const vp_paged_attn* a, void* stream);
 int vp_paged_prefill(const vp_paged* c, const vp_paged_attn* a, void* stream);

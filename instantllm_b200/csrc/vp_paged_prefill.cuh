@@ -45,13 +45,14 @@ struct PfShape {
 
 constexpr int PF_RECORDS = 640;            // records at most: four per SM, for 160
 constexpr int PF_SORT = 128;               // requests that are sorted by length, at most
+constexpr int PF_JOIN = 8;                 // records joined at a time
 constexpr int PF_LEAST = 16;               // tiles of a piece, at least
 
 struct PfParams {
   vp_paged c;
   vp_paged_attn a;
   float* rec;         // records of block_rows rows, one per piece of a cut block
-  unsigned* tickets;  // [records][2 row tiles], then the scheduler's two
+  unsigned* tickets;  // [2 steps of a join][records][2 row tiles], then the scheduler's two
   int group, block_rows, sms, most;  // most: pieces that a call can have
   int rows;                          // packed rows of a block: 256, or 128 where there are few blocks
   int cuts;                          // whether the table's longest request may be cut
@@ -522,6 +523,96 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       T* out = static_cast<T*>(a.out) + seq * a.out_seq + (long long)(first + qrow) * a.out_row + h * a.out_head;
       float* lse = a.lse ? a.lse + ((tree ? (long long)seq * a.rows : (long long)first) + qrow) * a.n_q + h : nullptr;
       float* rec = p.rec + (size_t)(record0 + cut) * rec_floats;
+      // The warpgroup's writes are out, and it is told whether it is the last of n to come (and the counter is reset).
+      auto arrive_last = [&](unsigned* ticket, int n) {
+        __threadfence();
+        __syncwarp();
+        asm volatile("barrier.sync %0, 128;" ::"r"(1 + i) : "memory");
+        if (row == 0) {
+          last_s[i] = atomicAdd(ticket, 1u) == (unsigned)(n - 1);
+          if (last_s[i]) *ticket = 0;
+        }
+        __syncwarp();
+        asm volatile("barrier.sync %0, 128;" ::"r"(1 + i) : "memory");
+        const bool last = last_s[i];
+        if (last) __threadfence();
+        return last;
+      };
+      // Records first, first + step, .. (n of them) of the row tile joined into the output, or into the first one:
+      // a thread a row, the weights in place of the maxima; then 4 elements a thread and turn, four turns'
+      // reads of 4 records in flight.
+      auto join = [&](int from, int n, int step, bool to_out) {
+        float* rec0 = p.rec + (size_t)(record0 + from) * rec_floats;
+        const size_t stride = step * rec_floats;
+        const int n_rows = min(128, f_end - f0 - i * 128);
+        float top = -INFINITY, sm = 0.f;
+        if (row < n_rows) {
+#pragma unroll 8
+          for (int k = 0; k < n; ++k) top = fmaxf(top, __ldcg(rec0 + k * stride + m_at + tid));
+          const float us = top == -INFINITY ? 0.f : top;
+#pragma unroll 8
+          for (int k = 0; k < n; ++k) sm += __ldcg(rec0 + k * stride + l_at + tid) * pg_exp2(__ldcg(rec0 + k * stride + m_at + tid) - us);
+          const float iv = !to_out ? 1.f : sm > 0.f ? 1.f / sm : sm == 0.f ? 0.f : sm;
+#pragma unroll 8
+          for (int k = 0; k < n; ++k) {
+            float* x = rec0 + k * stride + m_at + tid;
+            *x = pg_exp2(__ldcg(x) - us) * iv;
+          }
+          if (to_out && lse) *lse = sm == 0.f ? -INFINITY : (top + log2f(sm)) * 0.6931471805599453f;
+        }
+        __threadfence();
+        __syncwarp();
+        asm volatile("barrier.sync %0, 128;" ::"r"(1 + i) : "memory");
+        constexpr int W = 4;
+        for (int x0 = row; x0 < n_rows * (HD / 4); x0 += 128 * W) {
+          float4 acc[W] = {};
+          int mm[W], d[W];
+#pragma unroll
+          for (int e = 0; e < W; ++e) {
+            const int x = min(x0 + 128 * e, n_rows * (HD / 4) - 1);
+            mm[e] = i * 128 + x / (HD / 4), d[e] = x % (HD / 4) * 4;
+          }
+          for (int k0 = 0; k0 < n; k0 += 4) {
+            float4 v[W][4];
+            float w[W][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float* x = rec0 + min(k0 + k, n - 1) * stride;
+#pragma unroll
+              for (int e = 0; e < W; ++e) {
+                v[e][k] = __ldcg(reinterpret_cast<const float4*>(x + (size_t)mm[e] * HD + d[e]));
+                w[e][k] = __ldcg(x + m_at + mm[e]);
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int e = 0; e < W; ++e) {
+                const float f1 = k0 + k < n ? w[e][k] : 0.f;
+                acc[e].x += v[e][k].x * f1, acc[e].y += v[e][k].y * f1, acc[e].z += v[e][k].z * f1, acc[e].w += v[e][k].w * f1;
+              }
+          }
+#pragma unroll
+          for (int e = 0; e < W; ++e) {
+            if (x0 + 128 * e >= n_rows * (HD / 4)) break;
+            if (!to_out) {
+              *reinterpret_cast<float4*>(rec0 + (size_t)mm[e] * HD + d[e]) = acc[e];
+              continue;
+            }
+            const int r2 = (f0 + mm[e]) / p.group, h2 = head * p.group + (f0 + mm[e]) % p.group;
+            uint2 v2;
+            v2.x = PgType<T>::down(acc[e].x, acc[e].y);
+            v2.y = PgType<T>::down(acc[e].z, acc[e].w);
+            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + seq * a.out_seq + (long long)(first + r2) * a.out_row + h2 * a.out_head + d[e]) = v2;
+          }
+        }
+        if (!to_out) {
+          __syncwarp();
+          asm volatile("barrier.sync %0, 128;" ::"r"(1 + i) : "memory");
+          if (row < n_rows) rec0[m_at + tid] = top, rec0[l_at + tid] = sm;
+        }
+        __syncwarp();
+      };
       // one row tile: the second warpgroup hands its record over, 32 elements at a time, in its row tile's buffer
       unsigned char* part = qs + TILE + row * 128;
       float mine = 1.f, other = 0.f;
@@ -601,80 +692,18 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         if (valid && cuts == 1 && lse) *lse = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
         pf_fence_before();
         if (cuts > 1) {
-          __threadfence();
-          __syncwarp();
-          asm volatile("barrier.sync %0, 128;" ::"r"(1 + i) : "memory");
-          unsigned* ticket = p.tickets + record0 * 2 + i;
-          if (row == 0) last_s[i] = atomicAdd(ticket, 1u) == (unsigned)(cuts - 1);
-          __syncwarp();
-          asm volatile("barrier.sync %0, 128;" ::"r"(1 + i) : "memory");
-          if (last_s[i]) {
-            // All pieces of the row tile are there: a thread a row, their weights in place of their maxima;
-            // then 4 elements a thread and turn, two turns' reads of 8 pieces in flight.
-            __threadfence();
-            float* rec0 = p.rec + (size_t)record0 * rec_floats;
-            const int n_rows = min(128, f_end - f0 - i * 128);
-            if (row < n_rows) {
-              float top = -INFINITY, sm = 0.f;
-#pragma unroll 8
-              for (int k = 0; k < live; ++k) top = fmaxf(top, __ldcg(rec0 + k * rec_floats + m_at + tid));
-              const float us = top == -INFINITY ? 0.f : top;
-#pragma unroll 8
-              for (int k = 0; k < live; ++k)
-                sm += __ldcg(rec0 + k * rec_floats + l_at + tid) * pg_exp2(__ldcg(rec0 + k * rec_floats + m_at + tid) - us);
-              const float iv = sm > 0.f ? 1.f / sm : sm == 0.f ? 0.f : sm;
-#pragma unroll 8
-              for (int k = 0; k < live; ++k) {
-                float* x = rec0 + k * rec_floats + m_at + tid;
-                *x = pg_exp2(__ldcg(x) - us) * iv;
-              }
-              if (lse) *lse = sm == 0.f ? -INFINITY : (top + log2f(sm)) * 0.6931471805599453f;
-            }
-            __threadfence();
-            __syncwarp();
-            asm volatile("barrier.sync %0, 128;" ::"r"(1 + i) : "memory");
-            constexpr int W = 4;  // turns whose reads fly together
-            for (int x0 = row; x0 < n_rows * (HD / 4); x0 += 128 * W) {
-              float4 acc[W] = {};
-              int mm[W], d[W];
-#pragma unroll
-              for (int e = 0; e < W; ++e) {
-                const int x = min(x0 + 128 * e, n_rows * (HD / 4) - 1);
-                mm[e] = i * 128 + x / (HD / 4), d[e] = x % (HD / 4) * 4;
-              }
-              for (int k0 = 0; k0 < live; k0 += 4) {
-                float4 v[W][4];
-                float w[W][4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const float* x = rec0 + (size_t)min(k0 + k, live - 1) * rec_floats;
-#pragma unroll
-                  for (int e = 0; e < W; ++e) {
-                    v[e][k] = __ldcg(reinterpret_cast<const float4*>(x + (size_t)mm[e] * HD + d[e]));
-                    w[e][k] = __ldcg(x + m_at + mm[e]);
-                  }
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-#pragma unroll
-                  for (int e = 0; e < W; ++e) {
-                    const float f1 = k0 + k < live ? w[e][k] : 0.f;
-                    acc[e].x += v[e][k].x * f1, acc[e].y += v[e][k].y * f1, acc[e].z += v[e][k].z * f1, acc[e].w += v[e][k].w * f1;
-                  }
-              }
-#pragma unroll
-              for (int e = 0; e < W; ++e) {
-                if (x0 + 128 * e >= n_rows * (HD / 4)) break;
-                const int r2 = (f0 + mm[e]) / p.group, h2 = head * p.group + (f0 + mm[e]) % p.group;
-                uint2 v2;
-                v2.x = PgType<T>::down(acc[e].x, acc[e].y);
-                v2.y = PgType<T>::down(acc[e].z, acc[e].w);
-                *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + seq * a.out_seq + (long long)(first + r2) * a.out_row + h2 * a.out_head + d[e]) = v2;
-              }
-            }
-            if (row == 0) *ticket = 0;
+          // A few pieces are joined by the one that finishes last; of many, every PF_JOIN by their last one into
+          // the first one's record, and those by the last of all.
+          unsigned* t1 = p.tickets + 2 * (record0 + cut / PF_JOIN * PF_JOIN) + i;
+          unsigned* t2 = p.tickets + 2 * PF_RECORDS + 2 * record0 + i;
+          const bool deep = cuts > PF_JOIN + PF_JOIN / 2;
+          const int k_first = deep ? cut / PF_JOIN * PF_JOIN : 0, k_last = deep ? min(cuts, k_first + PF_JOIN) : cuts;
+          bool last = arrive_last(deep ? t1 : t2, k_last - k_first);
+          if (last && deep) {
+            join(k_first, max(0, min(k_last, live) - k_first), 1, false);
+            last = arrive_last(t2, (cuts + PF_JOIN - 1) / PF_JOIN);
           }
-          __syncwarp();
+          if (last) join(0, deep ? (live + PF_JOIN - 1) / PF_JOIN : live, deep ? PF_JOIN : 1, true);
         }
       }
       pf_fence_before();
@@ -684,7 +713,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   if (warp == PF_SCHEDULER) {
     // ---- the CTA's pieces: one for each CTA, then whoever comes first has the next, from the last request's
     // last block on. Which CTA has a piece does not show in the results. ----
-    unsigned* next = p.tickets + 2 * PF_RECORDS;  // and the number of CTAs that have come to the end
+    unsigned* next = p.tickets + 4 * PF_RECORDS;  // and the number of CTAs that have come to the end
     for (int r = 0;; ++r) {
       if (r >= 2) wait_warp(&info_empty[r & 1], ((r >> 1) - 1) & 1);
       unsigned idx = blockIdx.x;

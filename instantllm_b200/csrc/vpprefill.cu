@@ -6,7 +6,7 @@
 
 namespace {
 
-static_assert(PF_RECORDS >= 4 * PG_MAX_CTAS && (2 * PF_RECORDS + 2) * sizeof(unsigned) <= WORK_HEAD, "records and their counters");
+static_assert(PF_RECORDS >= 4 * PG_MAX_CTAS && (4 * PF_RECORDS + 2) * sizeof(unsigned) <= WORK_HEAD, "records and their counters");
 
 template <typename T, int HD>
 int tiles_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {

@@ -26,7 +26,7 @@ from ._lib import VpError, VpPaged, VpPagedAttn, VpPagedRows, check
 TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 DEV_ERR_TIMEOUT, DEV_ERR_PAGE, DEV_ERR_SLOT = 4, 16, 32
 MAX_ROWS = 16
-WORK_ZEROED = 8192
+WORK_ZEROED = 16384
 
 # The argument structs (VpPagedRows, VpPagedAttn) are packed in one go: a call of a few microseconds on the GPU should
 # not take longer to prepare, and setting two dozen ctypes fields takes 2 us.
