@@ -533,6 +533,27 @@ def test_append_in_place_and_one_row():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("src", [torch.float16, torch.float32])
+def test_append_large_call_equals_small_ones(src):
+    """A call too large for L2 (it runs in another shape) writes the bits of the same rows in small calls."""
+    nq, nkv, hd, ps, n = 32, 8, 128, 64, 3500
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn((n, nq + 2 * nkv, hd), generator=g, device="cuda").to(src)
+    pages = -(-n // ps)
+    table = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)[None]
+    seq, slot = torch.zeros(n, dtype=torch.int32, device="cuda"), torch.arange(n, dtype=torch.int32, device="cuda")
+    rope = paged.rope_table(n, hd)
+    got = []
+    for step in (n, 500):
+        kv = paged.PagedLayer(*torch.zeros((2, pages, nkv, ps, hd), dtype=torch.float16, device="cuda"), table)
+        q = [kv.append(x[a:a + step, :nq], x[a:a + step, nq:nq + nkv], x[a:a + step, nq + nkv:], seq[a:a + step], slot[a:a + step],
+                       slot[a:a + step], rope) for a in range(0, n, step)]
+        got.append((torch.cat(q), kv.k, kv.v))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits():
     """A pool of more than 2^32 elements: its last page is written and read like its first."""
     hd, ps, nkv, nq = 64, 64, 2, 14
