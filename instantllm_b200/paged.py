@@ -22,6 +22,7 @@ import torch
 
 from . import _lib
 from ._lib import VpError, VpPaged, VpPagedAttn, VpPagedRows, check
+from .synth import tree_to_buffer
 
 TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 DEV_ERR_TIMEOUT, DEV_ERR_PAGE, DEV_ERR_SLOT = 4, 16, 32
@@ -44,14 +45,11 @@ def rope_table(rows: int, rot_dim: int = 64, theta: float = 1e6, device=0) -> to
 
 
 def ancestor_masks(trees) -> torch.Tensor:
-    """Ancestor bitmasks int32 [n][16] of trees in the verify pass's form (dicts of synth.seeded_tree and the like: n and
-    parent), the row's own bit included; unused rows are 0."""
+    """Ancestor bitmasks int32 [n][16] of draft trees (dicts as in synth.seeded_tree), the row's own bit included: the last
+    part of the verify pass's tree buffer. Unused rows are 0."""
     out = torch.zeros((len(trees), MAX_ROWS), dtype=torch.int32)
     for i, t in enumerate(trees):
-        anc = []
-        for r in range(t["n"]):
-            anc.append((0 if r == 0 else anc[t["parent"][r]]) | 1 << r)
-        out[i, :t["n"]] = torch.tensor(anc, dtype=torch.int32)
+        out[i, :t["n"]] = torch.from_numpy(tree_to_buffer(t)[49:49 + t["n"]])
     return out
 
 

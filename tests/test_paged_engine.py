@@ -1,0 +1,126 @@
+"""The model over the paged cache (instantllm_b200/paged_engine.py) against the CPU oracle and against VerifyEngine: prompts in
+a batch and in chunks, one token a step, draft trees with their commit."""
+import numpy as np
+import pytest
+
+from instantllm_b200 import synth
+
+VOCAB = 4096
+
+
+@pytest.fixture(scope="module")
+def model():
+    import torch  # noqa: F401
+
+    from instantllm_b200.paged_engine import PagedEngine
+    from oracle import qwen_oracle as Q
+
+    w = synth.make_weights("q4", n_layers=2, vocab=VOCAB, seed=21)
+    return PagedEngine(w, n_pages=64, page_size=16, max_seqs=6, max_len=160), Q.model_from_weights(w), w
+
+
+def prompt(n, seed):
+    return (synth.make_prompt(n, seed=seed) % VOCAB).tolist()
+
+
+@pytest.mark.gpu
+def test_prompts_chunks_and_steps(model):
+    """Logits of a ragged batch, of a second chunk over it, and of single steps: within the passes' own bound of the fp32
+    oracle (fp16 activations: 0.05)."""
+    from oracle import qwen_oracle as Q
+
+    eng, m, _ = model
+    first = {3: prompt(37, 1), 0: prompt(1, 2), 5: prompt(64, 3)}
+    second = {0: prompt(20, 4), 5: prompt(3, 5)}
+    caches = {s: Q.KVCache(2, 160) for s in first}
+    got = eng.prefill(first).cpu().numpy()
+    want = [Q.forward_causal(m, caches[s], t, 0) for s, t in first.items()]
+    assert np.abs(got - np.stack(want)).max() < 0.05
+    got = eng.prefill(second).cpu().numpy()
+    want = [Q.forward_causal(m, caches[s], t, len(first[s])) for s, t in second.items()]
+    assert np.abs(got - np.stack(want)).max() < 0.05
+    pos = {s: len(first[s]) + len(second.get(s, [])) for s in first}
+    for step in range(3):
+        toks = {s: 7 * step + s for s in first}
+        got = eng.decode(toks).cpu().numpy()
+        want = [Q.forward_causal(m, caches[s], [toks[s]], pos[s] + step) for s in first]
+        assert np.abs(got - np.stack(want)).max() < 0.05
+    for s in first:
+        eng.release(s)
+    eng.kv.check()
+    assert eng.kv.free_pages == 64
+
+
+@pytest.mark.gpu
+def test_trees_and_commit(model):
+    """Trees of different sizes in one pass: logits against the oracle's tree pass, the committed path and the compacted
+    cache against a causal continuation."""
+    from oracle import qwen_oracle as Q
+
+    eng, m, _ = model
+    rng = np.random.default_rng(9)
+    prompts = {1: prompt(30, 6), 2: prompt(50, 7)}
+    first = dict(zip(prompts, eng.prefill(prompts).argmax(-1).tolist()))
+    caches, truth = {}, {}
+    for s, p in prompts.items():
+        caches[s] = Q.KVCache(2, 160)
+        Q.forward_causal(m, caches[s], p, 0)
+        truth[s] = Q.greedy(m, p, 10)[0]
+    trees = {1: synth.seeded_tree(rng, truth[1], n=16, p_match=0.9, vocab=VOCAB),
+             2: synth.seeded_tree(rng, truth[2], n=5, p_match=0.9, vocab=VOCAB)}
+    logits, out = eng.verify(trees, first)
+    logits = logits.cpu().numpy()
+    for i, s in enumerate(trees):
+        n = trees[s]["n"]
+        want = Q.tree_pass(m, caches[s].copy(), len(prompts[s]), first[s], trees[s])
+        assert np.abs(logits[i, :n] - want).max() < 0.05
+        assert len(out[s]) >= 1 and eng.lens[s] == len(prompts[s]) + len(out[s])
+        # the cache now holds prompt, root and accepted drafts in order: the next step agrees with a causal run over them
+        ids = prompts[s] + [first[s]] + out[s]
+        got = eng.decode({s: ids[-1]})[0].cpu().numpy()
+        assert np.abs(got - Q.forward_causal(m, Q.KVCache(2, 160), ids, 0)).max() < 0.05
+    for s in prompts:
+        eng.release(s)
+    eng.kv.check()
+
+
+@pytest.mark.gpu
+def test_generate_with_and_without_trees(model):
+    """Trees change no token of a greedy decode; VerifyEngine, on the same weights, takes the same ones as long as the two best
+    logits are not within rounding of each other."""
+    from instantllm_b200.engine import VerifyEngine
+
+    eng, _, w = model
+    prompts = [prompt(n, 30 + n) for n in (5, 33, 17, 60)]
+    plain = eng.generate(prompts, 12)
+    rng = np.random.default_rng(3)
+
+    def tree_fn(s, ids):  # drafts from the known continuation, some of them wrong
+        done = len(ids) - len(prompts[s])
+        return synth.seeded_tree(rng, (plain[s] + [0] * 20)[done:], n=16, p_match=0.7, vocab=VOCAB)
+
+    assert eng.generate(prompts, 12, tree_fn=tree_fn) == plain
+    ve = VerifyEngine(w, max_ctx=160, max_steps=64)
+    for p, got in zip(prompts, plain):
+        ve.begin(0, 12)
+        ve.prefill(p)
+        for _ in range(11):
+            ve.pass_(synth.root_tree())
+        want = ve.tokens(12)
+        same = next((i for i, (a, b) in enumerate(zip(got, want)) if a != b), len(got))
+        if same < len(got):  # the first difference must be a near tie
+            lg = eng.prefill({0: p + got[:same]})[0]
+            eng.release(0)
+            assert abs(float(lg[got[same]] - lg[want[same]])) < 0.05
+    ve.close()
+
+
+def test_dense_layouts_match_the_oracle():
+    """The dequantised weights of every format (CPU)."""
+    from instantllm_b200.paged_engine import _dense
+    from oracle import qwen_oracle as Q
+
+    rng = np.random.default_rng(0)
+    for fmt in ("q4", "q8", "q8g32", "f16"):
+        m = synth.make_matrix(fmt, 32, 128, rng)
+        assert np.array_equal(_dense(m, "cpu").numpy(), Q.dequant(m).astype(np.float16))
