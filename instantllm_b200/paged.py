@@ -15,26 +15,26 @@ table) is told by `check()`. The reference keeps one contiguous cache of one req
 from __future__ import annotations
 
 import ctypes
-import struct
 from typing import Optional
 
 import torch
 
 from . import _lib
-from ._lib import VpError, VpPaged, VpPagedAttn, VpPagedRows, check
+from ._lib import VpError, VpPaged, check
 from .synth import tree_to_buffer
 
-TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+TYPES = {torch.float16: 0, torch.bfloat16: 1}
 DEV_ERR_TIMEOUT, DEV_ERR_PAGE, DEV_ERR_SLOT = 4, 16, 32
 MAX_ROWS = 16
-WORK_ZEROED = 16384
 
-# The argument structs (VpPagedRows, VpPagedAttn) are packed in one go: a call of a few microseconds on the GPU should
-# not take longer to prepare, and setting two dozen ctypes fields takes 2 us.
-_ROWS = struct.Struct("8P8q6i")
-_ATTN = struct.Struct("8PQ6qf5i")
-assert _ROWS.size == ctypes.sizeof(VpPagedRows) and _ATTN.size <= ctypes.sizeof(VpPagedAttn)
-_I32, _F32 = torch.int32, torch.float32
+
+def _extension():
+    """The tensor side of the calls (csrc/paged_torch.cpp); like the library below it, it has no fallback."""
+    try:
+        from . import _paged
+    except ImportError as e:
+        raise VpError(f"instantllm_b200/_paged.so cannot be loaded ({e}): build it with instantllm_b200.build.build_torch()") from e
+    return _paged
 
 
 def rope_table(rows: int, rot_dim: int = 64, theta: float = 1e6, device=0) -> torch.Tensor:
@@ -53,16 +53,6 @@ def ancestor_masks(trees) -> torch.Tensor:
     return out
 
 
-# the current stream's handle without a Stream object around it (2 us), where torch has it
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda i: torch.cuda.current_stream(i).cuda_stream)
-
-
-def _index(t: torch.Tensor, what: str, shape, device: int) -> int:
-    if t.dtype is not _I32 or t.shape != shape or t.get_device() != device or not t.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous int32 tensor of shape {shape} on cuda:{device}")
-    return t.data_ptr()
-
-
 class PagedLayer:
     """One layer of a paged cache. k, v: [pages][heads][page_size][head_dim] in fp16 or bf16, elements of a slot adjacent, any
     strides in multiples of 8 elements (a [pages][page_size][heads][head_dim] pool transposed will do), the same for both;
@@ -79,7 +69,7 @@ class PagedLayer:
             raise ValueError("the elements of a slot must be adjacent")
         if table.dtype != torch.int32 or table.dim() != 2 or table.device != k.device or table.stride(1) != 1:
             raise ValueError("table must be an int32 [requests][pages] tensor on the pools' device, rows contiguous")
-        self.lib = _lib.load()
+        _lib.load()
         self.k, self.v, self.table, self.device, self.dtype = k, v, table, k.device, k.dtype
         self.pages, self.n_kv, self.page_size, self.head_dim = k.shape
         if status is None:
@@ -93,23 +83,9 @@ class PagedLayer:
         self._c = VpPaged(k.data_ptr(), v.data_ptr(), table.data_ptr(), status.data_ptr(), page, head, slot,
                           table.stride(0) if n > 1 else width, TYPES[k.dtype], self.n_kv, self.head_dim, self.page_size,
                           self.pages, n, width)
-        self._r, self._a = VpPagedRows(), VpPagedAttn()
-        self._cp, self._rp, self._ap = (ctypes.addressof(x) for x in (self._c, self._r, self._a))
-        self._index_of_device, self._need = self.device.index, {}
-
-    def _stream(self) -> int:
-        if torch.cuda.current_device() != self._index_of_device:
-            raise ValueError(f"the cache lives on {self.device}: make it the current device")
-        return _raw_stream(self._index_of_device)
-
-    def _out(self, like: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
-        if out is None:
-            if like.dtype is self.dtype and like.is_contiguous():
-                return torch.empty_like(like)
-            return torch.empty(like.shape, dtype=self.dtype, device=self.device)
-        if out.shape != like.shape or out.dtype is not self.dtype or out.get_device() != self._index_of_device or out.stride(-1) != 1:
-            raise ValueError("out must have q's shape and the cache's type, elements of a head adjacent")
-        return out
+        self._at = ctypes.addressof(self._c)
+        ext = _extension()
+        self._append, self._attend = ext.append, ext.attend
 
     def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq: torch.Tensor, slot: torch.Tensor,
                pos: Optional[torch.Tensor], rope: Optional[torch.Tensor], interleaved: bool = False,
@@ -118,41 +94,8 @@ class PagedLayer:
         projection will do): keys rotated to pos and values go to slot[t] of request seq[t] (seq < 0: not stored), the
         rotated queries are returned, in the cache's type. rope: fp32 [positions][rot_dim / 2][2] (rope_table), None for
         no rotation; interleaved: pairs (2i, 2i + 1) instead of (i, i + rot_dim / 2)."""
-        if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.dtype != q.dtype or v.dtype != q.dtype:
-            raise ValueError("q, k and v must be [rows][heads][head_dim] of one type")
-        n, nq, hd = q.shape
-        if k.shape != (n, self.n_kv, self.head_dim) or hd != self.head_dim:
-            raise ValueError(f"expected k and v of shape {(n, self.n_kv, self.head_dim)} and heads of {self.head_dim}")
-        if q.dtype is not self.dtype and q.dtype is not torch.float32:
-            raise ValueError("rows must have the cache's type or fp32")
-        qs, ks, vs = q.stride(), k.stride(), v.stride()
-        if qs[2] != 1 or ks[2] != 1 or vs[2] != 1:
-            raise ValueError("the elements of a head must be adjacent")
-        dev = self._index_of_device
-        if q.get_device() != dev or k.get_device() != dev or v.get_device() != dev:
-            raise ValueError(f"rows must be on cuda:{dev}")
-        shape = (n,)
-        places = _index(seq, "seq", shape, dev), _index(slot, "slot", shape, dev)
-        if rope is None:
-            places += None, None
-            turns = 0, 0
-        else:
-            if pos is None:
-                raise ValueError("a rotation needs pos")
-            rs = rope.shape
-            if len(rs) != 3 or rs[2] != 2 or rope.dtype is not _F32 or not rope.is_contiguous() or rope.get_device() != dev:
-                raise ValueError(f"rope must be a contiguous fp32 [positions][rot_dim / 2][2] tensor on cuda:{dev}")
-            places += _index(pos, "pos", shape, dev), rope.data_ptr()
-            turns = rs[0], 2 * rs[1]
-        out = self._out(q, out)
-        os = out.stride()
-        _ROWS.pack_into(self._r, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *(x or 0 for x in places),
-                        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
-                        TYPES[q.dtype], n, nq, *turns, 1 if interleaved else 0)
-        rc = self.lib.vp_paged_append(self._cp, self._rp, self._stream())
-        if rc:
-            check(rc, "vp_paged_append")
-        return out
+        r = self._append(self._at, self.device.index, q, k, v, seq, slot, pos, rope, interleaved, out)
+        return r if r.__class__ is not int else check(r, "vp_paged_append")
 
     def decode(self, q: torch.Tensor, lens: torch.Tensor, mask: Optional[torch.Tensor] = None,
                seqs: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0, scale: Optional[float] = None,
@@ -162,57 +105,16 @@ class PagedLayer:
         slot j (its own bit included; ancestor_masks), None for a causal chain. seqs: int32 [n], the requests' rows of the
         table (None: 0 .. n - 1). window > 0: a row sees the last `window` positions and the first `sinks`. Returns out
         like q, and with return_lse the log sum exp fp32 [n][rows][query heads]."""
-        shape, qs = q.shape, q.stride()
-        if len(shape) == 4:
-            n, rows, nq, _ = shape
-        elif len(shape) == 3:
-            (n, nq, _), rows, qs = shape, 1, (qs[0], 0, qs[1], qs[2])
-        else:
-            raise ValueError("q must be [n][rows][query heads][head_dim] or [n][query heads][head_dim]")
-        masks = 0 if mask is None else _index(mask, "mask", (n, rows), self._index_of_device)
-        return self._attend(self.lib.vp_paged_decode, "vp_paged_decode", q, qs, n, rows, nq, lens, seqs, masks, 0, window, sinks,
-                            scale, out, return_lse)
+        r = self._attend(False, self._at, self.device.index, self._work, q, lens, mask, None, seqs, window, sinks, scale, out, return_lse)
+        return r if r.__class__ is not int else check(r, "vp_paged_decode")
 
     def prefill(self, q: torch.Tensor, q_start: torch.Tensor, lens: torch.Tensor, seqs: Optional[torch.Tensor] = None,
                 window: int = 0, sinks: int = 0, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
                 return_lse: bool = False):
         """Causal attention of prompt rows: q [rows][query heads][head_dim], rows q_start[i] .. q_start[i + 1] - 1 being the last
         slots of lens[i] (already appended). Other arguments and results as in decode."""
-        if q.dim() != 3:
-            raise ValueError("q must be [rows][query heads][head_dim]")
-        n, qs = lens.shape[0], q.stride()
-        starts = _index(q_start, "q_start", (n + 1,), self._index_of_device)
-        return self._attend(self.lib.vp_paged_prefill, "vp_paged_prefill", q, (0, *qs), n, q.shape[0], q.shape[1], lens, seqs, 0,
-                            starts, window, sinks, scale, out, return_lse)
-
-    def _attend(self, call, name, q, qs, n, rows, nq, lens, seqs, masks, starts, window, sinks, scale, out, return_lse):
-        dev = self._index_of_device
-        if q.shape[-1] != self.head_dim or q.dtype is not self.dtype or q.get_device() != dev or qs[3] != 1:
-            raise ValueError(f"q must be {self.dtype} heads of {self.head_dim} on {self.device}, elements of a head adjacent")
-        places = _index(lens, "lens", (n,), dev)
-        if seqs is not None:
-            seqs = _index(seqs, "seqs", (n,), dev)
-        elif n > self._c.n_seqs:
-            raise ValueError(f"{n} requests, and a table of {self._c.n_seqs}")
-        out = self._out(q, out)
-        os = out.stride()
-        if len(os) == 3:
-            os = (0, *os) if starts else (os[0], 0, *os[1:])
-        lse = torch.empty(q.shape[:-1], dtype=_F32, device=self.device) if return_lse else None
-        need = self._need.get((nq, rows))
-        if need is None:
-            need = self._need[nq, rows] = self.lib.vp_paged_work_bytes(self.head_dim, nq, self.n_kv, rows)
-        work = self._work[0]
-        if work is None or work.numel() < need:
-            work = self._work[0] = torch.empty(max(need, WORK_ZEROED), dtype=torch.uint8, device=self.device)
-            work[:WORK_ZEROED].zero_()
-        _ATTN.pack_into(self._a, 0, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, places, seqs or 0, masks, starts,
-                        work.data_ptr(), work.numel(), qs[0], qs[1], qs[2], os[0], os[1], os[2],
-                        self.head_dim ** -0.5 if scale is None else scale, n, rows, nq, window, sinks)
-        rc = call(self._cp, self._ap, self._stream())
-        if rc:
-            check(rc, name)
-        return (out, lse) if return_lse else out
+        r = self._attend(True, self._at, self.device.index, self._work, q, lens, None, q_start, seqs, window, sinks, scale, out, return_lse)
+        return r if r.__class__ is not int else check(r, "vp_paged_prefill")
 
     def check(self) -> None:
         """Raises VpError if a call met a page or slot outside the table, or gave up a wait, since the last check();
