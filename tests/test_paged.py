@@ -464,6 +464,77 @@ def test_many_requests(kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [200, 1000, 2600])
+def test_very_many_short_requests(n):
+    """More requests than are sorted, than threads look at one each, than lengths are kept on the chip; every request checked
+    by its log sum exp and output at one row."""
+    rng = np.random.default_rng(n)
+    nq, nkv, hd, ps, dtype = 6, 2, 64, 16, torch.float16
+    lens = [int(x) for x in rng.integers(0, 40, n)]
+    lens[n // 2], lens[n - 1] = 700, 300
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, ps, dtype, fill=float("nan"))
+    ln = torch.tensor(lens, dtype=torch.int32).cuda()
+    one = torch.from_numpy(rng.standard_normal((n, 1, nq, hd)).astype(np.float32)).to(dtype)
+    ones = np.ones((n, 1), dtype=np.int64)
+
+    def near(got, masks, q, rows):
+        want = want_decode(q.double().numpy(), k, v, table, lens, masks, 0, 0, hd ** -0.5, ps)
+        compare(*got, [w for w in want if w[0][1] == rows - 1 and w[0][2] in (0, 5)], dtype, hd)
+
+    near(kv.decode(one.cuda(), ln, return_lse=True), ones, one, 1)
+    trees = torch.from_numpy(rng.standard_normal((n, 7, nq, hd)).astype(np.float32)).to(dtype)
+    chain = np.tile([(2 << r) - 1 for r in range(7)], (n, 1))
+    near(kv.decode(trees.cuda(), ln, return_lse=True), chain, trees, 7)
+    starts = torch.arange(n + 1, dtype=torch.int32).cuda() * 7
+    out, lse = kv.prefill(trees.view(-1, nq, hd).cuda(), starts, ln, return_lse=True)
+    near((out.view(n, 7, nq, hd), lse.view(n, 7, nq)), chain, trees, 7)
+    kv.check()
+
+
+@pytest.mark.gpu
+def test_prompt_rows_that_overlap_are_told():
+    """A q_start that runs backwards or past the rows: those requests are dropped or clipped, and check() tells it."""
+    rng = np.random.default_rng(2)
+    kv, *_ = make_cache(rng, [40, 40, 40], 2, 64, 16, torch.float16)
+    q = torch.zeros(40, 4, 64, dtype=torch.float16, device="cuda")
+    ln = torch.tensor([40, 40, 40], dtype=torch.int32).cuda()
+    for bad in ([0, 30, 20, 40], [0, 10, 20, 90], [-3, 10, 20, 40]):
+        kv.prefill(q, torch.tensor(bad, dtype=torch.int32).cuda(), ln)
+        with pytest.raises(_lib.VpError, match="slot"):
+            kv.check()
+    kv.prefill(q, torch.tensor([0, 10, 20, 40], dtype=torch.int32).cuda(), ln)
+    kv.check()
+
+
+@pytest.mark.gpu
+def test_prompts_left_over_for_a_last_round():
+    """As many equal blocks as leave a few over for a last round of the CTAs, against the oracle in sampled rows; the same bits
+    each time."""
+    rng = np.random.default_rng(12)
+    nq, nkv, hd, dtype, rows = 4, 1, 64, torch.float16, 256
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    n = (sms + 5) // 4 + 1  # four blocks of 256 packed rows each
+    lens = [int(x) for x in rng.integers(700, 900, n)]
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, 64, dtype, fill=float("nan"))
+    q = torch.from_numpy(rng.standard_normal((n * rows, nq, hd)).astype(np.float32)).to(dtype)
+    starts = torch.arange(n + 1, dtype=torch.int32).cuda() * rows
+    args = (q.cuda(), starts, torch.tensor(lens, dtype=torch.int32).cuda())
+    out, lse = kv.prefill(*args, return_lse=True)
+    for _ in range(5):
+        assert torch.equal(out, kv.prefill(*args))
+    kv.check()
+    want = []
+    for i in range(n):
+        for r in (0, 63, 64, 130, 255):
+            p = lens[i] - rows + r
+            ks, vs = (O.slots(x, table[i], p + 1) for x in (k, v))
+            for h in (0, 3):
+                t = i * rows + r
+                want.append(((t, h), O.attend(q[t, h].double().numpy(), ks[0], vs[0], np.ones(p + 1, dtype=bool), hd ** -0.5), p + 1))
+    compare(out, lse, want, dtype, hd)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("src,dtype", [(torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16),
                                        (torch.float32, torch.float16), (torch.float32, torch.bfloat16)])
 @pytest.mark.parametrize("nq,nkv,hd,rot,interleaved,layout", [(14, 2, 64, 64, False, "hnd"), (8, 2, 128, 128, True, "nhd"),
