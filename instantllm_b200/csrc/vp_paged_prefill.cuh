@@ -44,6 +44,7 @@ struct PfShape {
 };
 
 constexpr int PF_RECORDS = 640;            // records at most: four per SM, for 160
+constexpr int PF_AHEAD = 3;                // tiles of slots before a piece's end that the next piece is taken
 constexpr int PF_SORT = 128;               // requests that are sorted by length, at most
 constexpr int PF_JOIN = 8;                 // records joined at a time
 constexpr int PF_LEAST = 16;               // tiles of a piece, at least
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   unsigned char* qs = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   unsigned char* ring = qs + 2 * TILE;
   // of a buffer: its S is there, its weights are, its product into o is done; of a row tile: the piece's last product is
-  __shared__ uint64_t kv_full[SLOTS], kv_empty[SLOTS], s_full[BUFS], p_full[BUFS], o_done[BUFS], o_last[2], q_full, edge, drained, info_full[2], info_empty[2];
+  __shared__ uint64_t kv_full[SLOTS], kv_empty[SLOTS], s_full[BUFS], p_full[BUFS], o_done[BUFS], o_last[2], q_full, edge, drained, info_full[2], info_empty[2], wanted;
   __shared__ uint32_t tmem_base;
   __shared__ long long tile_sums[PF_THREADS / 32];
   __shared__ int sums[PF_THREADS / 32][2], starts[PF_THREADS], rec_starts[PF_THREADS], dead, last_s[2];
@@ -256,6 +257,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     mbar_init(&q_full, 9);  // the softmax warps and the issuer
     mbar_init(&edge, 1);
     mbar_init(&drained, 1);
+    mbar_init(&wanted, 1);
     fence_barrier_init();
     dead = 0;
   }
@@ -717,7 +719,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     for (int r = 0;; ++r) {
       if (r >= 2) wait_warp(&info_empty[r & 1], ((r >> 1) - 1) & 1);
       unsigned idx = blockIdx.x;
-      if (r > 0) {
+      if (r > 0) {  // taken when the last copies of the piece before are under way, not earlier: whoever is ahead takes more
+        wait_warp(&wanted, (r - 1) & 1);
         if (lane == 0) idx = gridDim.x + atomicAdd(next, 1u);
         idx = __shfl_sync(0xffffffffu, idx, 0);
       }
@@ -804,6 +807,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       // a request outside the table has no slots, and no page is looked up for it
       const int32_t* pages = c.table + table_row * c.table_stride;
       for (int j = 0; j < n_max; ++j) {
+        if (j == max(0, n_max - PF_AHEAD) && lane == 0) pg_arrive(&wanted);
         const int s0 = sp.at(j0 + j) * PF_TS, slot = s0 + lane * box;
         int page = c.n_pages;  // a box that nobody sees fills zeros
         if (lane < boxes && slot < see_end && (slot + box > see_lo || slot < a.sinks)) {
@@ -850,6 +854,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         }
         if (is_dead()) break;
       }
+      if (n_max == 0 && lane == 0) pg_arrive(&wanted);
     }
     // copies still in flight land before the CTA may end (they have, unless a wait ran out)
     for (uint32_t k = issued > SLOTS ? issued - SLOTS : 0; k < issued; ++k) mbar_wait_warp(&kv_full[k % SLOTS], (k / SLOTS) & 1);
