@@ -12,15 +12,22 @@
 // them as pairs) and both o (head_dim columns each). A unit is a row tile with a tile of slots; units go
 // round the buffers in order, first row tile, second row tile, next slots, so with three buffers the
 // next S of a row tile is there before its present weights are. A block of one row tile has both
-// warpgroups too: they take its tiles of slots in turns and join their two records at the end. One warp brings K and V tiles (TMA boxes of one page each), one thread
-// issues the products, and two warpgroups, one tile each and one row a thread, do the softmax: while
-// one of them works on its tile, the tensor cores work on the other's.
+// warpgroups too: they take its tiles of slots in turns and join their two records at the end. One warp
+// brings K and V tiles (TMA boxes of one page each), one thread issues the products, and two
+// warpgroups, one row a thread, do the softmax: while one of them works on its tile, the tensor
+// cores work on the other's.
 //
 // Work: one piece per (request, block, head), dealt out to one CTA per SM, the blocks with the most slots
 // first. Where that gives a CTA more than its share, a block's tiles are cut into pieces of about an
 // even share of all tiles (PF_LEAST at least); the pieces leave records in the work buffer and the
 // one that finishes last (a counter per row tile, back at zero afterwards) joins them in order. A
 // scheduler warp looks up the next piece, and its K and V arrive, while the present one is computed.
+//
+// Measured: a prompt of 8,192 rows, 32 + 2 x 8 heads of 128, bf16: 493 us, 1,116 TFLOP/s (67% of cuBLAS at bf16); of 64:
+// 388 us, where the exponentials alone are 50% of the tensor rate. 16 prompts of 186 to 2,048 rows, 14 + 2 x 2 heads of 64:
+// 85 us; one of 256: 11 us; 64 requests with 16 rows each over 151 to 2,064 slots: 27 us. A 256 x 128 tile of scores
+// takes 1.76 us at head_dim 64 (load and maximum 0.37, exponentials of both warpgroups 1.1, next S 0.25) and 2.25 at 128
+// (0.37, 0.83, then its own two products 0.55 and 0.45 to be told).
 #pragma once
 #include "vp_paged_decode.cuh"
 
@@ -44,10 +51,12 @@ struct PfShape {
 };
 
 constexpr int PF_RECORDS = 640;            // records at most: four per SM, for 160
-constexpr int PF_AHEAD = 3;                // tiles of slots before a piece's end that the next piece is taken
-constexpr int PF_SORT = 128;               // requests that are sorted by length, at most
-constexpr int PF_JOIN = 8;                 // records joined at a time
-constexpr int PF_LEAST = 16;               // tiles of a piece, at least
+constexpr int PF_AHEAD = 3;                // tiles of slots before a piece's end that the next piece is taken (two pieces
+                                           // ahead: 4,096 rows 79 us instead of 62, as the CTAs no longer even out)
+constexpr int PF_SORT = 128;               // requests that are sorted by length, at most (16 prompts: 100 us unsorted, 90
+                                           // sorted; the sort is n steps a thread, 0.5 us at 128)
+constexpr int PF_JOIN = 8;                 // records joined at a time (16 rows over 60,000 slots: 50 us, all 74 at once 68)
+constexpr int PF_LEAST = 16;               // tiles of a piece, at least (64 trees: 26.7 us; with 8, whose joins cost what they save: 28.3)
 
 struct PfParams {
   vp_paged c;
@@ -358,6 +367,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   };
   auto is_dead = [&] { return *(volatile int*)&dead != 0; };
 
+  if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_OTHER_REGS));
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PF_SOFTMAX_REGS));
     // ---- softmax: warpgroup i has row tile i (or every other tile of slots), a thread row f ----
@@ -710,9 +720,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       }
       pf_fence_before();
     }
-  } else {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_OTHER_REGS));
-  if (warp == PF_SCHEDULER) {
+  } else if (warp == PF_SCHEDULER) {
     // ---- the CTA's pieces: one for each CTA, then whoever comes first has the next, from the last request's
     // last block on. Which CTA has a piece does not show in the results. ----
     unsigned* next = p.tickets + 4 * PF_RECORDS;  // and the number of CTAs that have come to the end
@@ -942,7 +950,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     if (lead) pf_commit(&drained);
     mbar_wait_warp(&drained, 0);
     pf_fence_before();
-  }
   }
   cta_sync();
   pf_fence_after();
