@@ -19,7 +19,7 @@
 //    joins them in the order of the slots, so results do not depend on which CTA that is.
 // Measured: 4 requests of 103,871 to 131,072 slots, 32 + 2 x 8 heads of 128, bf16: 267 us, 6.9 TB/s (a plain copy: 6.5;
 // with a producer warp filling a ring for all warps: 430 us). 64 requests of 130 to 2,048 slots, 14 + 2 x 2 heads of
-// 64: 14.9 us; 128 requests with a window of 1,024: 23 us; one request of 257 slots: 6.2 us, of which 2.4 us pass before
+// 64: 14.9 us; 128 requests with a window of 1,024: 20 us; one request of 257 slots: 6.7 us, of which 2.9 us pass before
 // the first tile is asked for (lengths, shares, pages), 0.9 until it is there, 0.65 a tile, 0.8 for the join.
 #pragma once
 #include "vp_paged.cuh"
@@ -35,6 +35,7 @@ constexpr int DC_ROWS = 16;
 constexpr int DC_TILE = 4096;                       // bytes of K (and of V) per tile
 constexpr int DC_STAGES = 2;                        // per warp
 constexpr int DC_LENS = 2048;                       // lengths kept in shared memory
+constexpr int DC_SHORT = 64;                        // tiles of a CTA's share, at most, for whole pairs
 
 template <int HD>
 struct DcShape {
@@ -167,8 +168,8 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
   float2* join_ml = reinterpret_cast<float2*>(join + DC_WARPS * DC_ROWS * PITCH);
   int* lens_s = reinterpret_cast<int*>(join_ml + DC_WARPS * DC_ROWS);
   __shared__ uint64_t full[DC_WARPS][DC_STAGES], q_full[2];
-  __shared__ int warp_sums[DC_THREADS / 32];
-  __shared__ int first_seq, first_tile, dead, last_flag;  // first_tile: number of first_seq's first tile
+  __shared__ int warp_sums[DC_THREADS / 32], warp_most[DC_THREADS / 32], warp_least[DC_THREADS / 32];
+  __shared__ int first_seq, first_tile, t0_s, t1_s, dead, last_flag;  // first_tile: number of first_seq's first tile
 
   const vp_paged& c = p.c;
   const vp_paged_attn& a = p.a;
@@ -190,44 +191,81 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
   // tiles of all requests: every thread counts a run of them, then a scan over the CTA
   const int chunk = (a.n + DC_THREADS - 1) / DC_THREADS;
   const int i0 = min(a.n, tid * chunk), i1 = min(a.n, i0 + chunk);
-  int mine = 0;
+  int mine = 0, most = 0, least = 1 << 30;
   for (int i = i0; i < i1; ++i) {
     const int len = pg_seq(c, a.seqs, a.lens, i).len;
     if (i < DC_LENS) lens_s[i] = len;
-    mine += dc_span<TS>(len, rows, a.window, a.sinks).tiles * c.n_kv;
+    const int tiles = dc_span<TS>(len, rows, a.window, a.sinks).tiles;
+    mine += tiles * c.n_kv;
+    most = max(most, tiles);
+    least = min(least, tiles);
   }
+  most = __reduce_max_sync(0xffffffffu, most);
+  least = __reduce_min_sync(0xffffffffu, least);
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) warp_sums[warp] = incl;
+  if (lane == 31) warp_sums[warp] = incl, warp_most[warp] = most, warp_least[warp] = least;
   cta_sync();
   int before = 0, N = 0;
 #pragma unroll
   for (int w = 0; w < DC_THREADS / 32; ++w) {
     if (w < warp) before += warp_sums[w];
     N += warp_sums[w];
+    most = max(most, warp_most[w]);
+    least = min(least, warp_least[w]);
   }
-  const int G = min((N + p.min_tiles - 1) / p.min_tiles, (int)gridDim.x), cta = blockIdx.x;
+  // Even shares of the tiles; or, where the requests are about equally long and the shares small, whole pairs
+  // (cuts == 1) or even cuts of them: a pair that ends inside a CTA's share costs a join (16 requests of 300
+  // slots: 7.5 us, 11.8 with even shares; 64 of 1,000: 11.4 and 14.5; 128 with a window of 1,024: 20.4 and 22.9).
+  const int cta = blockIdx.x, pairs = a.n * c.n_kv;
+  int G = min((N + p.min_tiles - 1) / p.min_tiles, (int)gridDim.x), cuts = 0;
+  if (4ll * most <= 5ll * least && N <= DC_SHORT * (int)gridDim.x) {
+    cuts = 2 * pairs > (int)gridDim.x ? 1 : min((int)gridDim.x / pairs, (most + p.min_tiles - 1) / p.min_tiles);
+    G = min((int)gridDim.x, pairs * cuts);
+  }
   if (cta >= G) return;
-  const PgShare share(N, G);
-  const int t0 = share.first(cta), t1 = share.first(cta + 1);
+  const PgShare share(cuts ? pairs : N, G);  // of tiles, or of pairs
   int at = before + incl - mine;
-  if (at <= t0 && t0 < at + mine) {
+  if (!cuts) {
+    const int t = share.first(cta);
+    if (tid == 0) t0_s = t, t1_s = share.first(cta + 1);
+    if (at <= t && t < at + mine) {
+      for (int i = i0; i < i1; ++i) {
+        const int len = i < DC_LENS ? lens_s[i] : pg_seq(c, a.seqs, a.lens, i).len;
+        const int n = dc_span<TS>(len, rows, a.window, a.sinks).tiles * c.n_kv;
+        if (t < at + n) {
+          first_seq = i;
+          first_tile = at;
+          break;
+        }
+        at += n;
+      }
+    }
+  } else {
+    const int q0 = cuts == 1 ? share.first(cta) : cta / cuts, q1 = cuts == 1 ? share.first(cta + 1) : q0 + 1;
+    const int s0 = q0 / c.n_kv, s1 = q1 / c.n_kv;  // their requests
+    if (cuts == 1 && tid == 0 && s1 == a.n) t1_s = N;
+    __syncwarp();
     for (int i = i0; i < i1; ++i) {
       const int len = i < DC_LENS ? lens_s[i] : pg_seq(c, a.seqs, a.lens, i).len;
-      const int n = dc_span<TS>(len, rows, a.window, a.sinks).tiles * c.n_kv;
-      if (t0 < at + n) {
+      const int tiles = dc_span<TS>(len, rows, a.window, a.sinks).tiles;
+      if (i == s0) {
+        const int t = at + (q0 - s0 * c.n_kv) * tiles, k = cuts == 1 ? 0 : cta - q0 * cuts;
         first_seq = i;
         first_tile = at;
-        break;
+        t0_s = t + k * tiles / cuts;
+        if (cuts > 1) t1_s = t + (k + 1) * tiles / cuts;
       }
-      at += n;
+      if (cuts == 1 && i == s1) t1_s = at + (q1 - s1 * c.n_kv) * tiles;
+      at += tiles * c.n_kv;
     }
   }
   cta_sync();
+  const int t0 = t0_s, t1 = t1_s;
 
   // Waits of a whole warp; after one that ran out none waits any more, and the call ends with an error status.
   auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -514,7 +552,8 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
     }
     if (more) dc_arrive(DC_FREE);  // the warps come for it before each further run
     if (alone) continue;
-    const int c0 = share.owner(pair_at), c1 = share.owner(pair_at + tiles - 1);
+    const int c0 = cuts ? (seq * c.n_kv + head) * cuts : share.owner(pair_at);
+    const int c1 = cuts ? c0 + cuts - 1 : share.owner(pair_at + tiles - 1);
     __threadfence();
     __syncwarp();
     asm volatile("barrier.sync 1, 128;" ::: "memory");

@@ -464,6 +464,24 @@ def test_many_requests(kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,length,hd,nkv", [(1, 1500, 64, 2), (3, 2000, 128, 2), (20, 700, 64, 2), (73, 300, 64, 2), (75, 333, 64, 2), (160, 90, 128, 1),
+                                              (300, 50, 64, 3)])
+def test_decode_of_equally_long_requests(n, length, hd, nkv):
+    """About equal lengths: requests cut evenly, one pair of request and head a CTA, several of them."""
+    rng = np.random.default_rng(n)
+    nq, ps, dtype = 3 * nkv, 16, torch.float16
+    lens = [int(x) for x in rng.integers(length - length // 20, length + 1, n)]
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, ps, dtype, fill=float("nan"))
+    q = torch.from_numpy(rng.standard_normal((n, 1, nq, hd)).astype(np.float32)).to(dtype)
+    ln = torch.tensor(lens, dtype=torch.int32).cuda()
+    out, lse = kv.decode(q.cuda(), ln, return_lse=True)
+    for _ in range(5):
+        assert torch.equal(out, kv.decode(q.cuda(), ln))
+    kv.check()
+    compare(out, lse, want_decode(q.double().numpy(), k, v, table, lens, np.ones((n, 1), dtype=np.int64), 0, 0, hd ** -0.5, ps), dtype, hd)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [200, 1000, 2600])
 def test_very_many_short_requests(n):
     """More requests than are sorted, than threads look at one each, than lengths are kept on the chip; every request checked
