@@ -22,7 +22,7 @@ TORCH_OUT = PKG / "_paged.so"
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-shared", "-Xcompiler", "-fPIC", "--threads", "4",
     # no --use_fast_math: the pass must be shape-invariant and close to the fp32 reference
 ]
 

@@ -90,6 +90,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     want(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes() && k.scalar_type() == in && v.scalar_type() == in,
          "q, k and v must be [rows][heads][head_dim] of one type");
     const int64_t n = q.size(0);
+    want(n <= 0x7fffffff, "too many rows");
     want(q.size(2) == c.head_dim && k.size(0) == n && k.size(1) == c.n_kv && k.size(2) == c.head_dim,
          "expected k and v of " + std::to_string(n) + " rows and " + std::to_string(c.n_kv) + " heads of " + std::to_string(c.head_dim));
     want(in == call.type || in == at::kFloat, "rows must have the cache's type or fp32");
@@ -143,6 +144,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
          "q must have the cache's type, device and head_dim, elements of a head adjacent");
     want(lens.dim() == 1, "lens must be one-dimensional");
     const int64_t n = prompts ? lens.size(0) : q.size(0), rows = prompts ? q.size(0) : one ? 1 : q.size(1);
+    want(n < 0x7fffffff && rows <= 0x7fffffff, "too many rows");
     vp_paged_attn t{};
     t.lens = call.index(a[5], "lens", {n});
     t.mask = call.index(a[6], "mask", {n, rows}, true);

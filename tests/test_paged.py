@@ -117,6 +117,16 @@ def test_layer_wants_cuda_pools():
         paged.PagedLayer(k, k[:, :1], torch.zeros(1, 2, dtype=torch.int32))
 
 
+def test_extension_builds_and_refuses(lib):
+    """The tensor side builds against the installed torch, loads beside the library and refuses a wrong call (no GPU)."""
+    build.build_torch()
+    from instantllm_b200 import _paged
+
+    for call in (_paged.append, _paged.attend):
+        with pytest.raises(ValueError, match="arguments"):
+            call(1)
+
+
 def test_page_pool():
     p = paged.PagePool(6, 16, 3, 4)
     assert p.reserve(0, 17) == (0, [0, 1])
