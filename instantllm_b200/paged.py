@@ -56,8 +56,8 @@ def ancestor_masks(trees) -> torch.Tensor:
 class PagedLayer:
     """One layer of a paged cache. k, v: [pages][heads][page_size][head_dim] in fp16 or bf16, elements of a slot adjacent, any
     strides in multiples of 8 elements (a [pages][page_size][heads][head_dim] pool transposed will do), the same for both;
-    table: int32 [requests][pages per request]. status: int32 [1] and work (uint8, zeroed) may be shared between layers that
-    run on one stream."""
+    table: int32 [requests][pages per request]. status (int32 [1]) and work (a list of one entry, the workspace or None) may be
+    shared between layers that run on one stream."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, status: Optional[torch.Tensor] = None,
                  work: Optional[list] = None):

@@ -535,6 +535,23 @@ def test_prompt_rows_that_overlap_are_told():
 
 
 @pytest.mark.gpu
+def test_c_entry_ignores_what_a_prompt_call_has_not():
+    """vp_paged_prefill through the C ABI alone: the fields of a decode call (request strides, masks) hold anything."""
+    rng = np.random.default_rng(8)
+    kv, k, v, table = make_cache(rng, [50, 20], 2, 64, 16, torch.float16)
+    q = torch.from_numpy(rng.standard_normal((60, 4, 64)).astype(np.float32)).half().cuda()
+    ln, starts = torch.tensor([50, 20], dtype=torch.int32).cuda(), torch.tensor([0, 45, 60], dtype=torch.int32).cuda()
+    want = kv.prefill(q, starts, ln)
+    lib, out = _lib.load(), torch.zeros_like(q)
+    work = torch.zeros(lib.vp_paged_work_bytes(64, 4, 2, 60), dtype=torch.uint8, device="cuda")
+    a = _lib.VpPagedAttn(q.data_ptr(), out.data_ptr(), None, ln.data_ptr(), None, 4096, starts.data_ptr(), work.data_ptr(), work.numel(),
+                         8 * 10 ** 9, 256, 64, -8 * 10 ** 9, 256, 64, 0.125, 2, 60, 4, 0, 0)
+    _lib.check(lib.vp_paged_prefill(ctypes.addressof(kv._c), ctypes.addressof(a), torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
 def test_prompts_left_over_for_a_last_round():
     """As many equal blocks as leave a few over for a last round of the CTAs, against the oracle in sampled rows; the same bits
     each time."""
