@@ -9,7 +9,7 @@
 // (length, page, K, V). So the query rows of one cache head (G heads x R rows, packed as m = r G + g)
 // share one read of the cache, and the work is cut into tiles of 8 KB (32 slots of 64, 16 of 128)
 // dealt out evenly: the tiles of all (request, head) pairs are numbered in order and every CTA takes
-// the same number of consecutive ones. One CTA per SM, two roles:
+// about the same number of consecutive ones. One CTA per SM, two roles:
 //  * eight consumer warps take turns over the tiles. Each has two stages of its own and refills a
 //    stage itself (TMA boxes of one page each) once it has computed on it (mma.sync), so the warps never
 //    wait for one another;
@@ -19,7 +19,7 @@
 //    joins them in the order of the slots, so results do not depend on which CTA that is.
 // Measured: 4 requests of 103,871 to 131,072 slots, 32 + 2 x 8 heads of 128, bf16: 267 us, 6.9 TB/s (a plain copy: 6.5;
 // with a producer warp filling a ring for all warps: 430 us). 64 requests of 130 to 2,048 slots, 14 + 2 x 2 heads of
-// 64: 14.9 us; 128 requests with a window of 1,024: 20 us; one request of 257 slots: 6.7 us, of which 2.9 us pass before
+// 64: 13.3 us; 128 requests with a window of 1,024: 20 us; one request of 257 slots: 6.7 us, of which 2.9 us pass before
 // the first tile is asked for (lengths, shares, pages), 0.9 until it is there, 0.65 a tile, 0.8 for the join.
 #pragma once
 #include "vp_paged.cuh"
@@ -35,6 +35,10 @@ constexpr int DC_ROWS = 16;
 constexpr int DC_TILE = 4096;                       // bytes of K (and of V) per tile
 constexpr int DC_STAGES = 2;                        // per warp
 constexpr int DC_LENS = 2048;                       // lengths kept in shared memory
+// Tiles that a run costs beside its own, in the even shares (64 requests of 130 to 2,048 slots: 13.3 us, 15.2 without,
+// 12.7 with 10, 14.2 with 24; 200 of 20 to 4,000: 25.6, 40, 26.7, 27.8; 30 of 100 to 4,000, 32 + 2 x 8 heads of 128:
+// 33, 53, 35, 35).
+constexpr int DC_RUN = 12;
 constexpr int DC_SHORT = 64;                        // tiles of a CTA's share, at most, for whole pairs
 
 template <int HD>
@@ -108,7 +112,6 @@ __device__ __forceinline__ void dc_sync(int bar) {
   asm volatile("barrier.sync %0, 384;" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void dc_arrive(int bar) {
-  __threadfence_block();
   __syncwarp();
   asm volatile("barrier.arrive %0, 384;" ::"r"(bar) : "memory");
 }
@@ -228,22 +231,29 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
     G = min((int)gridDim.x, pairs * cuts);
   }
   if (cta >= G) return;
-  const PgShare share(cuts ? pairs : N, G);  // of tiles, or of pairs
+  // A run of tiles of one pair costs about as much as DC_RUN tiles more, so shares are even in tiles and DC_RUN
+  // for each pair, which stand before its tiles in this count.
+  const PgShare share(cuts ? pairs : N + DC_RUN * pairs, G);  // of tiles, or of pairs
   int at = before + incl - mine;
   if (!cuts) {
-    const int t = share.first(cta);
-    if (tid == 0) t0_s = t, t1_s = share.first(cta + 1);
-    if (at <= t && t < at + mine) {
-      for (int i = i0; i < i1; ++i) {
-        const int len = i < DC_LENS ? lens_s[i] : pg_seq(c, a.seqs, a.lens, i).len;
-        const int n = dc_span<TS>(len, rows, a.window, a.sinks).tiles * c.n_kv;
-        if (t < at + n) {
-          first_seq = i;
-          first_tile = at;
-          break;
-        }
-        at += n;
+    const int v0 = share.first(cta), v1 = share.first(cta + 1);
+    if (tid == 0 && cta + 1 == G) t1_s = N;
+    __syncwarp();
+    for (int i = i0, v = at + DC_RUN * c.n_kv * i0; i < i1; ++i) {
+      const int len = i < DC_LENS ? lens_s[i] : pg_seq(c, a.seqs, a.lens, i).len;
+      const int tiles = dc_span<TS>(len, rows, a.window, a.sinks).tiles, width = tiles + DC_RUN, end = v + width * c.n_kv;
+      auto tile_at = [&](int x) {  // tiles before place x of the count
+        const int h = (x - v) / width;
+        return at + h * tiles + max(0, x - v - h * width - DC_RUN);
+      };
+      if (v <= v0 && v0 < end) {
+        first_seq = i;
+        first_tile = at;
+        t0_s = tile_at(v0);
       }
+      if (v <= v1 && v1 < end) t1_s = tile_at(v1);
+      at += tiles * c.n_kv;
+      v = end;
     }
   } else {
     const int q0 = cuts == 1 ? share.first(cta) : cta / cuts, q1 = cuts == 1 ? share.first(cta + 1) : q0 + 1;
@@ -266,6 +276,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
   }
   cta_sync();
   const int t0 = t0_s, t1 = t1_s;
+  if (t0 == t1) return;
 
   // Waits of a whole warp; after one that ran out none waits any more, and the call ends with an error status.
   auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -552,8 +563,8 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
     }
     if (more) dc_arrive(DC_FREE);  // the warps come for it before each further run
     if (alone) continue;
-    const int c0 = cuts ? (seq * c.n_kv + head) * cuts : share.owner(pair_at);
-    const int c1 = cuts ? c0 + cuts - 1 : share.owner(pair_at + tiles - 1);
+    const int pair = seq * c.n_kv + head, place = pair_at + DC_RUN * (pair + 1);  // of the pair's first tile
+    const int c0 = cuts ? pair * cuts : share.owner(place), c1 = cuts ? c0 + cuts - 1 : share.owner(place + tiles - 1);
     __threadfence();
     __syncwarp();
     asm volatile("barrier.sync 1, 128;" ::: "memory");

@@ -164,7 +164,7 @@ int decode_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
   p.group = a.n_q / c.n_kv;
   p.M = p.group * a.rows;
   // a CTA's ring: all of it flies at once (one request of 257 slots: 6.2 us; 10.4 with half as many, which split its heads,
-  // 8.5 with twice as many; 64 requests of 130 to 2,048: 14.8, 14.8 and 17.6)
+  // 8.5 with twice as many; 64 requests of 130 to 2,048: 14.8, 14.8 and 17.6 in even shares of tiles)
   p.min_tiles = DC_WARPS * DC_STAGES;
   p.page_shift = __builtin_ctz(c.page_size);
   p.tickets = static_cast<unsigned*>(a.work);
@@ -174,8 +174,8 @@ int decode_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
   int sms = 0;
   if (const int e = sm_count(&sms)) return e;
   const int tiles = (int)(((long long)c.max_pages * c.page_size + Sh::TS - 1) / Sh::TS);
-  const long long most = (long long)a.n * c.n_kv * tiles;
-  if (most > 0x7fffffff) return pfail(VP_ERR_ARG, "more slots than a launch holds");
+  const long long pairs = (long long)a.n * c.n_kv, most = pairs * tiles;
+  if (most + DC_RUN * pairs > 0x7fffffff) return pfail(VP_ERR_ARG, "more slots than a launch holds");
   return pg_launch("vp_paged_decode", k_paged_decode<T, HD>, (unsigned)(most < sms ? most : sms), DC_THREADS, Sh::SMEM, st, p, mk, mv);
 }
 
