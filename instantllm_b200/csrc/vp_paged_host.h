@@ -63,6 +63,14 @@ int check_attn(const vp_paged* c, const vp_paged_attn* a) {
   return VP_OK;
 }
 
+// A window past every position is none, and sinks past every position are all: the kernels subtract positions from them.
+vp_paged_attn in_range(const vp_paged_attn& a) {
+  vp_paged_attn t = a;
+  if (t.window > (1 << 30)) t.window = 0;
+  if (t.sinks > (1 << 30)) t.sinks = 1 << 30;
+  return t;
+}
+
 // Launches a kernel whose prologue may run while the kernel before it in the stream ends
 // (griddepcontrol.wait in the kernel stands before its first access to global memory).
 template <typename... P, typename... A>

@@ -221,13 +221,11 @@ int vp_paged_decode(const vp_paged* c, const vp_paged_attn* a, void* stream) try
   if (a->rows > PG_MAX_ROWS) return pfail(VP_ERR_ARG, "a decode call takes 1 to 16 rows per request");
   if (a->n == 0 || a->rows == 0) return VP_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->n_q / c->n_kv * a->rows > DC_ROWS) {
-    vp_paged_attn t = *a;
-    t.q_start = nullptr;
-    return pg_tiles(*c, t, st);
-  }
-  if (c->type == VP_T_F16) return c->head_dim == 64 ? decode_launch<__half, 64>(*c, *a, st) : decode_launch<__half, 128>(*c, *a, st);
-  return c->head_dim == 64 ? decode_launch<__nv_bfloat16, 64>(*c, *a, st) : decode_launch<__nv_bfloat16, 128>(*c, *a, st);
+  vp_paged_attn t = in_range(*a);
+  t.q_start = nullptr;
+  if (a->n_q / c->n_kv * a->rows > DC_ROWS) return pg_tiles(*c, t, st);
+  if (c->type == VP_T_F16) return c->head_dim == 64 ? decode_launch<__half, 64>(*c, t, st) : decode_launch<__half, 128>(*c, t, st);
+  return c->head_dim == 64 ? decode_launch<__nv_bfloat16, 64>(*c, t, st) : decode_launch<__nv_bfloat16, 128>(*c, t, st);
 } catch (const std::exception&) {
   return VP_ERR_NOMEM;
 }

@@ -58,7 +58,7 @@ extern "C" int vp_paged_prefill(const vp_paged* c, const vp_paged_attn* a, void*
   if (const int e = check_attn(c, a)) return e;
   if (a->n == 0 || a->rows == 0) return VP_OK;
   if (!a->q_start) return pfail(VP_ERR_ARG, "null q_start");
-  vp_paged_attn t = *a;  // what only a decode call has is not looked at
+  vp_paged_attn t = in_range(*a);  // what only a decode call has is not looked at
   t.q_seq = t.out_seq = 0;
   t.mask = nullptr;
   return pg_tiles(*c, t, static_cast<cudaStream_t>(stream));

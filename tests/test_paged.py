@@ -535,6 +535,22 @@ def test_prompt_rows_that_overlap_are_told():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks", [(2 ** 31 - 1, 2 ** 31 - 1), (2 ** 31 - 1, 0), (3, 2 ** 31 - 1), (2 ** 62, 2 ** 62)])
+def test_windows_and_sinks_past_everything(window, sinks):
+    """They are as none, and as all, also where a request is shorter than its new rows."""
+    rng = np.random.default_rng(9)
+    kv, *_ = make_cache(rng, [300, 3, 17], 2, 64, 16, torch.float16, fill=float("nan"))
+    ln = torch.tensor([300, 3, 17], dtype=torch.int32).cuda()
+    for rows, nq in ((5, 4), (16, 14)):
+        q = torch.from_numpy(rng.standard_normal((3, rows, nq, 64)).astype(np.float32)).half().cuda()
+        assert torch.equal(kv.decode(q, ln, window=window, sinks=sinks), kv.decode(q, ln))
+        starts = torch.arange(4, dtype=torch.int32).cuda() * rows
+        flat = q.view(-1, nq, 64)
+        assert torch.equal(kv.prefill(flat, starts, ln, window=window, sinks=sinks), kv.prefill(flat, starts, ln))
+    kv.check()
+
+
+@pytest.mark.gpu
 def test_c_entry_ignores_what_a_prompt_call_has_not():
     """vp_paged_prefill through the C ABI alone: the fields of a decode call (request strides, masks) hold anything."""
     rng = np.random.default_rng(8)
