@@ -39,7 +39,9 @@ constexpr int DC_LENS = 2048;                       // lengths kept in shared me
 // 12.7 with 10, 14.2 with 24; 200 of 20 to 4,000: 25.6, 40, 26.7, 27.8; 30 of 100 to 4,000, 32 + 2 x 8 heads of 128:
 // 33, 53, 35, 35).
 constexpr int DC_RUN = 12;
-constexpr int DC_SHORT = 64;                        // tiles of a CTA's share, at most, for whole pairs
+// Tiles of a CTA's share, at most, for whole pairs: past it the joins they save cost less than CTAs without a last pair
+// (32 + 2 x 8 heads of 128, 40 requests of 2,000 slots: 57 us, 70 with whole pairs; 16 of 16,000: 159 and 168).
+constexpr int DC_SHORT = 64;
 
 template <int HD>
 struct DcShape {
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
   }
   // Even shares of the tiles; or, where the requests are about equally long and the shares small, whole pairs
   // (cuts == 1) or even cuts of them: a pair that ends inside a CTA's share costs a join (16 requests of 300
-  // slots: 7.5 us, 11.8 with even shares; 64 of 1,000: 11.4 and 14.5; 128 with a window of 1,024: 20.4 and 22.9).
+  // slots: 7.3 us, 11.3 with even shares; 64 of 1,000: 11.3 and 14.4; 128 with a window of 1,024: 20.4 and 22.7).
   const int cta = blockIdx.x, pairs = a.n * c.n_kv;
   int G = min((N + p.min_tiles - 1) / p.min_tiles, (int)gridDim.x), cuts = 0;
   if (4ll * most <= 5ll * least && N <= DC_SHORT * (int)gridDim.x) {
