@@ -16,10 +16,11 @@
 //  * four joiner warps bring the queries of the next pair, and at the end of a pair's run add up the
 //    warps' records while the warps are on the next pair. A pair that several CTAs share leaves records
 //    in the work buffer; the CTA that finishes last (a counter per first CTA, back at zero afterwards)
-//    joins them in the order of the slots, so results do not depend on which CTA that is.
+//    joins them in the order of the slots, so results do not depend on which CTA that is. Of many records,
+//    each eight are first joined by the last CTA of those, in the buffer that the warps' records were in.
 // Measured: 4 requests of 103,871 to 131,072 slots, 32 + 2 x 8 heads of 128, bf16: 267 us, 6.9 TB/s (a plain copy: 6.5;
 // with a producer warp filling a ring for all warps: 430 us). 64 requests of 130 to 2,048 slots, 14 + 2 x 2 heads of
-// 64: 13.3 us; 128 requests with a window of 1,024: 20 us; one request of 257 slots: 6.7 us, of which 2.9 us pass before
+// 64: 12.8 us; 128 requests with a window of 1,024: 20 us; one request of 257 slots: 6.7 us, of which 2.9 us pass before
 // the first tile is asked for (lengths, shares, pages), 0.9 until it is there, 0.65 a tile, 0.8 for the join.
 #pragma once
 #include "vp_paged.cuh"
@@ -35,13 +36,18 @@ constexpr int DC_ROWS = 16;
 constexpr int DC_TILE = 4096;                       // bytes of K (and of V) per tile
 constexpr int DC_STAGES = 2;                        // per warp
 constexpr int DC_LENS = 2048;                       // lengths kept in shared memory
-// Tiles that a run costs beside its own, in the even shares (64 requests of 130 to 2,048 slots: 13.3 us, 15.2 without,
+// Tiles that a run costs beside its own, in the even shares (64 requests of 130 to 2,048 slots: 13.3 us then, 15.2 without,
 // 12.7 with 10, 14.2 with 24; 200 of 20 to 4,000: 25.6, 40, 26.7, 27.8; 30 of 100 to 4,000, 32 + 2 x 8 heads of 128:
 // 33, 53, 35, 35).
 constexpr int DC_RUN = 12;
 // Tiles of a CTA's share, at most, for whole pairs: past it the joins they save cost less than CTAs without a last pair
 // (32 + 2 x 8 heads of 128, 40 requests of 2,000 slots: 57 us, 70 with whole pairs; 16 of 16,000: 159 and 168).
 constexpr int DC_SHORT = 64;
+// Rounds of reads (8 records, 128 items of 4 elements), at most, in which the last CTA joins a pair's records by itself;
+// more records go eight at a time. 16 records of 4 rows of 128: 11.1 us a call, 13.1 by eights; 18 of 7 rows of 64 (3 rounds):
+// 21.1 and 22.4; 18 of 16 rows of 128 (12 rounds): 23.7 by eights, 29 otherwise; 50 of 8 rows of 128 (14): 14.9 and 22.
+constexpr int DC_FLAT = 3;
+constexpr int DC_LEVELS = 3;                        // of joins that leave a record: 8^3 parts a pair, more than CTAs
 
 template <int HD>
 struct DcShape {
@@ -53,14 +59,14 @@ struct DcShape {
   static constexpr size_t SMEM = 1024 + RING + 2 * QBUF + JOIN + DC_WARPS * DC_ROWS * 8 + DC_LENS * 4;
 };
 
-// Floats of one record of `rows` rows: o, then m, then l; a multiple of 16 bytes.
+// Floats of one record of `rows` rows: o, then (m, l) of each row; a multiple of 16 bytes.
 __host__ __device__ constexpr size_t pg_record(int rows, int hd) { return ((size_t)rows * (hd + 2) + 3) / 4 * 4; }
 
 struct DcParams {
   vp_paged c;
   vp_paged_attn a;
-  float* rec;         // [grid][2] records of M rows
-  unsigned* tickets;  // [grid]
+  float* rec;         // [grid][DC_LEVELS][2] records of M rows
+  unsigned* tickets;  // [grid][DC_LEVELS][2]
   int group, M, min_tiles, page_shift;  // G, G R, fewest tiles per CTA, log2 of the page size
 };
 
@@ -522,6 +528,24 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
     *reinterpret_cast<uint2*>(out) = v;
     if (a.lse && d == 0) a.lse[((long long)seq * rows + row) * a.n_q + h] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
   };
+  // Records of a CTA's part of a pair (level 0), and of the parts from it on that were joined first and second. A CTA has at most one pair that begins
+  // in it and ends elsewhere, and one that began elsewhere.
+  auto record = [&](int cc, bool begins, int level) { return p.rec + (size_t)(2 * DC_LEVELS * cc + 2 * level + begins) * rec_floats; };
+  // Whether this CTA is the last of n whose records are out; the counter is back at zero then. The barriers carry the
+  // order of one thread's atomic to the others' records.
+  auto last = [&](unsigned* ticket, int n) {
+    __syncwarp();
+    asm volatile("barrier.sync 1, 128;" ::: "memory");
+    if (jt == 0) {
+      unsigned before;
+      asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(ticket) : "memory");
+      last_flag = before == (unsigned)(n - 1);
+      if (last_flag) *ticket = 0;
+    }
+    __syncwarp();
+    asm volatile("barrier.sync 1, 128;" ::: "memory");
+    return last_flag != 0;
+  };
   DcWalk<TS> w(p, lens_s, first_seq, first_tile, t0, t1);
   queries(w.seq, w.head, 0);
   bool more = true;
@@ -531,79 +555,97 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
     w.advance(n);
     more = w.more();
     if (more) queries(w.seq, w.head, r + 1);  // the warps are done with the queries of run r - 1
-    float* rec = p.rec + (size_t)(u0 == 0 ? 2 * cta + 1 : 2 * cta) * rec_floats;
-    dc_sync(DC_FILLED);
-    // item: row m, 4 elements
-    for (int it = jt; it < p.M * (HD / 4); it += DC_JOINERS) {
-      const int m = it / (HD / 4), d = it % (HD / 4) * 4;
-      float2 ml[DC_WARPS];
-      float top = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < DC_WARPS; ++k) {
-        ml[k] = join_ml[k * DC_ROWS + m];
-        top = fmaxf(top, ml[k].x);
-      }
-      const float use = top == -INFINITY ? 0.f : top;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      float l = 0.f;
-#pragma unroll
-      for (int k = 0; k < DC_WARPS; ++k) {
-        const float f = pg_exp2(ml[k].x - use);
-        const float4 v = *reinterpret_cast<const float4*>(join + (k * DC_ROWS + m) * PITCH + d);
-        l += ml[k].y * f;
-        acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
-      }
-      if (alone) {
-        put(seq, head, m, d, top, l, acc);
-      } else {
-        *reinterpret_cast<float4*>(rec + (size_t)m * HD + d) = acc;
-        if (d == 0) {
-          rec[(size_t)p.M * HD + m] = top;
-          rec[(size_t)p.M * (HD + 1) + m] = l;
-        }
-      }
-    }
-    if (more) dc_arrive(DC_FREE);  // the warps come for it before each further run
-    if (alone) continue;
     const int pair = seq * c.n_kv + head, place = pair_at + DC_RUN * (pair + 1);  // of the pair's first tile
-    const int c0 = cuts ? pair * cuts : share.owner(place), c1 = cuts ? c0 + cuts - 1 : share.owner(place + tiles - 1);
-    __threadfence();
-    __syncwarp();
-    asm volatile("barrier.sync 1, 128;" ::: "memory");
-    if (jt == 0) last_flag = atomicAdd(&p.tickets[c0], 1u) == (unsigned)(c1 - c0);
-    __syncwarp();
-    asm volatile("barrier.sync 1, 128;" ::: "memory");
-    if (!last_flag) continue;
-    __threadfence();
-    for (int it = jt; it < p.M * (HD / 4); it += DC_JOINERS) {
-      const int m = it / (HD / 4), d = it % (HD / 4) * 4;
-      float top = -INFINITY, l = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k0 = c0; k0 <= c1; k0 += 8) {  // 8 records at a time: their reads fly together
-        float mk8[8], l8[8];
-        float4 v8[8];
+    const int c0 = alone ? cta : cuts ? pair * cuts : share.owner(place);
+    const int c1 = alone ? cta : cuts ? c0 + cuts - 1 : share.owner(place + tiles - 1);
+    dc_sync(DC_FILLED);
+    // Joins the first n records of the buffer; item: row m, 4 elements.
+    auto joined = [&](int n_rec, float* rec) {
+      for (int it = jt; it < p.M * (HD / 4); it += DC_JOINERS) {
+        const int m = it / (HD / 4), d = it % (HD / 4) * 4;
+        float2 ml[DC_WARPS];
+        float top = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int cc = min(k0 + k, c1);
-          const float* x = p.rec + (size_t)(cc == c0 ? 2 * cc + 1 : 2 * cc) * rec_floats;
-          mk8[k] = __ldcg(x + (size_t)p.M * HD + m);
-          l8[k] = __ldcg(x + (size_t)p.M * (HD + 1) + m);
-          v8[k] = __ldcg(reinterpret_cast<const float4*>(x + (size_t)m * HD + d));
+        for (int k = 0; k < DC_WARPS; ++k) {
+          ml[k] = k < n_rec ? join_ml[k * DC_ROWS + m] : make_float2(-INFINITY, 0.f);
+          top = fmaxf(top, ml[k].x);
         }
+        const float use = top == -INFINITY ? 0.f : top;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (k0 + k > c1) continue;
-          const float nt = fmaxf(top, mk8[k]), use = nt == -INFINITY ? 0.f : nt;
-          const float fo = pg_exp2(top - use), fn = pg_exp2(mk8[k] - use);
-          l = l * fo + l8[k] * fn;
-          acc.x = acc.x * fo + v8[k].x * fn, acc.y = acc.y * fo + v8[k].y * fn;
-          acc.z = acc.z * fo + v8[k].z * fn, acc.w = acc.w * fo + v8[k].w * fn;
-          top = nt;
+        for (int k = 0; k < DC_WARPS; ++k) {
+          if (k >= n_rec) continue;
+          const float f = pg_exp2(ml[k].x - use);
+          const float4 v = *reinterpret_cast<const float4*>(join + (k * DC_ROWS + m) * PITCH + d);
+          l += ml[k].y * f;
+          acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+        }
+        if (!rec) {
+          put(seq, head, m, d, top, l, acc);
+        } else {
+          *reinterpret_cast<float4*>(rec + (size_t)m * HD + d) = acc;
+          if (d == 0) *reinterpret_cast<float2*>(rec + (size_t)p.M * HD + 2 * m) = make_float2(top, l);
         }
       }
-      put(seq, head, m, d, top, l, acc);
+    };
+    joined(DC_WARPS, alone ? nullptr : record(cta, u0 == 0, 0));
+    const int parts = c1 - c0 + 1;
+    if (alone || (parts + 7) / 8 * ((p.M * (HD / 4) + DC_JOINERS - 1) / DC_JOINERS) <= DC_FLAT) {
+      if (more) dc_arrive(DC_FREE);  // the warps come for it before each further run
+      if (alone || !last(&p.tickets[2 * DC_LEVELS * c0 + 1], parts)) continue;
+#pragma unroll 1
+      for (int it = jt; it < p.M * (HD / 4); it += DC_JOINERS) {
+        const int m = it / (HD / 4), d = it % (HD / 4) * 4;
+        float top = -INFINITY, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int k0 = 0; k0 < parts; k0 += 8) {  // 8 records at a time: their reads fly together
+          float2 ml[8];
+          float4 v8[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int kk = min(k0 + k, parts - 1);
+            const float* x = record(c0 + kk, kk == 0, 0);
+            ml[k] = __ldcg(reinterpret_cast<const float2*>(x + (size_t)p.M * HD + 2 * m));
+            v8[k] = __ldcg(reinterpret_cast<const float4*>(x + (size_t)m * HD + d));
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            if (k0 + k >= parts) continue;
+            const float nt = fmaxf(top, ml[k].x), use = nt == -INFINITY ? 0.f : nt;
+            const float fo = pg_exp2(top - use), fn = pg_exp2(ml[k].x - use);
+            l = l * fo + ml[k].y * fn;
+            acc.x = acc.x * fo + v8[k].x * fn, acc.y = acc.y * fo + v8[k].y * fn;
+            acc.z = acc.z * fo + v8[k].z * fn, acc.w = acc.w * fo + v8[k].w * fn;
+            top = nt;
+          }
+        }
+        put(seq, head, m, d, top, l, acc);
+      }
+      continue;
     }
-    if (jt == 0) p.tickets[c0] = 0;
+    // 8 parts at a time through the buffer, then 8 times 8, and all; each time in the last CTA of those that add to it
+    for (int level = 0, span = 1;; ++level) {
+      const int from = c0 + (cta - c0) / (8 * span) * (8 * span);
+      const int n_rec = (min(8 * span, c1 + 1 - from) + span - 1) / span;
+      if (!last(&p.tickets[2 * DC_LEVELS * from + 2 * level + (from == c0)], n_rec)) break;
+#pragma unroll 1
+      for (int k = 0; k < n_rec; ++k) {
+        const float* x = record(from + k * span, from == c0 && k == 0, level);
+        for (int it = jt; it < p.M * (HD / 4); it += DC_JOINERS)
+          pg_cp16(join + (k * DC_ROWS + it / (HD / 4)) * PITCH + it % (HD / 4) * 4, x + it * 4);
+        if (2 * jt < p.M) pg_cp16(join_ml + k * DC_ROWS + 2 * jt, x + p.M * HD + 4 * jt);
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+      asm volatile("barrier.sync 1, 128;" ::: "memory");
+      span *= 8;
+      const bool all = from == c0 && from + span > c1;
+      joined(n_rec, all ? nullptr : record(from, from == c0, level + 1));
+      if (all) break;
+    }
+    if (more) dc_arrive(DC_FREE);
   }
 }
 

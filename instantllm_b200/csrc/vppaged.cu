@@ -211,7 +211,7 @@ size_t vp_paged_work_bytes(int32_t head_dim, int32_t n_q, int32_t n_kv, int32_t 
   if ((head_dim != 64 && head_dim != 128) || n_kv < 1 || n_q < 1 || n_q % n_kv || n_q / n_kv > PG_MAX_GROUP || rows < 1)
     return 0;
   const long long m = (long long)n_q / n_kv * rows;
-  const size_t few = PG_MAX_CTAS * 2 * pg_record(m < DC_ROWS ? (int)m : DC_ROWS, head_dim);
+  const size_t few = PG_MAX_CTAS * 2 * DC_LEVELS * pg_record(m < DC_ROWS ? (int)m : DC_ROWS, head_dim);
   const size_t many = PF_RECORDS * pg_record(m < PF_ROWS ? (int)m : PF_ROWS, head_dim);
   return WORK_HEAD + (few > many ? few : many) * sizeof(float);
 }

@@ -297,6 +297,25 @@ def test_decode_very_long(hd, n, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("nq,nkv,hd,rows,lens", [(1, 1, 64, 1, [60001]), (9, 1, 64, 1, [70003, 5]), (8, 1, 128, 1, [30001, 9, 12001]), (8, 1, 128, 2, [30001]),
+                                                 (14, 2, 64, 2, [40001]), (5, 1, 128, 3, [6001, 0, 9001]), (32, 8, 128, 4, [13001]), (12, 4, 64, 4, [2001])])
+def test_decode_joins_of_many_parts(nq, nkv, hd, rows, lens):
+    """One head's slots over up to all CTAs: records joined at once, by eights, by eights of eights, call after call with
+    the same bits."""
+    rng = np.random.default_rng(lens[0] + nq)
+    dtype, ps, n = torch.float16, 64, len(lens)
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, ps, dtype, fill=float("nan"))
+    q = torch.from_numpy(rng.standard_normal((n, rows, nq, hd)).astype(np.float32)).to(dtype)
+    masks = tree_masks(rng, n, rows)
+    d, m, ln = q.cuda(), torch.from_numpy(masks.astype(np.int32)).cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+    outs = [kv.decode(d, ln, mask=m, return_lse=True) for _ in range(12)]
+    kv.check()
+    for o, lse in outs[1:]:
+        assert torch.equal(o, outs[0][0]) and torch.equal(lse, outs[0][1])
+    compare(*outs[0], want_decode(q.double().numpy(), k, v, table, lens, masks, 0, 0, hd ** -0.5, ps), dtype, hd)
+
+
+@pytest.mark.gpu
 def test_decode_large_scores_and_empty_masks():
     """Scores far past exp's range, rising and falling along the cache; rows whose mask has no bit see the old slots only, and
     nothing when there are none."""
