@@ -129,7 +129,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 }
 
 // attend(prompts, cache, device, work, q, lens, mask, q_start, seqs, window, sinks, scale, out, return_lse)
-// -> out, or (out, lse), or an error code. work: a list of one tensor (or None), the workspace of the cache's layers.
+// -> out, or (out, lse), or an error code. work: a list whose first tensor is the workspace of the cache's layers.
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return guarded([&]() -> PyObject* {
     want(n_args == 14, "attend takes 14 arguments");
@@ -158,19 +158,15 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       lse = at::empty(q.sizes().slice(0, q.dim() - 1), at::TensorOptions().dtype(at::kFloat).device(at::kCUDA, (c10::DeviceIndex)call.device));
       t.lse = lse.mutable_data_ptr<float>();
     }
-    const size_t need = vp_paged_work_bytes(c.head_dim, t.n_q, c.n_kv, (int32_t)rows);
-    PyObject* held = PyList_GetItem(a[3], 0);  // borrowed
-    if (!held) return nullptr;
-    at::Tensor work;
-    if (held != Py_None) work = tensor(held, "work");
-    if (!work.defined() || (size_t)work.numel() < need) {
-      work = at::empty({(int64_t)std::max<size_t>(need, VP_PAGED_WORK_ZEROED)},
-                       at::TensorOptions().dtype(at::kByte).device(at::kCUDA, (c10::DeviceIndex)call.device));
-      work.narrow(0, 0, VP_PAGED_WORK_ZEROED).zero_();
-      PyList_SetItem(a[3], 0, THPVariable_Wrap(work));
-    }
+    // The layer brought the workspace when it was built, large enough for every call: a captured graph holds its address, and
+    // its counters were zeroed outside any capture, so a call never makes or replaces one.
+    PyObject* held = PyList_Size(a[3]) > 0 ? PyList_GetItem(a[3], 0) : Py_None;  // borrowed
+    if (PyErr_Occurred()) return nullptr;
+    const at::Tensor& work = tensor(held, "work");
+    want(call.here(work) && (size_t)work.nbytes() >= vp_paged_work_bytes(c.head_dim, t.n_q, c.n_kv, (int32_t)rows),
+         "the layer's workspace was replaced by another");
     t.work = work.data_ptr();
-    t.work_bytes = (uint64_t)work.numel();
+    t.work_bytes = (uint64_t)work.nbytes();
     t.q = q.const_data_ptr();
     t.out = out.data_ptr();
     const int heads = (int)q.dim() - 2;

@@ -26,6 +26,7 @@ from .synth import tree_to_buffer
 TYPES = {torch.float16: 0, torch.bfloat16: 1}
 DEV_ERR_TIMEOUT, DEV_ERR_PAGE, DEV_ERR_SLOT = 4, 16, 32
 MAX_ROWS = 16
+WORK_ZEROED = 16384  # VP_PAGED_WORK_ZEROED
 
 
 def _extension():
@@ -35,6 +36,19 @@ def _extension():
     except ImportError as e:
         raise VpError(f"instantllm_b200/_paged.so cannot be loaded ({e}): build it with instantllm_b200.build.build_torch()") from e
     return _paged
+
+
+def _workspace(work: list, head_dim: int, device: torch.device) -> None:
+    """work[0] becomes a workspace for every call over heads of this size, its counters zeroed: a call never allocates one, since
+    a captured graph holds its address and would only record the zeroing. A smaller one that was there moves back in the
+    list: graphs may hold its address too."""
+    # a record has 256 rows at most, whatever the call: this is the most (0 for heads that every call refuses)
+    need = _lib.load().vp_paged_work_bytes(head_dim, 64, 1, MAX_ROWS)
+    if work and work[0] is not None and work[0].nbytes >= need:
+        return
+    new = torch.empty(max(need, WORK_ZEROED), dtype=torch.uint8, device=device)
+    new[:WORK_ZEROED].zero_()
+    work[:] = [new] + [w for w in work if w is not None]
 
 
 def rope_table(rows: int, rot_dim: int = 64, theta: float = 1e6, device=0) -> torch.Tensor:
@@ -56,8 +70,9 @@ def ancestor_masks(trees) -> torch.Tensor:
 class PagedLayer:
     """One layer of a paged cache. k, v: [pages][heads][page_size][head_dim] in fp16 or bf16, elements of a slot adjacent, any
     strides in multiples of 8 elements (a [pages][page_size][heads][head_dim] pool transposed will do), the same for both;
-    table: int32 [requests][pages per request]. status (int32 [1]) and work (a list of one entry, the workspace or None) may be
-    shared between layers that run on one stream."""
+    table: int32 [requests][pages per request]. status (int32 [1]) and work (a list that holds the workspace, or [None]) may be
+    shared between layers that run on one stream. The workspace (43 MB at head_dim 64, 85 at 128) is made here, once, for
+    calls of any size, so that graphs may capture any of them, the first one included."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, status: Optional[torch.Tensor] = None,
                  work: Optional[list] = None):
@@ -72,9 +87,12 @@ class PagedLayer:
         _lib.load()
         self.k, self.v, self.table, self.device, self.dtype = k, v, table, k.device, k.dtype
         self.pages, self.n_kv, self.page_size, self.head_dim = k.shape
+        if torch.cuda.is_current_stream_capturing():
+            raise VpError("a layer cannot be built while a graph is captured: its workspace would only be zeroed by the replay")
         if status is None:
             status = torch.zeros(1, dtype=torch.int32, device=k.device)
         self.status, self._work = status, [None] if work is None else work
+        _workspace(self._work, self.head_dim, k.device)
         n, width = table.shape
         # strides of extents of 1 mean nothing: the dense ones stand in for them
         slot = k.stride(2)

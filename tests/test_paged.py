@@ -819,3 +819,74 @@ def test_other_stream_and_graph():
     torch.cuda.synchronize()
     replayed = third.clone()
     assert torch.equal(replayed, step()) and not torch.equal(replayed, first)
+
+
+def test_workspace_serves_every_call(lib):
+    """The workspace that a layer makes when it is built is the largest that any call asks for."""
+    for hd in (64, 128):
+        most = lib.vp_paged_work_bytes(hd, 64, 1, paged.MAX_ROWS)
+        for nq, nkv in ((14, 2), (32, 8), (12, 12), (64, 1), (256, 4), (9, 1)):
+            for rows in (1, 2, 3, 7, 15, 16, 17, 37, 64, 256, 5000, 1 << 24):
+                assert 0 < lib.vp_paged_work_bytes(hd, nq, nkv, rows) <= most
+    work = [None]
+    paged._workspace(work, 64, "cpu")
+    first = work[0]
+    assert first.nbytes == lib.vp_paged_work_bytes(64, 64, 1, 16) and not first[:paged.WORK_ZEROED].any()
+    paged._workspace(work, 64, "cpu")
+    assert len(work) == 1 and work[0] is first
+    paged._workspace(work, 128, "cpu")  # a layer of larger heads on the same list: the first one stays alive behind the new
+    assert len(work) == 2 and work[1] is first and work[0].nbytes > first.nbytes
+
+
+@pytest.mark.gpu
+def test_graph_outlives_larger_calls():
+    """A decode captured as the layer's very first call, then calls of every size before its first replay and between
+    replays: the graph's results are the eager ones, no tensor of others is written, and eager calls before the first
+    replay are right too."""
+    rng = np.random.default_rng(21)
+    lens, nq, nkv, hd = [9001, 3, 700], 14, 2, 64  # the first request is split and joined
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, 64, torch.float16)
+    q = torch.from_numpy(rng.standard_normal((3, 1, nq, hd)).astype(np.float32)).half()
+    d, ln = q.cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+    many = torch.from_numpy(rng.standard_normal((710, nq, hd)).astype(np.float32)).half().cuda()
+    starts = torch.tensor([0, 400, 401, 710], dtype=torch.int32).cuda()
+    tree = torch.from_numpy(rng.standard_normal((3, 16, nq, hd)).astype(np.float32)).half().cuda()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, lse = kv.decode(d, ln, return_lse=True)
+    eager = kv.decode(d, ln, return_lse=True)
+    compare(*eager, want_decode(q.double().numpy(), k, v, table, lens, np.ones((3, 1), dtype=np.int64), 0, 0, hd ** -0.5, 64),
+            torch.float16, hd)
+    big = kv.prefill(many, starts, ln), kv.decode(tree, ln)
+    others = [torch.full((n,), 7, dtype=torch.uint8, device="cuda") for n in (1 << 20, 1 << 21, 1 << 22, 1 << 24, 5 << 23) for _ in range(4)]
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager[0]) and torch.equal(lse, eager[1])
+        assert torch.equal(kv.prefill(many, starts, ln), big[0]) and torch.equal(kv.decode(tree, ln), big[1])
+    assert all(bool((x == 7).all()) for x in others)
+    kv.check()
+    with pytest.raises(_lib.VpError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            d + 1
+            paged.PagedLayer(kv.k, kv.v, kv.table)
+
+
+@pytest.mark.gpu
+def test_workspace_is_the_layers_own():
+    """A workspace that somebody put in the place of the layer's is refused, not replaced."""
+    rng = np.random.default_rng(22)
+    kv, *_ = make_cache(rng, [20], 2, 64, 16, torch.float16)
+    q, ln = torch.zeros(1, 1, 14, 64, dtype=torch.float16, device="cuda"), torch.tensor([20], dtype=torch.int32).cuda()
+    mine = kv._work[0]
+    kv._work[0] = mine[:1 << 16]
+    with pytest.raises(ValueError, match="workspace"):
+        kv.decode(q, ln)
+    kv._work[0] = None
+    with pytest.raises(ValueError, match="work"):
+        kv.decode(q, ln)
+    kv._work[0] = mine
+    kv.decode(q, ln)
+    kv.check()
