@@ -72,6 +72,16 @@ __device__ __forceinline__ void pg_cp_arrive(uint64_t* bar) {
 __device__ __forceinline__ void pg_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// Wait of a whole warp that ends early once `dead` (shared memory) is set; false if the phase is not complete. The lanes
+// leave on a vote, as in mbar_wait_warp.
+__device__ __forceinline__ bool pg_wait(uint64_t* bar, uint32_t parity, const int* dead) {
+  const unsigned long long t0 = globaltimer();
+  for (uint32_t i = 0; i < (1u << 26); ++i) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((i & 63) == 0 && __any_sync(0xffffffffu, *(const volatile int*)dead || globaltimer() - t0 > WAIT_NS)) return false;
+  }
+  return false;
+}
 __device__ __forceinline__ float pg_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -269,6 +269,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     mbar_init(&wanted, 1);
     fence_barrier_init();
     dead = 0;
+    info[0].seq = info[1].seq = -1;
   }
   if (warp == PF_PRODUCER && lane == 0) {
     pg_prefetch_map(&mk);
@@ -354,18 +355,32 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   pf_fence_after();
   const uint32_t tmem = tmem_base;
 
-  // Waits of a whole warp. After one that ran out none waits any more, and the call ends
-  // with an error status.
+  // Waits of a whole warp. After one that ran out none waits any more, and the call ends with an error status: the
+  // scheduler hands out no more pieces, and everybody goes through those that are out, without waiting, to the end. No role
+  // leaves before: the softmax warps meet at named barriers, which have no limit and want all of them. So the hand-over
+  // of pieces itself is always waited for. Its limit is many times that of the others: no role passes more than one wait that
+  // runs out.
   auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
     __syncwarp();
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return;
-    if (!*(volatile int*)&dead && !mbar_wait_warp(bar, parity)) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    const bool there = pg_wait(bar, parity, &dead);
+    if (!there) {
       pg_status(c.status, VP_DEV_ERR_TIMEOUT);
       *(volatile int*)&dead = 1;
     }
     __syncwarp();
+    return there;
   };
-  auto is_dead = [&] { return *(volatile int*)&dead != 0; };
+  auto wait_piece = [&](uint64_t* bar, uint32_t parity) {
+    __syncwarp();
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return;
+#pragma unroll 1
+    for (int k = 0; k < 8; ++k)
+      if (mbar_wait_warp(bar, parity)) return;
+    pg_status(c.status, VP_DEV_ERR_TIMEOUT);
+    *(volatile int*)&dead = 1;
+    __syncwarp();
+  };
 
   if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_OTHER_REGS));
   if (warp < 8) {
@@ -380,7 +395,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     uint32_t units = 0, n_last = 0;  // units of all pieces so far, phases of o_last so far
     // Queries of piece r on their way into the row tile's buffer, once the last product that reads it is done.
     auto fetch = [&](int r) {
-      wait_warp(&info_full[r & 1], (r >> 1) & 1);
+      wait_piece(&info_full[r & 1], (r >> 1) & 1);
       const PfPiece& in = info[r & 1];
       const int f = in.f0 + tid;  // with one row tile the second warpgroup has none to bring
       if (in.seq >= 0 && f < in.f_end) {
@@ -406,7 +421,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       fetched = false;
       const PfPiece& in = info[r & 1];
       const int seq = in.seq, f_end = in.f_end, f0 = in.f0, head = in.head, first = in.first, base = in.base;
-      if (seq < 0 || is_dead()) break;
+      if (seq < 0) break;
       const bool two = f_end > f0 + 128;  // row tiles
       const int i_row = two ? i : 0, f = f0 + i_row * 128 + row;
       const int n_t = !two ? (in.n0 + 1 - i) / 2 : i ? in.n1 : in.n0, j0 = in.j0, cuts = in.cuts, cut = in.cut, live = in.live, record0 = in.record0;
@@ -725,7 +740,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     // last block on. Which CTA has a piece does not show in the results. ----
     unsigned* next = p.tickets + 4 * PF_RECORDS;  // and the number of CTAs that have come to the end
     for (int r = 0;; ++r) {
-      if (r >= 2) wait_warp(&info_empty[r & 1], ((r >> 1) - 1) & 1);
+      if (r >= 2) wait_piece(&info_empty[r & 1], ((r >> 1) - 1) & 1);
       unsigned idx = blockIdx.x;
       if (r > 0) {  // taken when the last copies of the piece before are under way, not earlier: whoever is ahead takes more
         wait_warp(&wanted, (r - 1) & 1);
@@ -738,7 +753,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         piece = -1;
       }
       PfPiece& in = info[r & 1];
-      if (piece < 0 || is_dead()) {
+      if (__any_sync(0xffffffffu, piece < 0 || *(volatile int*)&dead)) {
         if (lane == 0) {
           in.seq = -1;
           pg_arrive(&info_full[r & 1]);
@@ -801,20 +816,21 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     // ---- K and V tiles, in the order of their use: K0 V0 K1 V1 ... ----
     const int box = min(c.page_size, PF_TS), boxes = PF_TS / box;
     uint32_t issued = 0, edges = 0;
+    bool gone = false;  // a wait ran out: nothing is refilled any more
     for (int r = 0;; ++r) {
-      wait_warp(&info_full[r & 1], (r >> 1) & 1);
+      wait_piece(&info_full[r & 1], (r >> 1) & 1);
       const PfPiece& in = info[r & 1];
       const int seq = in.seq, table_row = in.row, head = in.head, j0 = in.j0, n_max = max(in.n0, in.n1), see_lo = in.see_lo, see_end = in.see_end, base = in.base;
       const uint32_t any = in.any;
       PfSpan sp;
       sp.ns = in.ns;
       sp.ws = in.ws;
-      if (seq < 0 || is_dead()) break;
+      if (seq < 0) break;
       __syncwarp();
       if (lane == 0) pg_arrive(&info_empty[r & 1]);
       // a request outside the table has no slots, and no page is looked up for it
       const int32_t* pages = c.table + table_row * c.table_stride;
-      for (int j = 0; j < n_max; ++j) {
+      for (int j = 0; j < n_max && !gone; ++j) {
         if (j == max(0, n_max - PF_AHEAD) && lane == 0) pg_arrive(&wanted);
         const int s0 = sp.at(j0 + j) * PF_TS, slot = s0 + lane * box;
         int page = c.n_pages;  // a box that nobody sees fills zeros
@@ -831,8 +847,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv, ++issued) {
           const uint32_t st = issued % SLOTS;
-          if (issued >= SLOTS) wait_warp(&kv_empty[st], (issued / SLOTS - 1) & 1);
-          if (is_dead()) break;
+          if (issued >= SLOTS && !gone) gone = !wait_warp(&kv_empty[st], (issued / SLOTS - 1) & 1);
+          if (gone) break;
           const bool patch = kv && ragged;
           uint64_t* bar = patch ? &edge : &kv_full[st];
           unsigned char* tile = ring + (size_t)st * TILE;
@@ -844,7 +860,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
               pg_box(tile + d * PANEL + lane * box * 128, kv ? &mv : &mk, d, slot & (c.page_size - 1), head, page, bar);
           }
           if (patch) {
-            wait_warp(&edge, edges & 1);
+            gone = !wait_warp(&edge, edges & 1);
             ++edges;
             for (int x = lane; x < PF_TS; x += 32) {
               const int sl = s0 + x;
@@ -860,11 +876,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
             if (lane == 0) pg_arrive(&kv_full[st]);
           }
         }
-        if (is_dead()) break;
       }
       if (n_max == 0 && lane == 0) pg_arrive(&wanted);
     }
     // copies still in flight land before the CTA may end (they have, unless a wait ran out)
+    if (edges) mbar_wait_warp(&edge, (edges - 1) & 1);
     for (uint32_t k = issued > SLOTS ? issued - SLOTS : 0; k < issued; ++k) mbar_wait_warp(&kv_full[k % SLOTS], (k / SLOTS) & 1);
   } else if (warp == PF_ISSUER) {
     // ---- products. The whole warp walks, one elected lane issues: what the operands' descriptors come from
@@ -899,11 +915,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     };
     uint32_t used = 0, units = 0;  // K and V tiles, and units, of all pieces so far
     for (int r = 0;; ++r) {
-      wait_warp(&info_full[r & 1], (r >> 1) & 1);
+      wait_piece(&info_full[r & 1], (r >> 1) & 1);
       const PfPiece& in = info[r & 1];
       const int seq = __shfl_sync(0xffffffffu, in.seq, 0), n0 = __shfl_sync(0xffffffffu, in.n0, 0), n1 = __shfl_sync(0xffffffffu, in.n1, 0);
       const bool two = __shfl_sync(0xffffffffu, in.f_end - in.f0, 0) > 128;
-      if (seq < 0 || is_dead()) break;
+      if (seq < 0) break;
       __syncwarp();
       if (lead) {
         pg_arrive(&info_empty[r & 1]);
@@ -930,7 +946,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         if (!two || i) free_tile(k);  // the second row tile sees every tile of slots that the first does
       };
       for (int u = 0; u < min(n, BUFS); ++u) start(u);
-      for (int u = 0; u < n && !is_dead(); ++u) {
+      for (int u = 0; u < n; ++u) {
         int i;
         const int j = tile_of(u, i);
         const uint32_t g = units + u, v = used + 2 * j + 1;

@@ -890,3 +890,28 @@ def test_workspace_is_the_layers_own():
     kv._work[0] = mine
     kv.decode(q, ln)
     kv.check()
+
+
+def kernel_source(name):
+    return (build.PKG / "csrc" / name).read_text()
+
+
+def test_tile_kernel_goes_through_its_pieces_to_the_end():
+    """A wait that runs out must end in a status. The tile kernel's softmax warps meet at named barriers, which have no limit and
+    want all of them, so no role may leave by a flag that another has not seen yet: only the scheduler looks at it, and
+    everybody leaves at the piece that says so, whose hand-over is always waited for. Copies that were not waited for land
+    before the CTA ends. Told from the source: on a sound kernel no wait can be made to run out."""
+    src = kernel_source("vp_paged_prefill.cuh")
+    parts = [src.index(x) for x in ("---- softmax", "---- the CTA's pieces", "---- K and V tiles", "---- products")] + [len(src)]
+    softmax, scheduler, producer, issuer = (src[a:b] for a, b in zip(parts, parts[1:]))
+    assert "dead" not in softmax + issuer
+    for role in (softmax, producer, issuer):
+        loop = role[role.index("for (int r = 0;; ++r) {"):]
+        assert [x.strip() for x in loop.splitlines() if "seq < 0" in x and "break" in x] == ["if (seq < 0) break;"]
+        assert "wait_piece(&info_full" in role and "wait_warp(&info_full" not in role
+        assert "pg_arrive(&info_empty" in role[role.index("if (seq < 0) break;"):]
+    assert "wait_piece(&info_empty" in scheduler and "__any_sync(0xffffffffu, piece < 0 || *(volatile int*)&dead)" in scheduler
+    waits = src[src.index("auto wait_piece"):src.index("if (warp >= 8) asm")]
+    assert "pg_wait" not in waits and waits.count("dead") == 1  # it sets the flag, and does not look at it
+    assert producer.count("gone = !wait_warp") == 2 and "if (gone) break;" in producer
+    assert "mbar_wait_warp(&edge" in producer
