@@ -181,6 +181,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
   __shared__ uint64_t full[DC_WARPS][DC_STAGES], q_full[2];
   __shared__ int warp_sums[DC_THREADS / 32], warp_most[DC_THREADS / 32], warp_least[DC_THREADS / 32];
   __shared__ int first_seq, first_tile, t0_s, t1_s, dead, last_flag;  // first_tile: number of first_seq's first tile
+  __shared__ int gave_up[DC_WARPS];  // the first tile of a warp whose wait ran out
 
   const vp_paged& c = p.c;
   const vp_paged_attn& a = p.a;
@@ -191,6 +192,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
   if (tid < DC_WARPS * DC_STAGES) mbar_init(&full[0][0] + tid, 1);
   if (tid < 2) mbar_init(&q_full[tid], DC_JOINERS);
   if (tid == 0) dead = 0;
+  if (tid < DC_WARPS) gave_up[tid] = -1;
   if (tid < 32) fence_barrier_init();
   for (int i = tid; i < 2 * Sh::QBUF / 16; i += DC_THREADS) reinterpret_cast<uint4*>(qbuf)[i] = make_uint4(0, 0, 0, 0);
   if (tid == 32) {
@@ -286,14 +288,17 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
   const int t0 = t0_s, t1 = t1_s;
   if (t0 == t1) return;
 
-  // Waits of a whole warp; after one that ran out none waits any more, and the call ends with an error status.
+  // Waits of a whole warp: whether the phase is complete. After one that ran out none waits any more, and the call ends with an
+  // error status; everybody goes on to the end, as the roles meet at named barriers that want all of them.
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     __syncwarp();
-    if (!*(volatile int*)&dead && !mbar_wait_warp(bar, parity)) {
+    const bool there = pg_wait(bar, parity, &dead);
+    if (!there) {
       pg_status(c.status, VP_DEV_ERR_TIMEOUT);
       *(volatile int*)&dead = 1;
     }
     __syncwarp();
+    return there;
   };
 
   if (warp < DC_WARPS) {
@@ -399,7 +404,11 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
       float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
       for (; next < w.t + n; next += DC_WARPS, ++k_th) {
         const int st = k_th % DC_STAGES, s0 = w.slot(w.u + next - w.t);
-        wait(&full[warp][st], (k_th / DC_STAGES) & 1);
+        if (!wait(&full[warp][st], (k_th / DC_STAGES) & 1)) {
+          if (lane == 0 && gave_up[warp] < 0) gave_up[warp] = k_th;
+          coming.any = false;  // nothing is asked for any more: a stage whose copy was not waited for is not refilled
+          ahead.t = t1;
+        }
         const uint32_t kb = stage0 + st * 2 * DC_TILE, vb = kb + DC_TILE;
         float s[NT][4], s2[NT][4];
         // lanes 0-7 .. 24-31 point at the lines of four 8 x 8 matrices: 8 slots, 32 elements; two sums
@@ -503,6 +512,11 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
       dc_arrive(DC_FILLED);
       w.advance(n);
     }
+    // copies still in flight land before the CTA may end (they have, unless a wait ran out)
+    __syncwarp();
+    const int left = gave_up[warp];
+    if (left >= 0)
+      for (int k = left; k < left + DC_STAGES && t0 + warp + k * DC_WARPS < t1; ++k) mbar_wait_warp(&full[warp][k % DC_STAGES], (k / DC_STAGES) & 1);
     return;
   }
 

@@ -915,3 +915,16 @@ def test_tile_kernel_goes_through_its_pieces_to_the_end():
     assert "pg_wait" not in waits and waits.count("dead") == 1  # it sets the flag, and does not look at it
     assert producer.count("gone = !wait_warp") == 2 and "if (gone) break;" in producer
     assert "mbar_wait_warp(&edge" in producer
+
+
+def test_decode_refills_nothing_after_a_wait_that_ran_out():
+    """A decode warp whose wait for a stage ran out asks for no more tiles (the copy may still arrive in the stage, and its barrier
+    counts one at a time), and waits once more for what is in flight before the CTA may end. Told from the source."""
+    src = kernel_source("vp_paged_decode.cuh")
+    warps = src[src.index("---- consumers"):src.index("---- joiners")]
+    at = warps.index("if (!wait(&full[warp][st]")
+    block = warps[at:warps.index("const uint32_t kb", at)]
+    assert "coming.any = false;" in block and "ahead.t = t1;" in block and "gave_up[warp] = k_th" in block
+    end = warps[warps.index("w.advance(n);"):]
+    assert "gave_up[warp]" in end and "mbar_wait_warp(&full[warp][k % DC_STAGES], (k / DC_STAGES) & 1)" in end
+    assert "pg_wait(bar, parity, &dead)" in src and "!*(volatile int*)&dead" not in src  # lanes agree on the flag
