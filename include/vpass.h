@@ -407,7 +407,8 @@ int vp_paged_append(const vp_paged* c, const vp_paged_rows* r, void* stream);
  * seqs (NULL: i) names request i's row of the table. Rows before a request's first slot (more rows
  * than its length) see nothing; rows of q that no request has are left alone in out. Strides as above;
  * lse is dense. work: vp_paged_work_bytes(..., rows of the call) bytes, 256-byte aligned, the first
- * VP_PAGED_WORK_ZEROED of them zeroed once before its first use (each call leaves them zero); calls
+ * VP_PAGED_WORK_ZEROED of them zeroed once before its first use (each call leaves them zero, but for one that ended
+ * in VP_DEV_ERR_TIMEOUT: zero them again then); calls
  * that share it must not overlap on the GPU, and it has to outlive every graph that captured one. Results depend on the
  * inputs alone, not on timing.
  *   limits   n_q a multiple of n_kv, n_q / n_kv <= 64; sinks >= 0, window >= 0. */

@@ -140,6 +140,9 @@ class PagedLayer:
         bits = int(self.status.item())
         if bits:
             self.status.zero_()
+            if bits & DEV_ERR_TIMEOUT:  # a call that gave up may have left counters that the next one would start from
+                for w in self._work:
+                    w[:WORK_ZEROED].zero_()
             raise VpError("the cache's calls met " + " and ".join(t for b, t in (
                 (DEV_ERR_PAGE, "a page outside the pool"),
                 (DEV_ERR_SLOT, "a request, slot, position or length outside the table"),

@@ -928,3 +928,26 @@ def test_decode_refills_nothing_after_a_wait_that_ran_out():
     end = warps[warps.index("w.advance(n);"):]
     assert "gave_up[warp]" in end and "mbar_wait_warp(&full[warp][k % DC_STAGES], (k / DC_STAGES) & 1)" in end
     assert "pg_wait(bar, parity, &dead)" in src and "!*(volatile int*)&dead" not in src  # lanes agree on the flag
+
+
+@pytest.mark.gpu
+def test_check_after_a_timeout_leaves_the_counters_zero():
+    """What a call that gave up leaves behind (its status bit, counters that are not back at zero) is gone after check(), on
+    every workspace that the layer has had; later calls are right."""
+    rng = np.random.default_rng(23)
+    lens, nq, nkv, hd = [9001, 3, 700], 14, 2, 64
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, 64, torch.float16)
+    one = torch.from_numpy(rng.standard_normal((3, 1, nq, hd)).astype(np.float32)).half().cuda()
+    tree = torch.from_numpy(rng.standard_normal((3, 16, nq, hd)).astype(np.float32)).half().cuda()
+    ln = torch.tensor(lens, dtype=torch.int32).cuda()
+    want = kv.decode(one, ln), kv.decode(tree, ln)
+    kv.check()
+    kv._work.append(torch.zeros(paged.WORK_ZEROED, dtype=torch.uint8, device="cuda"))
+    for w in kv._work:  # set by hand, with no call under way
+        w[:paged.WORK_ZEROED].fill_(1)
+    kv.status.fill_(paged.DEV_ERR_TIMEOUT)
+    with pytest.raises(_lib.VpError, match="void"):
+        kv.check()
+    assert not any(bool(w[:paged.WORK_ZEROED].any()) for w in kv._work)
+    assert torch.equal(kv.decode(one, ln), want[0]) and torch.equal(kv.decode(tree, ln), want[1])
+    kv.check()
