@@ -275,12 +275,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     pg_prefetch_map(&mk);
     pg_prefetch_map(&mv);
   }
-  __syncwarp();
-  if (warp == PF_ISSUER) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(PF_TMEM)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
   pdl_wait();
   // Pieces of all requests, in two sums: all tiles, which give the share of a CTA (left out where no
   // request can be long enough to be cut); pieces and records.
@@ -307,6 +301,14 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     one_last = s.last_tiles(p);
     s.see(p, 0, min(p.rows, s.n_new * p.group));
     tiles += (long long)s.blocks * (one_last + pf_span(s.lo, s.end, a.sinks).tiles);
+  }
+  // Tensor memory is taken here, beside the reads above, not in the prologue: the kernel before may be one that still waits
+  // for its own, on this SM, while this one would hold all of it and wait for its end.
+  __syncwarp();
+  if (warp == PF_ISSUER) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(PF_TMEM)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   int share = 1 << 30;
   if (p.cuts) {

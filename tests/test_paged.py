@@ -951,3 +951,10 @@ def test_check_after_a_timeout_leaves_the_counters_zero():
     assert not any(bool(w[:paged.WORK_ZEROED].any()) for w in kv._work)
     assert torch.equal(kv.decode(one, ln), want[0]) and torch.equal(kv.decode(tree, ln), want[1])
     kv.check()
+
+
+def test_tensor_memory_is_taken_after_the_kernel_before():
+    """A kernel whose prologue overlaps the one before it must hold nothing that that one could wait for. From the source."""
+    src = kernel_source("vp_paged_prefill.cuh")
+    body = src[src.index("k_paged_tiles(const"):]
+    assert body.index("pdl_wait();") < body.index("tcgen05.alloc")
