@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     if (!s.blocks || !p.cuts) continue;
     one_last = s.last_tiles(p);
     s.see(p, 0, min(p.rows, s.n_new * p.group));
-    tiles += (long long)s.blocks * (one_last + pf_span(s.lo, s.end, a.sinks).tiles);
+    tiles = min(tiles + (long long)s.blocks * (one_last + pf_span(s.lo, s.end, a.sinks).tiles), 1ll << 50);
   }
   // Tensor memory is taken here, beside the reads above, not in the prologue: the kernel before may be one that still waits
   // for its own, on this SM, while this one would hold all of it and wait for its end.
@@ -323,7 +323,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     // cache head. Rounded up by two so that the float division cannot make it less than an even half.
     share = max(PF_LEAST, (int)fminf((float)all * c.n_kv / (2 * p.sms), 1e8f) + 2);
   }
-  int pieces = 0, records = 0;
+  // Requests whose rows overlap can have more pieces than a word counts: the sums stop at PF_MANY, which is more than
+  // any call may have.
+  constexpr unsigned PF_MANY = 0x7fffffff;
+  unsigned pieces = 0;
+  int records = 0;
   for (int i = i0; i < i1; ++i) {
     int blocks = one_blocks, last = one_last;
     if (chunk > 1) {
@@ -333,24 +337,27 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     }
     if (!blocks) continue;
     const int n = p.cuts ? pf_cuts(last, share) : 1;
-    pieces += blocks * n * c.n_kv;
+    pieces = (unsigned)min(pieces + (unsigned long long)blocks * n * c.n_kv, (unsigned long long)PF_MANY);
     if (n > 1) records += blocks * n * c.n_kv;
   }
-  int incl = pieces, incl_r = records;
+  unsigned incl = pieces;
+  int incl_r = records;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o), x = __shfl_up_sync(0xffffffffu, incl_r, o);
-    if (lane >= o) incl += v, incl_r += x;
+    const unsigned v = __shfl_up_sync(0xffffffffu, incl, o);
+    const int x = __shfl_up_sync(0xffffffffu, incl_r, o);
+    if (lane >= o) incl = min(incl + v, PF_MANY), incl_r += x;
   }
-  if (lane == 31) sums[warp][0] = incl, sums[warp][1] = incl_r;
+  if (lane == 31) sums[warp][0] = (int)incl, sums[warp][1] = incl_r;
   cta_sync();
-  int at0 = incl - pieces, at_r0 = incl_r - records, total = 0;
+  unsigned at0 = incl - pieces, total = 0;
+  int at_r0 = incl_r - records;
 #pragma unroll
   for (int w = 0; w < PF_THREADS / 32; ++w) {
     if (w < warp) at0 += sums[w][0], at_r0 += sums[w][1];
-    total += sums[w][0];
+    total = min(total + sums[w][0], PF_MANY);
   }
-  starts[tid] = at0;
+  starts[tid] = (int)at0;
   rec_starts[tid] = at_r0;
   pf_fence_before();
   cta_sync();
@@ -749,8 +756,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         if (lane == 0) idx = gridDim.x + atomicAdd(next, 1u);
         idx = __shfl_sync(0xffffffffu, idx, 0);
       }
-      int piece = idx < (unsigned)total ? total - 1 - (int)idx : -1;
-      if (total > p.most) {  // requests whose rows overlap
+      int piece = idx < total ? (int)(total - 1 - idx) : -1;
+      if (total > (unsigned)p.most) {  // requests whose rows overlap
         if (lane == 0) pg_status(c.status, VP_DEV_ERR_SLOT);
         piece = -1;
       }

@@ -40,7 +40,7 @@ int tiles_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
   const long long cuts = (tiles + PF_LEAST - 1) / PF_LEAST - 1;
   p.cuts = 2 * tiles > 3 * PF_LEAST;
   const long long more = !p.cuts ? 0 : pairs * cuts < 2 * p.sms ? pairs * cuts : 2 * p.sms;
-  if (pairs + more > 0x7fffffffll) return pfail(VP_ERR_ARG, "more rows than a launch holds");
+  if (pairs + more >= 0x7fffffffll) return pfail(VP_ERR_ARG, "more rows than a launch holds");
   p.most = (int)(pairs + more);
   return pg_launch(a.q_start ? "vp_paged_prefill" : "vp_paged_decode", k_paged_tiles<T, HD>, p.most < p.sms ? p.most : p.sms, PF_THREADS,
                    Sh::SMEM, st, p, mk, mv);

@@ -958,3 +958,21 @@ def test_tensor_memory_is_taken_after_the_kernel_before():
     src = kernel_source("vp_paged_prefill.cuh")
     body = src[src.index("k_paged_tiles(const"):]
     assert body.index("pdl_wait();") < body.index("tcgen05.alloc")
+
+
+@pytest.mark.gpu
+def test_overlapping_rows_past_a_count_of_32_bits():
+    """Requests that all claim the same 2^30 rows have 2^32 pieces between them: told, and nothing is written."""
+    rng = np.random.default_rng(24)
+    n, rows = 1024, 1 << 30
+    kv, *_ = make_cache(rng, [40] * 2, 2, 64, 16, torch.float16, extra_rows=n - 2)
+    q = torch.zeros(1, 2, 64, dtype=torch.float16, device="cuda").expand(rows, 2, 64)
+    out = torch.full((1, 2, 64), 7.0, dtype=torch.float16, device="cuda")
+    starts = torch.tensor([0, rows] * (n // 2) + [0], dtype=torch.int32).cuda()
+    kv.prefill(q, starts, torch.full((n,), 40, dtype=torch.int32, device="cuda"), out=out.expand(rows, 2, 64))
+    with pytest.raises(_lib.VpError, match="slot"):
+        kv.check()
+    assert bool((out == 7).all())
+    one, ln = torch.ones(40, 4, 64, dtype=torch.float16, device="cuda"), torch.tensor([40], dtype=torch.int32).cuda()
+    kv.prefill(one, torch.tensor([0, 40], dtype=torch.int32).cuda(), ln)
+    kv.check()
