@@ -394,7 +394,8 @@ int vp_paged_append(const vp_paged* c, const vp_paged_rows* r, void* stream);
 
 /* Attention over the cache: out = softmax(scale q K^T) V over the slots that a row sees, per query
  * head (head h reads cache head h / (n_q / n_kv)); lse, if not NULL, its log sum exp (natural). A row
- * that sees nothing gives zeros and -inf. Scores, softmax statistics and sums are fp32.
+ * that sees nothing gives zeros and -inf. Scores, softmax statistics and sums are fp32; the weights exp(S - m) are
+ * rounded to the cache's type for the product with V.
  * vp_paged_decode: the newest rows of n requests, `rows` (1..16) each, which are the last slots of
  *   lens[i]: q and out [n][rows][n_q][head_dim], lse [n][rows][n_q]. Row r sees every slot before the
  *   new ones, and new slot j if bit j of mask[i * rows + r] is set (NULL: j <= r), so a draft tree is

@@ -3,7 +3,10 @@
 //
 // Mathematics. Per request and cache head: S = scale q K^T over the visible slots,
 // p = 2^(S log2 e - m) with the running maximum m, l = sum p, o = sum p v; two such records (m, l, o)
-// over disjoint slots join as m* = max, l* = sum l 2^(m - m*), o* likewise, and out = o / l.
+// over disjoint slots join as m* = max, l* = sum l 2^(m - m*), o* likewise, and out = o / l. The second product's operand, p,
+// is rounded to the cache's type, as the tensor cores take it: an output is then off by up to one unit of that rounding more
+// than the exact result's own (l adds up the unrounded p). fp16 has nothing below 2^-24, so there m is taken DC_LIFT below the
+// maximum: weights reach 2^DC_LIFT, and those lost to o are below 2^-39 of the largest, which 2^17 slots do not add up.
 //
 // Bound: the bytes of K and V, each read once, and for small calls the chain of dependent reads
 // (length, page, K, V). So the query rows of one cache head (G heads x R rows, packed as m = r G + g)
@@ -48,6 +51,8 @@ constexpr int DC_SHORT = 64;
 // 21.1 and 22.4; 18 of 16 rows of 128 (12 rounds): 23.7 by eights, 29 otherwise; 50 of 8 rows of 128 (14): 14.9 and 22.
 constexpr int DC_FLAT = 3;
 constexpr int DC_LEVELS = 3;                        // of joins that leave a record: 8^3 parts a pair, more than CTAs
+
+constexpr float DC_LIFT = 14.f;                     // log2 of the largest weight in fp16 (2^16 is past its range)
 
 template <int HD>
 struct DcShape {
@@ -451,7 +456,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
         for (int h = 0; h < 2; ++h) {
           mn[h] = fmaxf(mn[h], __shfl_xor_sync(0xffffffffu, mn[h], 1));
           mn[h] = fmaxf(mn[h], __shfl_xor_sync(0xffffffffu, mn[h], 2));
-          mn[h] = fmaxf(mx[h], mn[h] * cexp);
+          mn[h] = fmaxf(mx[h], fmaf(mn[h], cexp, PgType<T>::BF16 ? 0.f : -DC_LIFT));
           use[h] = mn[h] == -INFINITY ? 0.f : mn[h];
           f[h] = pg_exp2(mx[h] - use[h]);
           mx[h] = mn[h];

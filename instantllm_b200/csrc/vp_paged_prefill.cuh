@@ -2,8 +2,10 @@
 // vp_paged_decode where the new rows of a request and the heads of a group make more than 16.
 //
 // Mathematics as in vp_paged_decode.cuh: a running maximum m and sum l over tiles of 128 slots. The
-// maximum that the weights are taken against only moves when the tile's is more than 2^8 above it
-// (weights then reach 2^8 at most, and out = o / l does not depend on it), so o is rarely rescaled.
+// maximum that the weights are taken against only moves when the tile's is more than 2^PF_SLACK above it
+// (out = o / l does not depend on it), so o is rarely rescaled. In fp16 it is taken PF_LIFT below: weights
+// reach 2^(PF_SLACK + PF_LIFT), within its range, and those lost to o are below 2^-32 of the largest, in all
+// 2^-15 of it over 2^17 slots.
 //
 // Bound: the tensor cores at head_dim 128, the exponentials (16 a clock and SM against 4,096 products)
 // at 64. The query rows of one cache head are packed as row G + g, 256 of them to a block as two
@@ -39,7 +41,8 @@ constexpr int PF_THREADS = 384;            // two softmax warpgroups, then one: 
 constexpr int PF_PRODUCER = 8, PF_ISSUER = 9, PF_SCHEDULER = 10;
 constexpr int PF_SOFTMAX_REGS = 208, PF_OTHER_REGS = 88;  // of the 168 a thread that the block is launched with
 constexpr uint32_t PF_TMEM = 512;          // columns
-constexpr float PF_SLACK = 8.f;            // log2 of the largest weight
+constexpr float PF_SLACK = 8.f;            // log2 (with 4 and a lift of 11, 2,048 rows over 6,001 to 8,191 slots with a window and 4 sinks: 96 us, 89 with these)
+constexpr float PF_LIFT = 7.f;             // log2, in fp16
 
 template <int HD>
 struct PfShape {
@@ -494,7 +497,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             t4[e] = fmaxf(fmaxf(t4[e], __uint_as_float(s[k + 2 * e])), __uint_as_float(s[k + 2 * e + 1]));
-        const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * cexp;
+        const float top = fmaf(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])), cexp, PgType<T>::BF16 ? 0.f : -PF_LIFT);
         const bool move = top > m + PF_SLACK || (m == -INFINITY && top > m);
         if (__any_sync(0xffffffffu, move)) {
           // a row's maximum moves by its own scores alone: what the other rows of the warp hold (rows past the

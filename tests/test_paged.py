@@ -976,3 +976,41 @@ def test_overlapping_rows_past_a_count_of_32_bits():
     one, ln = torch.ones(40, 4, 64, dtype=torch.float16, device="cuda"), torch.tensor([40], dtype=torch.int32).cuda()
     kv.prefill(one, torch.tensor([0, 40], dtype=torch.int32).cuda(), ln)
     kv.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kind,lift", [("one", 14), ("tree", 7), ("prompt", 7)])
+def test_small_weights_of_many_slots(kind, lift, hd, dtype):
+    """One slot far above 60,000 others whose weights, 2^-26.7 of its own each, carry all of the output: the weights that fp16
+    rounds are taken 2^lift higher, so what is lost of each is at most half of 2^(-24 - lift)."""
+    rng = np.random.default_rng(25)
+    n, nq, ps, rows = 60001, 4, 64, {"one": 1, "tree": 5, "prompt": 5}[kind]
+    kv, _, _, table = make_cache(rng, [n], 1, hd, ps, dtype)
+    kv.k.zero_()
+    kv.k[..., 0] = -18.5
+    kv.v.copy_(1000 + torch.randint(-8, 9, kv.v.shape, device="cuda") * 4)
+    top = int(table[0, 0])
+    kv.k[top, 0, 3, 0] = 0
+    kv.v[top, 0, 3] = 0
+    k, v = kv.k.cpu().double().numpy(), kv.v.cpu().double().numpy()
+    q = torch.zeros(1, rows, nq, hd, dtype=dtype)
+    q[..., 0] = 1
+    q[..., 1] = torch.arange(rows * nq).view(1, rows, nq)  # meets zeros
+    ln = torch.tensor([n], dtype=torch.int32).cuda()
+    if kind == "prompt":
+        out, lse = (x[None] for x in kv.prefill(q[0].cuda(), torch.tensor([0, rows], dtype=torch.int32).cuda(), ln, scale=1.0, return_lse=True))
+    else:
+        out, lse = kv.decode(q.cuda(), ln, scale=1.0, return_lse=True)
+    kv.check()
+    out, lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
+    u, step = U[dtype], 2.0 ** (-25 - lift) if dtype == torch.float16 else 0.0
+    ks, vs = (O.slots(p, table[0], n) for p in (k, v))
+    for r in range(rows):
+        seen = np.arange(n) <= n - rows + r
+        o, le, spread, smax = O.attend(q[0, r, 0].double().numpy(), ks[0], vs[0], seen, 1.0)
+        assert 0.5 < o.min()
+        tol = u * np.abs(o) + (u + 2 * (hd * 2.0 ** -23 * smax + 2.0 ** -20)) * spread + step * n * np.abs(vs).max()
+        assert (np.abs(out[0, r] - o) <= tol).all(), (r, float(np.abs(out[0, r] - o).max()), float(tol.min()))
+        assert (np.abs(lse[0, r] - le) <= hd * 2.0 ** -23 * smax + 2.0 ** -20 + 2.0 ** -22 * abs(le)).all()
