@@ -368,14 +368,13 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
       uint32_t bits[2] = {1, 1}, any = 1;
       int lo[2];  // first old slot beside the sinks that the row sees
       int least = 1;
-      bool there[2];
+      const bool there[2] = {g < p.M && sp.base + row_of[0] >= 0, g + 8 < p.M && sp.base + row_of[1] >= 0};
       if (plain) {
         lo[0] = lo[1] = a.window ? sp.base + 1 - a.window : 0;
       } else {
         uint32_t anc = 0;
         if (lane < rows)
           anc = a.mask ? (uint32_t)a.mask[(long long)seq * rows + lane] & ((1u << rows) - 1) : (2u << lane) - 1;
-        any = __reduce_or_sync(0xffffffffu, anc);
         least = __reduce_min_sync(0xffffffffu, lane < rows ? __popc(anc) : 32);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -393,9 +392,8 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
           bits[0] &= keep[0];
           bits[1] &= keep[1];
         }
+        any = __reduce_or_sync(0xffffffffu, (there[0] ? bits[0] : 0u) | (there[1] ? bits[1] : 0u));
       }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) there[h] = g + 8 * h < p.M && sp.base + row_of[h] >= 0;
       const int first_seen = a.window ? sp.base + least - a.window : 0;  // beside the sinks, by any row
       uint32_t qf[KS][4];
       wait(&q_full[r & 1], (r >> 1) & 1);

@@ -157,7 +157,7 @@ struct PfSeq {
   int lo, end;                                 // of the last range asked for
   __device__ __forceinline__ void see(const PfParams& p, int f, int g) {
     const bool tree = !p.a.q_start;
-    const int p_lo = tree ? base + least - 1 : base + f / p.group;
+    const int p_lo = tree ? base + min(least, p.a.window) - 1 : base + f / p.group;  // a tree's new slots go by its masks, not by lo
     end = tree ? len : base + (g - 1) / p.group + 1;
     lo = p.a.window ? max(0, p_lo - p.a.window + 1) : 0;
   }
@@ -179,6 +179,7 @@ __device__ __forceinline__ PfSeq pf_seq(const PfParams& p, int i) {
     if (s.first != x || next != y || next < s.first) pg_status(p.c.status, VP_DEV_ERR_SLOT);
     s.n_new = max(0, next - s.first);
   } else if (p.a.window && p.a.mask) {
+    s.least = p.a.rows;
     for (int r = 0; r < p.a.rows; ++r)
       s.least = min(s.least, __popc((uint32_t)p.a.mask[(long long)i * p.a.rows + r] & ((1u << p.a.rows) - 1)));
   }
@@ -810,7 +811,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           const int place = s.base + __popc(__shfl_sync(0xffffffffu, anc, j)) - 1;
           if (!a.window || pos - place < a.window || place < a.sinks) keep |= 1u << j;
         }
-        const uint32_t any = __reduce_or_sync(0xffffffffu, anc);
+        const uint32_t any = __reduce_or_sync(0xffffffffu, s.base + lane >= 0 ? anc & keep : 0u);
         if (lane < PG_MAX_ROWS) in.masks[lane] = (anc & keep) | (uint32_t)__popc(anc) << 16;
         if (lane == 0) in.any = any;
       }

@@ -1014,3 +1014,31 @@ def test_small_weights_of_many_slots(kind, lift, hd, dtype):
         tol = u * np.abs(o) + (u + 2 * (hd * 2.0 ** -23 * smax + 2.0 ** -20)) * spread + step * n * np.abs(vs).max()
         assert (np.abs(out[0, r] - o) <= tol).all(), (r, float(np.abs(out[0, r] - o).max()), float(tol.min()))
         assert (np.abs(lse[0, r] - le) <= hd * 2.0 ** -23 * smax + 2.0 ** -20 + 2.0 ** -22 * abs(le)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nkv", [(4, 2), (14, 2)])  # both attention kernels
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (3, 2), (40, 0)])
+def test_slots_that_no_row_sees_hold_anything(nq, nkv, window, sinks):
+    """NaN and infinities in every slot that no row of the call sees: new slots outside all masks, new slots in a mask that the
+    window has left behind, new slots that only rows before the first slot name, old slots just before every row's window."""
+    rng = np.random.default_rng(26 + window)
+    hd, ps, rows = 64, 16, 5
+    lens = [300, 3, 77, 5, 140]
+    masks = np.array([[0b00001, 0b00000, 0b00101, 0b00110, 0b00111], [0b11111] * 2 + [0b00100, 0b01000, 0b01100], [0b11111] * 5,
+                      [0] * 5, [0b00011, 0b00011, 0b00111, 0b01110, 0b10110]])
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, ps, torch.float16, fill=float("nan"))
+    hidden = 0
+    for i, n in enumerate(lens):
+        seen = O.sees_tree(n, [int(m) for m in masks[i]], window, sinks).any(0)
+        for j in np.flatnonzero(~seen):
+            at = int(table[i, j // ps]), slice(None), j % ps
+            kv.k[at], kv.v[at] = float("nan"), float("inf") if j % 2 else float("nan")
+            k[at], v[at] = 0, 0
+            hidden += 1
+    assert hidden > 0
+    q = torch.from_numpy(rng.standard_normal((len(lens), rows, nq, hd)).astype(np.float32)).half()
+    out, lse = kv.decode(q.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), mask=torch.from_numpy(masks.astype(np.int32)).cuda(),
+                         window=window, sinks=sinks, return_lse=True)
+    kv.check()
+    compare(out, lse, want_decode(q.double().numpy(), k, v, table, lens, masks, window, sinks, hd ** -0.5, ps), torch.float16, hd)
