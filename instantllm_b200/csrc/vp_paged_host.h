@@ -43,7 +43,8 @@ int check_cache(const vp_paged* c) {
 
 bool bad_strides(int64_t a, int64_t b, int unit) { return a % unit || b % unit; }
 
-int check_attn(const vp_paged* c, const vp_paged_attn* a) {
+// prompts: q_start names the rows, and what only a decode call has (request strides, masks) is not looked at
+int check_attn(const vp_paged* c, const vp_paged_attn* a, bool prompts) {
   if (const int e = check_cache(c)) return e;
   if (!a) return pfail(VP_ERR_ARG, "null arguments");
   if (a->n < 0 || a->rows < 0 || a->n > (1 << 24)) return pfail(VP_ERR_ARG, "n or rows out of range");
@@ -55,7 +56,7 @@ int check_attn(const vp_paged* c, const vp_paged_attn* a) {
   if (!a->q || !a->out || !a->lens) return pfail(VP_ERR_ARG, "null q, out or lens");
   if (off16(a->q) || off16(a->out)) return pfail(VP_ERR_ARG, "q and out must be 16-byte aligned");
   if (bad_strides(a->q_row, a->q_head, 8) || bad_strides(a->out_row, a->out_head, 8) ||
-      bad_strides(a->q_seq, a->out_seq, 8))
+      (!prompts && bad_strides(a->q_seq, a->out_seq, 8)))
     return pfail(VP_ERR_ARG, "strides of q and out must be multiples of 8 elements");
   if (!a->work || (reinterpret_cast<uintptr_t>(a->work) & 255)) return pfail(VP_ERR_ARG, "work must be 256-byte aligned");
   if (a->work_bytes < vp_paged_work_bytes(c->head_dim, a->n_q, c->n_kv, a->rows))

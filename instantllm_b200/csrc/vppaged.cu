@@ -217,7 +217,7 @@ size_t vp_paged_work_bytes(int32_t head_dim, int32_t n_q, int32_t n_kv, int32_t 
 }
 
 int vp_paged_decode(const vp_paged* c, const vp_paged_attn* a, void* stream) try {
-  if (const int e = check_attn(c, a)) return e;
+  if (const int e = check_attn(c, a, false)) return e;
   if (a->rows > PG_MAX_ROWS) return pfail(VP_ERR_ARG, "a decode call takes 1 to 16 rows per request");
   if (a->n == 0 || a->rows == 0) return VP_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -55,10 +55,10 @@ int pg_tiles(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
 }
 
 extern "C" int vp_paged_prefill(const vp_paged* c, const vp_paged_attn* a, void* stream) try {
-  if (const int e = check_attn(c, a)) return e;
+  if (const int e = check_attn(c, a, true)) return e;
   if (a->n == 0 || a->rows == 0) return VP_OK;
   if (!a->q_start) return pfail(VP_ERR_ARG, "null q_start");
-  vp_paged_attn t = in_range(*a);  // what only a decode call has is not looked at
+  vp_paged_attn t = in_range(*a);
   t.q_seq = t.out_seq = 0;
   t.mask = nullptr;
   return pg_tiles(*c, t, static_cast<cudaStream_t>(stream));

@@ -1042,3 +1042,33 @@ def test_slots_that_no_row_sees_hold_anything(nq, nkv, window, sinks):
                          window=window, sinks=sinks, return_lse=True)
     kv.check()
     compare(out, lse, want_decode(q.double().numpy(), k, v, table, lens, masks, window, sinks, hd ** -0.5, ps), torch.float16, hd)
+
+
+def test_prompt_calls_look_at_no_request_strides(lib):
+    """Request strides of any value pass a prompt call's checks (here up to the next refusal, that of q_start) and are refused
+    by a decode call; no device is needed."""
+    c = good_cache()
+    for kw in (dict(q_seq=3), dict(out_seq=-5), dict(q_seq=2 ** 63 - 1, out_seq=-(2 ** 63) + 1)):
+        a = good_attn(q_start=None, **kw)
+        assert lib.vp_paged_prefill(ctypes.addressof(c), ctypes.addressof(a), None) == -1
+        assert b"q_start" in lib.vp_last_error()
+        a = good_attn(n=2, **kw)
+        assert lib.vp_paged_decode(ctypes.addressof(c), ctypes.addressof(a), None) == -1
+        assert b"strides" in lib.vp_last_error()
+
+
+@pytest.mark.gpu
+def test_c_prompt_call_with_odd_request_strides():
+    """The same through the C ABI: the outputs are those of the Python call."""
+    rng = np.random.default_rng(27)
+    kv, *_ = make_cache(rng, [50, 20], 2, 64, 16, torch.float16)
+    q = torch.from_numpy(rng.standard_normal((60, 4, 64)).astype(np.float32)).half().cuda()
+    ln, starts = torch.tensor([50, 20], dtype=torch.int32).cuda(), torch.tensor([0, 45, 60], dtype=torch.int32).cuda()
+    want = kv.prefill(q, starts, ln)
+    lib, out = _lib.load(), torch.zeros_like(q)
+    work = torch.zeros(lib.vp_paged_work_bytes(64, 4, 2, 60), dtype=torch.uint8, device="cuda")
+    a = _lib.VpPagedAttn(q.data_ptr(), out.data_ptr(), None, ln.data_ptr(), None, 0, starts.data_ptr(), work.data_ptr(), work.numel(),
+                         12345, 256, 64, -3, 256, 64, 0.125, 2, 60, 4, 0, 0)
+    _lib.check(lib.vp_paged_prefill(ctypes.addressof(kv._c), ctypes.addressof(a), torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
