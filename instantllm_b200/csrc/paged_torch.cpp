@@ -27,6 +27,9 @@ const at::Tensor& tensor(PyObject* o, const char* name) {
   return THPVariable_Unpack(o);
 }
 
+// The stride of a dimension; torch leaves any number in those of one element, which mean nothing.
+int64_t stride(const at::Tensor& t, int d) { return t.size(d) == 1 ? 0 : t.stride(d); }
+
 // An int argument, held within 32 bits (a window past every length is no window).
 int32_t small(PyObject* o) {
   const long x = PyLong_AsLong(o);
@@ -115,10 +118,10 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     r.k = k.const_data_ptr();
     r.v = v.const_data_ptr();
     r.q_out = out.data_ptr();
-    r.q_row = q.stride(0), r.q_head = q.stride(1);
-    r.k_row = k.stride(0), r.k_head = k.stride(1);
-    r.v_row = v.stride(0), r.v_head = v.stride(1);
-    r.out_row = out.stride(0), r.out_head = out.stride(1);
+    r.q_row = stride(q, 0), r.q_head = stride(q, 1);
+    r.k_row = stride(k, 0), r.k_head = stride(k, 1);
+    r.v_row = stride(v, 0), r.v_head = stride(v, 1);
+    r.out_row = stride(out, 0), r.out_head = stride(out, 1);
     r.type = in == at::kFloat ? VP_T_F32 : c.type;
     r.rows = (int32_t)n;
     r.n_q = (int32_t)q.size(1);
@@ -170,10 +173,10 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     t.q = q.const_data_ptr();
     t.out = out.data_ptr();
     const int heads = (int)q.dim() - 2;
-    t.q_head = q.stride(heads), t.out_head = out.stride(heads);
-    if (prompts) t.q_row = q.stride(0), t.out_row = out.stride(0);
-    else t.q_seq = q.stride(0), t.out_seq = out.stride(0);
-    if (!prompts && !one) t.q_row = q.stride(1), t.out_row = out.stride(1);
+    t.q_head = stride(q, heads), t.out_head = stride(out, heads);
+    if (prompts) t.q_row = stride(q, 0), t.out_row = stride(out, 0);
+    else t.q_seq = stride(q, 0), t.out_seq = stride(out, 0);
+    if (!prompts && !one) t.q_row = stride(q, 1), t.out_row = stride(out, 1);
     t.scale = a[11] == Py_None ? 1.f / std::sqrt((float)c.head_dim) : (float)PyFloat_AsDouble(a[11]);
     t.n = (int32_t)n;
     t.rows = (int32_t)rows;

@@ -1072,3 +1072,79 @@ def test_c_prompt_call_with_odd_request_strides():
     _lib.check(lib.vp_paged_prefill(ctypes.addressof(kv._c), ctypes.addressof(a), torch.cuda.current_stream().cuda_stream))
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+def odd(t, dims):
+    """t in memory of its own whose strides in these dimensions, all of one element, are odd numbers."""
+    shape = list(t.shape)
+    assert all(shape[d] == 1 for d in dims)
+    strides = [7 + 2 * d if d in dims else x for d, x in enumerate(t.stride())]
+    return t.as_strided(t.shape, strides)
+
+
+@pytest.mark.gpu
+def test_strides_of_extents_of_one_mean_nothing():
+    """One row, one request, one head: whatever torch holds as their strides, the call is the contiguous one's."""
+    rng = np.random.default_rng(28)
+    kv, *_ = make_cache(rng, [50], 1, 64, 16, torch.float16)
+    ln, starts = torch.tensor([50], dtype=torch.int32).cuda(), torch.tensor([0, 1], dtype=torch.int32).cuda()
+    idx = [torch.tensor([i], dtype=torch.int32).cuda() for i in (0, 49, 49)]
+    rope = paged.rope_table(50)
+    for nq, dims in ((1, (0, 1, 2)), (4, (0, 1))):
+        q = torch.from_numpy(rng.standard_normal((1, 1, nq, 64)).astype(np.float32)).half().cuda()
+        want = kv.decode(q, ln)
+        assert torch.equal(kv.decode(odd(q, dims), ln, out=odd(torch.zeros_like(q), dims)), want)
+        flat = tuple(d - 1 for d in dims if d)
+        assert torch.equal(kv.decode(odd(q[0], flat), ln), want[0])
+        assert torch.equal(kv.prefill(odd(q[0], flat), starts, ln, out=odd(torch.zeros_like(q[0]), flat)), kv.prefill(q[0], starts, ln))
+        k, v = (torch.from_numpy(rng.standard_normal((1, 1, 64)).astype(np.float32)).half().cuda() for _ in range(2))
+        turned = kv.append(q[0], k, v, *idx, rope)
+        held = kv.k.clone(), kv.v.clone()
+        got = kv.append(odd(q[0], flat), odd(k, (0, 1)), odd(v, (0, 1)), *idx, rope, out=odd(torch.zeros_like(q[0]), flat))
+        assert torch.equal(got, turned) and torch.equal(kv.k, held[0]) and torch.equal(kv.v, held[1])
+    kv.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq", [4, 14])
+def test_results_into_given_tensors_and_strided_queries(nq):
+    """out= with strides of its own, four-dimensional queries that are slices, pools whose heads lie further apart than their
+    slots: the bits of the contiguous call, and nothing beside them."""
+    rng = np.random.default_rng(29)
+    n, rows, hd, nkv, ps, lens = 3, 5, 64, 2, 16, [300, 40, 77]
+    kv, k, v, table = make_cache(rng, lens, nkv, hd, ps, torch.float16)
+    wide = torch.full((2, kv.pages, nkv + 1, ps + 3, hd + 8), 5.0, dtype=torch.float16, device="cuda")
+    for x, y in zip(wide, (kv.k, kv.v)):
+        x[:, :nkv, :ps, :hd] = y
+    far = paged.PagedLayer(wide[0, :, :nkv, :ps, :hd], wide[1, :, :nkv, :ps, :hd], kv.table)
+    big = torch.from_numpy(rng.standard_normal((n, rows + 2, nq + 3, hd + 8)).astype(np.float32)).half().cuda()
+    q = big[:, 1:rows + 1, 2:nq + 2, 8:]
+    ln, starts = torch.tensor(lens, dtype=torch.int32).cuda(), torch.arange(n + 1, dtype=torch.int32).cuda() * rows
+
+    def given(*shape):
+        x = torch.full((*shape[:-2], shape[-2] + 1, shape[-1] + 8), 9.0, dtype=torch.float16, device="cuda")
+        return x, x[..., :shape[-2], :shape[-1]]
+
+    want, wl = kv.decode(q.contiguous(), ln, return_lse=True)
+    for c in (kv, far):
+        whole, out = given(n, rows, nq, hd)
+        got, gl = c.decode(q, ln, out=out, return_lse=True)
+        assert got.data_ptr() == out.data_ptr() and torch.equal(out, want) and torch.equal(gl, wl)
+        out.fill_(9)
+        assert bool((whole == 9).all())
+        whole, out = given(n * rows, nq, hd)
+        flat = q.contiguous().view(n * rows, nq, hd)
+        c.prefill(flat, starts, ln, out=out)
+        assert torch.equal(out, kv.prefill(flat, starts, ln))
+        out.fill_(9)
+        assert bool((whole == 9).all())
+        c.check()
+    x = torch.from_numpy(rng.standard_normal((n, 2 * nkv, hd)).astype(np.float32)).half().cuda()
+    seq, last = torch.arange(n, dtype=torch.int32).cuda(), ln - 1
+    a = kv.append(q[:, 0].contiguous(), x[:, :nkv], x[:, nkv:], seq, last, last, paged.rope_table(400))
+    whole, out = given(n, nq, hd)
+    far.append(q[:, 0], x[:, :nkv], x[:, nkv:], seq, last, last, paged.rope_table(400), out=out)
+    assert torch.equal(out, a) and torch.equal(far.k, kv.k) and torch.equal(far.v, kv.v)
+    out.fill_(9)
+    far.k.fill_(5), far.v.fill_(5)
+    assert bool((whole == 9).all()) and bool((wide == 5).all())
