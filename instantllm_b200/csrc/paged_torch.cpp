@@ -1,6 +1,7 @@
 // Python side of the paged-cache operators (instantllm_b200/paged.py): checks the tensors of a call, allocates its results and
 // hands it to the C ABI (include/vpass.h, vp_paged_*). Written against torch's C++ tensors because a call of a few
 // microseconds on the GPU took 7 us to check and pack in Python.
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -8,6 +9,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <stdexcept>
 #include <string>
 
@@ -25,6 +27,13 @@ void want(bool ok, const std::string& what) {
 const at::Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) throw Refused(std::string(name) + " must be a tensor");
   return THPVariable_Unpack(o);
+}
+
+// The operators have no backward: a result that silently has no gradient would be wrong.
+void no_grad(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : ts)
+    want(!t->requires_grad(), "the paged operators have no gradients: call them under torch.no_grad() or on detached tensors");
 }
 
 // The stride of a dimension; torch leaves any number in those of one element, which mean nothing.
@@ -89,6 +98,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const Call call(a[0], a[1]);
     const vp_paged& c = *call.c;
     const at::Tensor &q = tensor(a[2], "q"), &k = tensor(a[3], "k"), &v = tensor(a[4], "v");
+    no_grad({&q, &k, &v});
     const at::ScalarType in = q.scalar_type();
     want(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes() && k.scalar_type() == in && v.scalar_type() == in,
          "q, k and v must be [rows][heads][head_dim] of one type");
@@ -142,6 +152,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const at::Tensor &q = tensor(a[4], "q"), &lens = tensor(a[5], "lens");
     want(q.dim() == 3 || (q.dim() == 4 && !prompts), prompts ? "q must be [rows][query heads][head_dim]"
                                                              : "q must be [n][rows][query heads][head_dim] or [n][query heads][head_dim]");
+    no_grad({&q});
     const bool one = q.dim() == 3 && !prompts;
     want(q.size(-1) == c.head_dim && q.scalar_type() == call.type && call.here(q) && q.stride(-1) == 1,
          "q must have the cache's type, device and head_dim, elements of a head adjacent");

@@ -9,8 +9,9 @@
 
 `kv[l]` is a PagedLayer; it can also be built over pools and a table that the caller owns. Like an engine's context, a cache
 (and the layers of one PagedKV) serves one stream at a time. Calls run on torch's current stream, allocate only their
-results, synchronise nothing and can be captured in a CUDA graph; what the device finds wrong (a page or slot outside the
-table) is told by `check()`. The reference keeps one contiguous cache of one request (Engine.swift:113).
+results, synchronise nothing and can be captured in a CUDA graph; they have no gradients, and refuse tensors that want
+one. What the device finds wrong (a page or slot outside the table) is told by `check()`. The reference keeps one contiguous
+cache of one request (Engine.swift:113).
 """
 from __future__ import annotations
 

@@ -1148,3 +1148,28 @@ def test_results_into_given_tensors_and_strided_queries(nq):
     out.fill_(9)
     far.k.fill_(5), far.v.fill_(5)
     assert bool((whole == 9).all()) and bool((wide == 5).all())
+
+
+@pytest.mark.gpu
+def test_tensors_that_want_a_gradient_are_refused():
+    """The operators have no backward, so they say so instead of returning a result without one."""
+    rng = np.random.default_rng(30)
+    kv, *_ = make_cache(rng, [20], 2, 64, 16, torch.float16)
+    q = torch.from_numpy(rng.standard_normal((1, 14, 64)).astype(np.float32)).half().cuda()
+    x = torch.from_numpy(rng.standard_normal((1, 4, 64)).astype(np.float32)).half().cuda()
+    ln, starts = torch.tensor([20], dtype=torch.int32).cuda(), torch.tensor([0, 1], dtype=torch.int32).cuda()
+    idx = [torch.tensor([i], dtype=torch.int32).cuda() for i in (0, 19, 19)]
+    rope = paged.rope_table(20)
+    g, y = q.clone().requires_grad_(), x.clone().requires_grad_()
+    calls = [lambda q, x: kv.decode(q, ln), lambda q, x: kv.prefill(q, starts, ln),
+             lambda q, x: kv.append(q, x[:, :2], x[:, 2:], *idx, rope)]
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call(g, y)
+        want = call(q, x)
+        with torch.no_grad():
+            assert torch.equal(call(g, y), want)
+        assert torch.equal(call(g.detach(), y.detach()), want)
+    with pytest.raises(ValueError, match="gradient"):
+        calls[2](q, y)
+    kv.check()
