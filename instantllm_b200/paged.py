@@ -203,8 +203,13 @@ class PagePool:
         self.page_size, self.width = page_size, width
         self.held = [[] for _ in range(max_seqs)]
 
+    def _known(self, seq: int) -> None:
+        if not 0 <= seq < len(self.held):
+            raise IndexError(f"request {seq}, and a table of {len(self.held)}")
+
     def reserve(self, seq: int, n_slots: int):
         """(first new entry of the request's row, the new pages). Nothing changes when the pool cannot serve it."""
+        self._known(seq)
         held = self.held[seq]
         need = -(-n_slots // self.page_size)
         if need > self.width:
@@ -218,6 +223,7 @@ class PagePool:
         return at, new
 
     def release(self, seq: int):
+        self._known(seq)
         held, self.held[seq] = self.held[seq], []
         self.free.extend(reversed(held))
         return held

@@ -1173,3 +1173,15 @@ def test_tensors_that_want_a_gradient_are_refused():
     with pytest.raises(ValueError, match="gradient"):
         calls[2](q, y)
     kv.check()
+
+
+def test_page_pool_knows_its_requests():
+    """A request below zero is none: it does not stand for one counted from the end."""
+    p = paged.PagePool(6, 16, 3, 4)
+    p.reserve(2, 20)
+    for seq in (-1, -3, 3):
+        with pytest.raises(IndexError, match="request"):
+            p.reserve(seq, 64)
+        with pytest.raises(IndexError, match="request"):
+            p.release(seq)
+    assert p.held == [[], [], [0, 1]] and len(p.free) == 4
