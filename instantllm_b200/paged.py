@@ -182,6 +182,12 @@ class PagedKV:
         if new:
             self.table[seq, at:at + len(new)] = torch.tensor(new, dtype=torch.int32).to(self.device)
 
+    def reserve_all(self, slots: dict) -> None:
+        """reserve(request, slots) for each of several requests, or VpError and no page to any of them."""
+        self._pool.fits(slots)
+        for seq, n_slots in slots.items():
+            self.reserve(seq, n_slots)
+
     def release(self, seq: int) -> None:
         """All pages of request `seq` go back to the pool."""
         if self._pool.release(seq):
@@ -207,18 +213,25 @@ class PagePool:
         if not 0 <= seq < len(self.held):
             raise IndexError(f"request {seq}, and a table of {len(self.held)}")
 
-    def reserve(self, seq: int, n_slots: int):
-        """(first new entry of the request's row, the new pages). Nothing changes when the pool cannot serve it."""
-        self._known(seq)
-        held = self.held[seq]
-        need = -(-n_slots // self.page_size)
-        if need > self.width:
-            raise VpError(f"{n_slots} slots, and a table row of {self.width} pages of {self.page_size}")
-        more = need - len(held)
+    def fits(self, slots: dict) -> int:
+        """Pages that the requests lack for these numbers of slots; VpError when the pool or a row of the table cannot hold them."""
+        more = 0
+        for seq, n_slots in slots.items():
+            self._known(seq)
+            need = -(-n_slots // self.page_size)
+            if need > self.width:
+                raise VpError(f"{n_slots} slots, and a table row of {self.width} pages of {self.page_size}")
+            more += max(0, need - len(self.held[seq]))
         if more > len(self.free):
             raise VpError(f"{more} pages wanted, {len(self.free)} free")
+        return more
+
+    def reserve(self, seq: int, n_slots: int):
+        """(first new entry of the request's row, the new pages). Nothing changes when the pool cannot serve it."""
+        more = self.fits({seq: n_slots})
+        held = self.held[seq]
         at = len(held)
-        new = [self.free.pop() for _ in range(max(0, more))]
+        new = [self.free.pop() for _ in range(more)]
         held.extend(new)
         return at, new
 

@@ -80,8 +80,7 @@ class PagedEngine:
         n = [len(prompts[s]) for s in seqs]
         if min(n) < 1:
             raise ValueError("a prompt has at least one token")
-        for s, k in zip(seqs, n):
-            self.kv.reserve(s, self.lens[s] + k)
+        self.kv.reserve_all({s: self.lens[s] + k for s, k in zip(seqs, n)})
         slot = np.concatenate([self.lens[s] + np.arange(k) for s, k in zip(seqs, n)])
         starts = np.concatenate([[0], np.cumsum(n)])
         ids, lens = self._i32(seqs), self._i32([self.lens[s] + k for s, k in zip(seqs, n)])
@@ -103,8 +102,7 @@ class PagedEngine:
         keys and values move up behind the root (the commit's compaction). keep: rows that stay without commit."""
         seqs = list(trees)
         rows = max(t["n"] for t in trees.values())
-        for s in seqs:
-            self.kv.reserve(s, self.lens[s] + rows)
+        self.kv.reserve_all({s: self.lens[s] + rows for s in seqs})
         base = np.array([self.lens[s] for s in seqs])
         pad = [list(range(trees[s]["n"])) + [0] * (rows - trees[s]["n"]) for s in seqs]  # rows past a tree are its root again
         real = np.array([[r < trees[s]["n"] for r in range(rows)] for s in seqs])

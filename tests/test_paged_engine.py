@@ -124,3 +124,37 @@ def test_dense_layouts_match_the_oracle():
     for fmt in ("q4", "q8", "q8g32", "f16"):
         m = synth.make_matrix(fmt, 32, 128, rng)
         assert np.array_equal(_dense(m, "cpu").numpy(), Q.dequant(m).astype(np.float16))
+
+
+def test_a_batch_gets_all_its_pages_or_none():
+    """Requests that the pool cannot hold together leave no page behind with any of them (host side)."""
+    from instantllm_b200 import paged
+    from instantllm_b200._lib import VpError
+
+    p = paged.PagePool(6, 16, 3, 4)
+    assert p.fits({0: 32, 1: 64}) == 6 and p.fits({0: 0}) == 0
+    for bad in ({0: 33, 1: 64}, {0: 16, 2: 65}):
+        with pytest.raises(VpError):
+            p.fits(bad)
+    with pytest.raises(IndexError):
+        p.fits({0: 16, -1: 16})
+    assert p.held == [[], [], []] and len(p.free) == 6
+    p.reserve(0, 20)
+    assert p.fits({0: 32, 1: 64}) == 4
+
+
+@pytest.mark.gpu
+def test_a_refused_batch_takes_no_pages(model):
+    """The first prompt of a batch fits and the second does not: neither keeps pages, and each alone is served."""
+    from instantllm_b200._lib import VpError
+    from instantllm_b200.paged_engine import PagedEngine
+
+    eng = PagedEngine(model[2], n_pages=12, page_size=16, max_seqs=3, max_len=160)
+    with pytest.raises(VpError, match="pages wanted"):
+        eng.prefill({0: prompt(100, 1), 1: prompt(120, 2)})
+    assert eng.kv.free_pages == 12 and eng.lens == [0, 0, 0]
+    eng.prefill({0: prompt(100, 1)})
+    with pytest.raises(VpError, match="pages wanted"):
+        eng.prefill({0: prompt(30, 1), 1: prompt(70, 2)})
+    assert eng.kv.free_pages == 5 and eng.lens == [100, 0, 0]
+    eng.kv.check()
