@@ -101,20 +101,28 @@ class PagedEngine:
         request commits: the longest path whose drafts equal their parents' argmax, then one more. The accepted rows'
         keys and values move up behind the root (the commit's compaction). keep: rows that stay without commit."""
         seqs = list(trees)
-        rows = max(t["n"] for t in trees.values())
-        self.kv.reserve_all({s: self.lens[s] + rows for s in seqs})
-        base = np.array([self.lens[s] for s in seqs])
-        pad = [list(range(trees[s]["n"])) + [0] * (rows - trees[s]["n"]) for s in seqs]  # rows past a tree are its root again
-        real = np.array([[r < trees[s]["n"] for r in range(rows)] for s in seqs])
-        tok = [[roots[s]] + list(trees[s]["tok"][1:trees[s]["n"]]) for s in seqs]
-        tok = np.array([[t[i] for i in p] for t, p in zip(tok, pad)])
-        depth = np.array([[trees[s]["depth"][i] for i in p] for s, p in zip(seqs, pad)])
-        masks = ancestor_masks([trees[s] for s in seqs])[:, :rows].contiguous().to(self.device)
-        ids, lens = self._i32(seqs), self._i32(base + rows)
-        x = self._rows(tok.ravel(), np.where(real, np.array(seqs)[:, None], -1).ravel(), (base[:, None] + np.arange(rows)).ravel(),
+        n = np.array([trees[s]["n"] for s in seqs])
+        rows = int(n.max())
+        self.kv.reserve_all({s: self.lens[s] + k for s, k in zip(seqs, n.tolist())})
+        base, pad = np.array([self.lens[s] for s in seqs]), rows - n
+        # All requests of a call have as many rows, the last slots of each: a smaller tree stands behind padding rows, which are
+        # its last old slots (not stored again), so that it takes no slot beyond its own.
+        at = np.arange(rows) - pad[:, None]  # row of the tree, negative for padding
+        real, tree_row = at >= 0, np.maximum(at, 0)
+        tok = np.array([[roots[s]] + [trees[s]["tok"][r] if 0 < r < trees[s]["n"] else 0 for r in range(1, rows)] for s in seqs])
+        depth = np.array([[trees[s]["depth"][r] if r < trees[s]["n"] else 0 for r in range(rows)] for s in seqs])
+        tok, depth = np.take_along_axis(tok, tree_row, 1), np.take_along_axis(depth, tree_row, 1)
+        anc = ancestor_masks([trees[s] for s in seqs]).numpy()[:, :rows].astype(np.int64)
+        below = (1 << pad)[:, None] - 1  # the old slots among the call's rows
+        anc = np.where(real, np.take_along_axis(anc, tree_row, 1) << pad[:, None] | below, (2 << np.arange(rows)) - 1)
+        masks, ids, lens = self._i32(anc), self._i32(seqs), self._i32(base + n)
+        x = self._rows(tok.ravel(), np.where(real, np.array(seqs)[:, None], -1).ravel(), (base[:, None] + tree_row).ravel(),
                        (base[:, None] + depth).ravel(),
                        lambda kv, q: kv.decode(q.view(len(seqs), rows, N_Q, HEAD), lens, mask=masks, seqs=ids, window=self.window,
                                                sinks=self.sinks))
+        if pad.any():  # back in the trees' order; rows past a tree are its root again
+            order = np.arange(len(seqs))[:, None] * rows + pad[:, None] + np.where(np.arange(rows) < n[:, None], np.arange(rows), 0)
+            x = x[self._i32(order.ravel()).long()]
         logits = self._logits(x).view(len(seqs), rows, -1)
         if not commit:
             for s in seqs:

@@ -126,6 +126,65 @@ def test_dense_layouts_match_the_oracle():
         assert np.array_equal(_dense(m, "cpu").numpy(), Q.dequant(m).astype(np.float16))
 
 
+@pytest.mark.gpu
+def test_small_trees_beside_large_ones(model):
+    """A request whose own tree still fits its row of the table is served beside one with a larger tree, down to a context of one
+    token; logits against the oracle's tree pass, tokens and lengths as committed alone, and no page beyond a request's own
+    slots."""
+    from oracle import qwen_oracle as Q
+
+    eng, m, _ = model
+    rng = np.random.default_rng(10)
+    prompts = {0: prompt(155, 8), 1: prompt(40, 9), 4: prompt(1, 10), 5: prompt(9, 11)}
+    sizes = {0: 5, 1: 16, 4: 1, 5: 7}
+    first = dict(zip(prompts, eng.prefill(prompts).argmax(-1).tolist()))
+    caches = {}
+    for s, p in prompts.items():
+        caches[s] = Q.KVCache(2, 180)
+        Q.forward_causal(m, caches[s], p, 0)
+    trees = {s: synth.seeded_tree(rng, Q.greedy(m, prompts[s], 10)[0], n=k, p_match=0.9, vocab=VOCAB) if k > 1 else synth.root_tree()
+             for s, k in sizes.items()}
+    logits, out = eng.verify(trees, first)
+    eng.kv.check()
+    logits = logits.cpu().numpy()
+    for i, s in enumerate(trees):
+        n = trees[s]["n"]
+        want = Q.tree_pass(m, caches[s].copy(), len(prompts[s]), first[s], trees[s])
+        assert np.abs(logits[i, :n] - want).max() < 0.05
+        assert np.array_equal(logits[i, n:], np.repeat(logits[i, :1], logits.shape[1] - n, 0))
+        assert len(eng.kv._pool.held[s]) == -(-(len(prompts[s]) + n) // 16)
+        ids = prompts[s] + [first[s]] + out[s]
+        assert eng.lens[s] == len(ids) - 1
+        if len(ids) <= 160:
+            got = eng.decode({s: ids[-1]})[0].cpu().numpy()
+            assert np.abs(got - Q.forward_causal(m, Q.KVCache(2, 180), ids, 0)).max() < 0.05
+    for s in prompts:
+        eng.release(s)
+    eng.kv.check()
+    assert eng.kv.free_pages == 64
+
+
+@pytest.mark.gpu
+def test_trees_of_different_sizes_under_a_window(model):
+    """The same trees in one call and each in its own, over a window that cuts into the padding: the passes' own bound apart."""
+    from instantllm_b200.paged_engine import PagedEngine
+
+    w = model[2]
+    rng = np.random.default_rng(11)
+    sizes = {0: 16, 1: 3, 2: 1, 3: 9}
+    prompts = {s: prompt(n, 40 + s) for s, n in {0: 60, 1: 35, 2: 20, 3: 4}.items()}
+    for window, sinks in ((6, 2), (20, 0)):
+        eng = PagedEngine(w, n_pages=64, page_size=16, max_seqs=4, max_len=160, window=window, sinks=sinks)
+        first = dict(zip(prompts, eng.prefill(prompts).argmax(-1).tolist()))
+        trees = {s: synth.seeded_tree(rng, [int(x) for x in rng.integers(0, VOCAB, 16)], n=k, vocab=VOCAB) if k > 1 else synth.root_tree()
+                 for s, k in sizes.items()}
+        got = eng.verify(trees, first, commit=False)[0].cpu().numpy()
+        for i, s in enumerate(trees):
+            alone = eng.verify({s: trees[s]}, first, commit=False)[0].cpu().numpy()
+            assert np.abs(got[i, :sizes[s]] - alone[0]).max() < 0.05
+        eng.kv.check()
+
+
 def test_a_batch_gets_all_its_pages_or_none():
     """Requests that the pool cannot hold together leave no page behind with any of them (host side)."""
     from instantllm_b200 import paged
