@@ -162,6 +162,8 @@ class PagedEngine:
     def generate(self, prompts: list, max_new: int, tree_fn: Optional[Callable] = None, eos=STOP_IDS) -> list:
         """Greedy token lists of all prompts (up to max_new each, a stop token included). tree_fn(request, committed tokens) ->
         draft tree whose root is the last of them; without it, one token a step."""
+        if max_new < 1:
+            return [[] for _ in prompts]
         out = {s: [] for s in range(len(prompts))}
         live = dict(enumerate(prompts))
         first = self.prefill(live).argmax(-1).tolist()

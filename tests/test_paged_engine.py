@@ -217,3 +217,13 @@ def test_a_refused_batch_takes_no_pages(model):
         eng.prefill({0: prompt(30, 1), 1: prompt(70, 2)})
     assert eng.kv.free_pages == 5 and eng.lens == [100, 0, 0]
     eng.kv.check()
+
+
+@pytest.mark.gpu
+def test_generate_no_tokens(model):
+    """A limit of no tokens gives none, and touches no request."""
+    eng = model[0]
+    free = eng.kv.free_pages
+    assert eng.generate([prompt(5, 1), prompt(9, 2)], 0) == [[], []]
+    assert [len(t) for t in eng.generate([prompt(5, 1), prompt(9, 2)], 1)] == [1, 1]
+    assert eng.kv.free_pages == free and eng.lens == [0] * 6
