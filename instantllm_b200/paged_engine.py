@@ -16,6 +16,7 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
+from ._lib import VpError
 from .paged import PagedKV, ancestor_masks, rope_table
 from .synth import FFN, HIDDEN, STOP_IDS
 
@@ -161,29 +162,39 @@ class PagedEngine:
 
     def generate(self, prompts: list, max_new: int, tree_fn: Optional[Callable] = None, eos=STOP_IDS) -> list:
         """Greedy token lists of all prompts (up to max_new each, a stop token included). tree_fn(request, committed tokens) ->
-        draft tree whose root is the last of them; without it, one token a step."""
+        draft tree whose root is the last of them; without it, one token a step. Requests 0 .. len(prompts) - 1 must be free,
+        and are again afterwards, also when it fails."""
         if max_new < 1:
             return [[] for _ in prompts]
+        held = [s for s, n in enumerate(self.lens[:len(prompts)]) if n]
+        if held:
+            raise VpError(f"requests {held} hold a context: release them first")
         out = {s: [] for s in range(len(prompts))}
         live = dict(enumerate(prompts))
-        first = self.prefill(live).argmax(-1).tolist()
-        new = {s: [t] for s, t in zip(live, first)}
-        while True:
-            for s in list(new):
-                for t in new[s]:
-                    out[s].append(t)
-                    if t in eos or len(out[s]) == max_new:
-                        self.release(s)
-                        del live[s]
-                        break
-            if not live:
-                self.kv.check()
-                return [out[s] for s in range(len(prompts))]
-            roots = {s: out[s][-1] for s in live}
-            if tree_fn is None:
-                new = {s: [t] for s, t in zip(live, self.decode(roots).argmax(-1).tolist())}
-            else:
-                new = self.verify({s: tree_fn(s, list(prompts[s]) + out[s]) for s in live}, roots)[1]
+        try:
+            first = self.prefill(live).argmax(-1).tolist() if live else []
+            new = {s: [t] for s, t in zip(live, first)}
+            while live:
+                for s in list(new):
+                    for t in new[s]:
+                        out[s].append(t)
+                        if t in eos or len(out[s]) == max_new:
+                            self.release(s)
+                            del live[s]
+                            break
+                if not live:
+                    break
+                roots = {s: out[s][-1] for s in live}
+                if tree_fn is None:
+                    new = {s: [t] for s, t in zip(live, self.decode(roots).argmax(-1).tolist())}
+                else:
+                    new = self.verify({s: tree_fn(s, list(prompts[s]) + out[s]) for s in live}, roots)[1]
+            self.kv.check()
+        finally:  # what a step that failed leaves
+            for s in live:
+                if s < len(self.lens):
+                    self.release(s)
+        return list(out.values())
 
 
 def main() -> None:

@@ -227,3 +227,33 @@ def test_generate_no_tokens(model):
     assert eng.generate([prompt(5, 1), prompt(9, 2)], 0) == [[], []]
     assert [len(t) for t in eng.generate([prompt(5, 1), prompt(9, 2)], 1)] == [1, 1]
     assert eng.kv.free_pages == free and eng.lens == [0] * 6
+
+
+@pytest.mark.gpu
+def test_generate_after_one_that_failed(model):
+    """A generate that runs out of pages half way, or whose drafts raise, leaves the engine as it was: the next one gives the tokens
+    of a fresh engine. Requests that hold a context are not generated onto."""
+    from instantllm_b200._lib import VpError
+    from instantllm_b200.paged_engine import PagedEngine
+
+    eng = PagedEngine(model[2], n_pages=5, page_size=16, max_seqs=3, max_len=160)
+    prompts = [prompt(30, 1), prompt(17, 2)]
+    want = model[0].generate(prompts, 6, eos=())
+
+    def bad(s, ids):
+        if len(ids) > 19:
+            raise KeyError("draft")
+        return synth.root_tree()
+
+    for fails, kind in ((lambda: eng.generate(prompts, 90, eos=()), VpError), (lambda: eng.generate(prompts, 90, tree_fn=bad, eos=()), KeyError),
+                        (lambda: eng.generate([prompt(3, i) for i in range(4)], 5), IndexError)):
+        with pytest.raises(kind):
+            fails()
+        assert eng.lens == [0, 0, 0] and eng.kv.free_pages == 5
+    assert eng.generate(prompts, 6, eos=()) == want
+    eng.prefill({1: prompt(4, 3)})
+    with pytest.raises(VpError, match="release"):
+        eng.generate(prompts, 6)
+    assert eng.lens == [0, 4, 0]
+    eng.release(1)
+    assert eng.generate([], 5) == []
