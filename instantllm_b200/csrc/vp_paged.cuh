@@ -1,5 +1,5 @@
-// Shared parts of the paged-cache operators (include/vpass.h, vp_paged_*): device views of the
-// cache and of a call, visibility of slots, element conversions.
+// Shared parts of the paged-cache operators (include/vpass.h, vp_paged_*): lengths of requests, copies, waits,
+// element conversions.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -17,33 +17,13 @@ __device__ __forceinline__ void pg_status(int32_t* status, int bits) {
   if (status) atomicOr(status, bits);
 }
 
-// A request's row of the table and its length, clipped to what the table holds.
-struct PgSeq {
-  const int32_t* pages;
-  int len;
-};
-__device__ __forceinline__ PgSeq pg_seq(const vp_paged& c, const int32_t* seqs, const int32_t* lens, int i) {
-  const int s = seqs ? seqs[i] : i;
-  int len = lens[i];
+// A request's length, clipped to what its row of the table holds; zero for a request outside the table.
+__device__ __forceinline__ int pg_len(const vp_paged& c, const int32_t* seqs, const int32_t* lens, int i) {
+  const int s = seqs ? seqs[i] : i, len = lens[i];
   const long long cap = (long long)c.max_pages * c.page_size;
-  if (s < 0 || s >= c.n_seqs || len < 0 || len > cap) {
-    pg_status(c.status, VP_DEV_ERR_SLOT);
-    len = s < 0 || s >= c.n_seqs || len < 0 ? 0 : (int)cap;
-  }
-  return {c.table + (s < 0 || s >= c.n_seqs ? 0 : (long long)s * c.table_stride), len};
-}
-
-// Whether a row of a decode call sees a slot. base: slots before the new rows; bits: the row's
-// mask; anc: masks of all new rows (for their positions when a window is set).
-__device__ __forceinline__ bool pg_sees(int slot, int len, int base, uint32_t bits, const uint32_t* anc, int window,
-                                        int sinks) {
-  if (slot >= len) return false;
-  int place = slot;
-  if (slot >= base) {
-    if (!((bits >> (slot - base)) & 1)) return false;
-    if (window) place = base + __popc(anc[slot - base]) - 1;
-  }
-  return !window || base + __popc(bits) - 1 - place < window || place < sinks;
+  const bool there = s >= 0 && s < c.n_seqs && len >= 0;
+  if (!there || len > cap) pg_status(c.status, VP_DEV_ERR_SLOT);
+  return !there ? 0 : len > cap ? (int)cap : len;
 }
 
 // One box of a pool into shared memory: the map's box of slots from `slot` of a page, in panels of 64

@@ -151,7 +151,7 @@ struct DcWalk {
     advance(t_ - t);
   }
   __device__ __forceinline__ void span() {
-    const int len = seq < DC_LENS ? lens_s[seq] : pg_seq(p.c, p.a.seqs, p.a.lens, seq).len;
+    const int len = seq < DC_LENS ? lens_s[seq] : pg_len(p.c, p.a.seqs, p.a.lens, seq);
     sp = dc_span<TS>(len, p.a.rows, p.a.window, p.a.sinks);
   }
   __device__ __forceinline__ bool more() const { return t < t1; }
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
   const int i0 = min(a.n, tid * chunk), i1 = min(a.n, i0 + chunk);
   int mine = 0, most = 0, least = 1 << 30;
   for (int i = i0; i < i1; ++i) {
-    const int len = pg_seq(c, a.seqs, a.lens, i).len;
+    const int len = pg_len(c, a.seqs, a.lens, i);
     if (i < DC_LENS) lens_s[i] = len;
     const int tiles = dc_span<TS>(len, rows, a.window, a.sinks).tiles;
     mine += tiles * c.n_kv;
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
     if (tid == 0 && cta + 1 == G) t1_s = N;
     __syncwarp();
     for (int i = i0, v = at + DC_RUN * c.n_kv * i0; i < i1; ++i) {
-      const int len = i < DC_LENS ? lens_s[i] : pg_seq(c, a.seqs, a.lens, i).len;
+      const int len = i < DC_LENS ? lens_s[i] : pg_len(c, a.seqs, a.lens, i);
       const int tiles = dc_span<TS>(len, rows, a.window, a.sinks).tiles, width = tiles + DC_RUN, end = v + width * c.n_kv;
       auto tile_at = [&](int x) {  // tiles before place x of the count
         const int h = (x - v) / width;
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
     if (cuts == 1 && tid == 0 && s1 == a.n) t1_s = N;
     __syncwarp();
     for (int i = i0; i < i1; ++i) {
-      const int len = i < DC_LENS ? lens_s[i] : pg_seq(c, a.seqs, a.lens, i).len;
+      const int len = i < DC_LENS ? lens_s[i] : pg_len(c, a.seqs, a.lens, i);
       const int tiles = dc_span<TS>(len, rows, a.window, a.sinks).tiles;
       if (i == s0) {
         const int t = at + (q0 - s0 * c.n_kv) * tiles, k = cuts == 1 ? 0 : cta - q0 * cuts;

@@ -183,7 +183,7 @@ __device__ __forceinline__ PfSeq pf_seq(const PfParams& p, int i) {
     for (int r = 0; r < p.a.rows; ++r)
       s.least = min(s.least, __popc((uint32_t)p.a.mask[(long long)i * p.a.rows + r] & ((1u << p.a.rows) - 1)));
   }
-  s.len = pg_seq(p.c, p.a.seqs, p.a.lens, i).len;
+  s.len = pg_len(p.c, p.a.seqs, p.a.lens, i);
   s.row = p.a.seqs ? p.a.seqs[i] : i;
   s.base = s.len - s.n_new;
   s.blocks = (int)(((unsigned)s.n_new * (unsigned)p.group + p.rows - 1) / p.rows);
