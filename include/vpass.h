@@ -360,7 +360,8 @@ void vp_graph_destroy(vp_graph* g);
  * fault: VP_DEV_ERR_PAGE a page outside [0, n_pages), read as zeros and not written;
  * VP_DEV_ERR_SLOT a request, slot, position or length outside the table (or the rotations), dropped
  * or clipped. Slots at or past a request's length, and slots that no row of a call sees, may hold
- * anything, NaN included. */
+ * anything, NaN included; a NaN or an infinity in the values of a slot that some row sees may reach the
+ * request's other rows of the same call too (a weight of zero times it). */
 enum vp_type { VP_T_F16 = 0, VP_T_BF16 = 1, VP_T_F32 = 2 };
 #define VP_DEV_ERR_PAGE 16
 #define VP_DEV_ERR_SLOT 32

@@ -21,10 +21,11 @@
 //    in the work buffer; the CTA that finishes last (a counter per first CTA, back at zero afterwards)
 //    joins them in the order of the slots, so results do not depend on which CTA that is. Of many records,
 //    each eight are first joined by the last CTA of those, in the buffer that the warps' records were in.
-// Measured: 4 requests of 103,871 to 131,072 slots, 32 + 2 x 8 heads of 128, bf16: 267 us, 6.9 TB/s (a plain copy: 6.5;
-// with a producer warp filling a ring for all warps: 430 us). 64 requests of 130 to 2,048 slots, 14 + 2 x 2 heads of
-// 64: 12.8 us; 128 requests with a window of 1,024: 20 us; one request of 257 slots: 6.7 us, of which 2.9 us pass before
-// the first tile is asked for (lengths, shares, pages), 0.9 until it is there, 0.65 a tile, 0.8 for the join.
+// Measured: 4 requests of 103,871 to 131,072 slots, 32 + 2 x 8 heads of 128, bf16: 270 us, 6.8 TB/s (a plain copy: 6.5;
+// calls on one input leave part of it in L2; with a producer warp filling a ring for all warps: 430 us). 64 requests of
+// 130 to 2,048 slots, 14 + 2 x 2 heads of 64: 12.7 us; 128 requests with a window of 1,024: 17.9 us; one request of 257
+// slots: 6.7 us, of which 2.9 us pass before the first tile is asked for (lengths, shares, pages), 0.9 until it is there,
+// 0.65 a tile, 0.8 for the join.
 #pragma once
 #include "vp_paged.cuh"
 
@@ -34,21 +35,20 @@ constexpr int DC_WARPS = 8;                         // consumer warps
 constexpr int DC_JOINERS = 128;                     // threads
 constexpr int DC_THREADS = DC_WARPS * 32 + DC_JOINERS;
 // Packed query rows of a pair: one MMA tile, which reads the cache at HBM speed. With more tiles a pair (this kernel for up
-// to 128 rows, one 16-row tile a warp) 64 requests of 112 rows took 62 us, on the tensor-memory kernel 27.
+// to 128 rows, one 16-row tile a warp) 64 requests of 112 rows took 62 us, on the tensor-memory kernel 25.
 constexpr int DC_ROWS = 16;
 constexpr int DC_TILE = 4096;                       // bytes of K (and of V) per tile
 constexpr int DC_STAGES = 2;                        // per warp
 constexpr int DC_LENS = 2048;                       // lengths kept in shared memory
-// Tiles that a run costs beside its own, in the even shares (64 requests of 130 to 2,048 slots: 13.3 us then, 15.2 without,
-// 12.7 with 10, 14.2 with 24; 200 of 20 to 4,000: 25.6, 40, 26.7, 27.8; 30 of 100 to 4,000, 32 + 2 x 8 heads of 128:
-// 33, 53, 35, 35).
+// Tiles that a run costs beside its own, in the even shares (64 requests of 130 to 2,048 slots: 12.7 us then, 14.2 without,
+// 13.5 with 24; 200 of 20 to 4,000: 23.3, 36.2, 25.5; 30 of 100 to 4,000, 32 + 2 x 8 heads of 128: 32.2, 51, 35).
 constexpr int DC_RUN = 12;
 // Tiles of a CTA's share, at most, for whole pairs: past it the joins they save cost less than CTAs without a last pair
-// (32 + 2 x 8 heads of 128, 40 requests of 2,000 slots: 57 us, 70 with whole pairs; 16 of 16,000: 159 and 168).
+// (32 + 2 x 8 heads of 128, 40 requests of 2,000 slots: 57 us, 70 with whole pairs; 16 of 16,000: 160.2 and 161.5).
 constexpr int DC_SHORT = 64;
 // Rounds of reads (8 records, 128 items of 4 elements), at most, in which the last CTA joins a pair's records by itself;
-// more records go eight at a time. 16 records of 4 rows of 128: 11.1 us a call, 13.1 by eights; 18 of 7 rows of 64 (3 rounds):
-// 21.1 and 22.4; 18 of 16 rows of 128 (12 rounds): 23.7 by eights, 29 otherwise; 50 of 8 rows of 128 (14): 14.9 and 22.
+// more records go eight at a time. 8 records of 4 rows of 128: 9.8 us a call, 10.9 by eights; 18 of them (3 rounds): 29.8
+// and 31; 18 of 16 rows of 128 (12 rounds): 21.5 by eights, 25.9 otherwise; 49 of 8 rows of 128 (14): 15.7 and 22.5.
 constexpr int DC_FLAT = 3;
 constexpr int DC_LEVELS = 3;                        // of joins that leave a record: 8^3 parts a pair, more than CTAs
 
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(DC_THREADS, 1)
   }
   // Even shares of the tiles; or, where the requests are about equally long and the shares small, whole pairs
   // (cuts == 1) or even cuts of them: a pair that ends inside a CTA's share costs a join (16 requests of 300
-  // slots: 7.3 us, 11.3 with even shares; 64 of 1,000: 11.3 and 14.4; 128 with a window of 1,024: 20.4 and 22.7).
+  // slots: 7.3 us, 10.6 with even shares; 64 of 1,000: 10.8 and 13.2; 128 with a window of 1,024: 17.9 and 19.5).
   const int cta = blockIdx.x, pairs = a.n * c.n_kv;
   int G = min((N + p.min_tiles - 1) / p.min_tiles, (int)gridDim.x), cuts = 0;
   if (4ll * most <= 5ll * least && N <= DC_SHORT * (int)gridDim.x) {

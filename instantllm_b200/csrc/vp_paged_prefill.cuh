@@ -25,11 +25,12 @@
 // one that finishes last (a counter per row tile, back at zero afterwards) joins them in order. A
 // scheduler warp looks up the next piece, and its K and V arrive, while the present one is computed.
 //
-// Measured: a prompt of 8,192 rows, 32 + 2 x 8 heads of 128, bf16: 493 us, 1,116 TFLOP/s (67% of cuBLAS at bf16); of 64:
-// 388 us, where the exponentials alone are 50% of the tensor rate. 16 prompts of 186 to 2,048 rows, 14 + 2 x 2 heads of 64:
-// 85 us; one of 256: 11 us; 64 requests with 16 rows each over 151 to 2,064 slots: 27 us. A 256 x 128 tile of scores
-// takes 1.76 us at head_dim 64 (load and maximum 0.37, exponentials of both warpgroups 1.1, next S 0.25) and 2.25 at 128
-// (0.37, 0.83, then its own two products 0.55 and 0.45 to be told).
+// Measured: a prompt of 8,192 rows, 32 + 2 x 8 heads of 128, bf16: 488 us, 1,128 TFLOP/s (68% of cuBLAS at bf16); of 64:
+// 372 us, where the exponentials alone are 50% of the tensor rate. 16 prompts of 186 to 2,048 rows, 14 + 2 x 2 heads of 64:
+// 82 us; one of 256: 10.5 us; 64 requests with 16 rows each over 151 to 2,064 slots: 25 us. Calls of equal blocks of 2 to
+// 16 tiles, head_dim 64: 7.2 us + 4.8 a block of a CTA + 1.46 a 256 x 128 tile of scores; at 128: 9.5 + 5.5 + 2.0 to 2.3. Of a
+// tile in a traced run, 1.76 us at 64: load and maximum 0.37, exponentials of both warpgroups 1.1, next S 0.25; 2.25 at
+// 128: 0.37, 0.83, then its own two products 0.55 and 0.45 to be told.
 #pragma once
 #include "vp_paged_decode.cuh"
 
@@ -55,11 +56,12 @@ struct PfShape {
 
 constexpr int PF_RECORDS = 640;            // records at most: four per SM, for 160
 constexpr int PF_AHEAD = 3;                // tiles of slots before a piece's end that the next piece is taken (two pieces
-                                           // ahead: 4,096 rows 79 us instead of 62, as the CTAs no longer even out)
-constexpr int PF_SORT = 128;               // requests that are sorted by length, at most (16 prompts: 100 us unsorted, 90
+                                           // ahead: 4,096 rows 76 us instead of 60, as the CTAs no longer even out)
+constexpr int PF_SORT = 128;               // requests that are sorted by length, at most (16 prompts: 87 us unsorted, 82
                                            // sorted; the sort is n steps a thread, 0.5 us at 128)
-constexpr int PF_JOIN = 8;                 // records joined at a time (16 rows over 60,000 slots: 50 us, all 74 at once 68)
-constexpr int PF_LEAST = 16;               // tiles of a piece, at least (64 trees: 26.7 us; with 8, whose joins cost what they save: 28.3)
+constexpr int PF_JOIN = 8;                 // records joined at a time (16 rows over 60,000 slots, 14 + 2 x 2 heads of 64: 46 us, all 74 at once 64)
+constexpr int PF_LEAST = 16;               // tiles of a piece, at least (64 trees: 25.1 us, one over 2,000 slots 22.5; with 8, whose joins cost
+                                           // more than they save: 27.7 and 26.3, but 16 rows over 60,000 slots 42 instead of 46)
 
 struct PfParams {
   vp_paged c;

@@ -20,7 +20,7 @@ namespace vp {
 // One CTA per row, HD / 16 threads per head: each turns two runs of 8 elements (or copies 16), so a
 // thread keeps its 8 (cos, sin) pairs in registers over the heads it serves. 16-byte accesses. Bytes
 // bound it: each row is read and written once, 452 MB of 32 + 2 x 8 heads of 128 in 75 us (6.05 TB/s,
-// 93% of the measured copy), one row in 2.2 us. A call of more than APPEND_STREAM bytes cannot leave
+// 93% of the measured copy), one row in 2.1 us. A call of more than APPEND_STREAM bytes cannot leave
 // its rows in L2 for the attention behind it, so it marks them as passing through, in CTAs of two warps
 // (88 us with the accesses and CTAs of a small call, which in turn takes 3.4 us for 5 MB against 3.75).
 constexpr int APPEND_THREADS = 128;
@@ -163,8 +163,8 @@ int decode_launch(const vp_paged& c, const vp_paged_attn& a, cudaStream_t st) {
   p.a = a;
   p.group = a.n_q / c.n_kv;
   p.M = p.group * a.rows;
-  // a CTA's ring: all of it flies at once (one request of 257 slots: 6.2 us; 10.4 with half as many, which split its heads,
-  // 8.5 with twice as many; 64 requests of 130 to 2,048: 14.8, 14.8 and 17.6 in even shares of tiles)
+  // a CTA's ring: all of it flies at once (one request of 257 slots: 6.7 us; 7.6 with half as many, which cut its heads, 6.7
+  // with twice as many; 64 requests of 130 to 2,048, in even shares of tiles: 12.7, 12.7 and 15.2; 16 of 300: 7.3, 8.4, 7.3)
   p.min_tiles = DC_WARPS * DC_STAGES;
   p.page_shift = __builtin_ctz(c.page_size);
   p.tickets = static_cast<unsigned*>(a.work);
