@@ -39,6 +39,11 @@ def _extension():
     return _paged
 
 
+def _not_captured() -> None:
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise VpError("a layer cannot get its status or workspace while a graph is captured: only the replay would zero them")
+
+
 def _workspace(work: list, head_dim: int, device: torch.device) -> None:
     """work[0] becomes a workspace for every call over heads of this size, its counters zeroed: a call never allocates one, since
     a captured graph holds its address and would only record the zeroing. A smaller one that was there moves back in the
@@ -47,6 +52,7 @@ def _workspace(work: list, head_dim: int, device: torch.device) -> None:
     need = _lib.load().vp_paged_work_bytes(head_dim, 64, 1, MAX_ROWS)
     if work and work[0] is not None and work[0].nbytes >= need:
         return
+    _not_captured()
     new = torch.empty(max(need, WORK_ZEROED), dtype=torch.uint8, device=device)
     new[:WORK_ZEROED].zero_()
     work[:] = [new] + [w for w in work if w is not None]
@@ -88,9 +94,8 @@ class PagedLayer:
         _lib.load()
         self.k, self.v, self.table, self.device, self.dtype = k, v, table, k.device, k.dtype
         self.pages, self.n_kv, self.page_size, self.head_dim = k.shape
-        if torch.cuda.is_current_stream_capturing():
-            raise VpError("a layer cannot be built while a graph is captured: its workspace would only be zeroed by the replay")
         if status is None:
+            _not_captured()
             status = torch.zeros(1, dtype=torch.int32, device=k.device)
         self.status, self._work = status, [None] if work is None else work
         _workspace(self._work, self.head_dim, k.device)

@@ -872,6 +872,12 @@ def test_graph_outlives_larger_calls():
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             d + 1
             paged.PagedLayer(kv.k, kv.v, kv.table)
+    g2 = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g2):  # another view of the cache, on the status and workspace that are there
+        late = paged.PagedLayer(kv.k, kv.v, kv.table, kv.status, kv._work).decode(d, ln)
+    g2.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(late, eager[0])
 
 
 @pytest.mark.gpu
